@@ -6,7 +6,7 @@ and Python callers; it computes nothing itself and has no fallback.
 """
 from . import abi
 from .operator import (Backend, KvPool, Tensor, YvexError, attention_requirement, bf16_bits_to_f32,
-                       f32_to_bf16_bits)
+                       f32_to_bf16_bits, row_ranges)
 
 __all__ = ["abi", "Backend", "KvPool", "Tensor", "YvexError", "attention_requirement",
-           "bf16_bits_to_f32", "f32_to_bf16_bits"]
+           "bf16_bits_to_f32", "f32_to_bf16_bits", "row_ranges"]

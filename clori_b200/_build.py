@@ -33,8 +33,9 @@ CC_FLAGS = ["-std=c11", "-O2", "-fPIC", "-Wall", "-Wextra", "-D_GNU_SOURCE", "-I
 
 def _sources():
     cuda = sorted(f for f in os.listdir(os.path.join(CSRC, "cuda")) if f.endswith(".cu"))
-    host = sorted(f for f in os.listdir(os.path.join(CSRC, "host")) if f.endswith(".c"))
-    return [os.path.join(CSRC, "cuda", f) for f in cuda], [os.path.join(CSRC, "host", f) for f in host]
+    host = [os.path.join(CSRC, folder, f) for folder in ("host", os.path.join("host", "extension"))
+            for f in sorted(os.listdir(os.path.join(CSRC, folder))) if f.endswith(".c")]
+    return [os.path.join(CSRC, "cuda", f) for f in cuda], host
 
 
 def _headers():

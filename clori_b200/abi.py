@@ -39,6 +39,7 @@ NUMERIC_BF16_F32_ACCUMULATE = 2
 NUMERIC_Q8_0_KV_F32_ACCUMULATE = 3
 BACKEND_KIND_CPU, BACKEND_KIND_CUDA = 0, 1
 KV_CONTIGUOUS, KV_BLOCK_TABLE = 0, 1
+KV_PLAIN, KV_E4M3, KV_I8 = 0, 1, 2  # yvx_kv_code
 MAX_DIMS = 4
 u64 = C.c_ulonglong
 
@@ -143,6 +144,39 @@ class GqaProblem(C.Structure):
     ]
 
 
+class ScoredProblem(C.Structure):
+    """yvx_scored_problem (include/yvex_b200/cuda_shim.h)."""
+    _fields_ = [
+        ("sessions", C.c_uint), ("query_rows", C.c_uint), ("query_heads", C.c_uint), ("kv_heads", C.c_uint),
+        ("head_dim", C.c_uint), ("causal", C.c_uint), ("scale", C.c_float), ("cap", C.c_float), ("window", C.c_uint),
+        ("query_dtype", C.c_int), ("kv_dtype", C.c_int), ("output_dtype", C.c_int), ("kv_code", C.c_int),
+        ("query", C.c_void_p), ("query_row_stride", u64), ("query_session_stride", u64), ("query_head_stride", u64),
+        ("output", C.c_void_p), ("key", C.c_void_p), ("value", C.c_void_p),
+        ("key_token_stride", u64), ("value_token_stride", u64), ("key_head_stride", u64), ("value_head_stride", u64),
+        ("key_outer_stride", u64), ("value_outer_stride", u64),
+        ("key_scales", C.c_void_p), ("value_scales", C.c_void_p), ("scale_block_stride", u64),
+        ("block_table", C.c_void_p), ("block_tokens", C.c_uint), ("block_table_stride", C.c_uint),
+        ("pool_blocks", C.c_uint), ("kv_tokens", C.c_void_p), ("kv_tokens_uniform", C.c_uint),
+        ("kv_tokens_max", C.c_uint), ("query_start", C.c_void_p), ("query_start_uniform", C.c_uint),
+        ("query_start_from_end", C.c_uint), ("row_first", C.c_void_p), ("row_end", C.c_void_p),
+        ("slopes", C.c_void_p), ("chunk_tokens", C.c_uint), ("max_splits", C.c_uint),
+        ("workspace", C.c_void_p), ("workspace_bytes", u64), ("status", C.c_void_p), ("force_general", C.c_int),
+    ]
+
+
+class Kv8AppendArgs(C.Structure):
+    """yvx_kv8_append_args (include/yvex_b200/cuda_shim.h)."""
+    _fields_ = [
+        ("sessions", C.c_uint), ("tokens", C.c_uint), ("kv_heads", C.c_uint), ("head_dim", C.c_uint),
+        ("code", C.c_int), ("dtype", C.c_int), ("key", C.c_void_p), ("value", C.c_void_p),
+        ("token_stride", u64), ("session_stride", u64), ("kv_tokens", C.c_void_p), ("kv_tokens_uniform", C.c_uint),
+        ("new_tokens", C.c_void_p), ("block_table", C.c_void_p), ("block_tokens", C.c_uint),
+        ("block_table_stride", C.c_uint), ("pool_blocks", C.c_uint), ("key_codes", C.c_void_p),
+        ("value_codes", C.c_void_p), ("code_token_stride", u64), ("code_head_stride", u64), ("code_block_stride", u64),
+        ("key_scales", C.c_void_p), ("value_scales", C.c_void_p), ("scale_block_stride", u64), ("status", C.c_void_p),
+    ]
+
+
 class LatentReduceArgs(C.Structure):
     """yvx_latent_reduce_args (include/yvex_b200/cuda_shim.h); the CPU checker's argument
     struct has the same layout."""
@@ -170,6 +204,48 @@ class KvCopy(C.Structure):
     """yvex_b200_kv_copy (include/yvex_b200/attention.h)."""
     _fields_ = [("needed", C.c_int), ("source_block", C.c_int), ("destination_block", C.c_int),
                 ("rows", C.c_uint)]
+
+
+class KvPagePool(C.Structure):
+    """yvx_kv_page_pool (include/yvex_b200/cuda_shim.h)."""
+    _fields_ = [("base", C.c_void_p), ("block_stride", u64), ("segment_stride", u64), ("row_bytes", u64),
+                ("fixed_bytes", u64), ("blocks", C.c_uint), ("segments", C.c_uint)]
+
+
+class KvPagesArgs(C.Structure):
+    """yvx_kv_pages_args (include/yvex_b200/cuda_shim.h); the copies are KvCopy records."""
+    _fields_ = [("pools", C.POINTER(KvPagePool)), ("copies", C.POINTER(KvCopy)), ("pool_count", C.c_uint),
+                ("copy_count", C.c_uint), ("block_tokens", C.c_uint)]
+
+
+class KvPagesPool(C.Structure):
+    """yvex_b200_kv_pages_pool (include/yvex_b200/attention.h)."""
+    _fields_ = [("tensor", C.c_void_p), ("segments", u64), ("whole", C.c_int)]
+
+
+class AttentionScoredRequest(C.Structure):
+    """yvex_b200_attention_scored_request (include/yvex_b200/attention.h)."""
+    _fields_ = [
+        ("session_count", u64), ("query_tokens", u64), ("query_heads", u64), ("key_value_heads", u64),
+        ("head_dimension", u64), ("key_value_tokens", u64), ("causal", C.c_int), ("scale", C.c_float),
+        ("score_cap", C.c_float), ("window", u64), ("kv_code", C.c_int), ("kv_layout", C.c_int),
+        ("query", C.c_void_p), ("key", C.c_void_p), ("value", C.c_void_p), ("key_scales", C.c_void_p),
+        ("value_scales", C.c_void_p), ("kv_tokens", C.c_void_p), ("query_start", C.c_void_p), ("block_table", C.c_void_p),
+        ("block_tokens", u64), ("max_blocks_per_session", u64), ("row_first", C.c_void_p), ("row_end", C.c_void_p),
+        ("slopes", C.c_void_p), ("query_token_stride", u64), ("kv_token_stride", u64), ("kv_head_stride", u64),
+        ("kv_outer_stride", u64), ("output", C.c_void_p),
+    ]
+
+
+class Kv8AppendRequest(C.Structure):
+    """yvex_b200_kv8_append_request (include/yvex_b200/attention.h)."""
+    _fields_ = [
+        ("session_count", u64), ("token_count", u64), ("key_value_heads", u64), ("head_dimension", u64),
+        ("kv_code", C.c_int), ("key", C.c_void_p), ("value", C.c_void_p), ("token_stride", u64), ("session_stride", u64),
+        ("kv_tokens", C.c_void_p), ("max_kv_tokens", u64), ("new_tokens", C.c_void_p), ("block_table", C.c_void_p),
+        ("block_tokens", u64), ("max_blocks_per_session", u64), ("key_codes", C.c_void_p), ("value_codes", C.c_void_p),
+        ("key_scales", C.c_void_p), ("value_scales", C.c_void_p),
+    ]
 
 
 class AttentionFailure(C.Structure):
@@ -534,8 +610,12 @@ EXPORTED_SYMBOLS = [
     "yvex_b200_kv_pool_commit", "yvex_b200_kv_pool_table", "yvex_b200_kv_pool_committed",
     "yvex_b200_kv_pool_reserved", "yvex_b200_kv_pool_free_blocks", "yvex_b200_kv_pool_block_refcount",
     "yvex_b200_kv_page_tokens", "yvex_b200_kv_page_touch", "yvex_b200_kv_block_row",
-    "yvex_b200_kv_sequence_shard",
+    "yvex_b200_kv_sequence_shard", "yvex_b200_kv_pool_session_truncate", "yvex_b200_kv_pool_compact",
+    "yvex_b200_kv_pages_copy_execute", "yvex_b200_attention_scored_execute", "yvex_b200_attention_row_ranges",
+    "yvex_b200_kv8_append_execute",
     # cuda_shim.h
+    "yvx_cuda_scored_plan", "yvx_cuda_scored_workspace_bytes", "yvx_cuda_scored_attention", "yvx_cuda_kv8_append",
+    "yvx_cuda_kv_pages_copy",
     "yvx_cuda_device_count", "yvx_cuda_device_select", "yvx_cuda_device_properties",
     "yvx_cuda_malloc", "yvx_cuda_free", "yvx_cuda_host_alloc", "yvx_cuda_host_free",
     "yvx_cuda_memset_async", "yvx_cuda_upload_async", "yvx_cuda_download_async",
@@ -710,6 +790,20 @@ def load():
     lib.yvx_cuda_gqa_partials_bytes.argtypes = [P(GqaProblem)]
     lib.yvx_cuda_gqa_plan_splits.restype = None
     lib.yvx_cuda_gqa_plan_splits.argtypes = [P(GqaProblem), C.c_int]
+    lib.yvx_cuda_scored_plan.restype = None
+    lib.yvx_cuda_scored_plan.argtypes = [P(ScoredProblem), C.c_int]
+    lib.yvx_cuda_scored_workspace_bytes.restype = u64
+    lib.yvx_cuda_scored_workspace_bytes.argtypes = [P(ScoredProblem)]
+    lib.yvx_cuda_scored_attention.argtypes = [P(ScoredProblem), vp, P(C.c_uint)]
+    lib.yvx_cuda_kv8_append.argtypes = [P(Kv8AppendArgs), vp]
+    lib.yvx_cuda_kv_pages_copy.argtypes = [P(KvPagesArgs), vp, P(C.c_uint)]
+    lib.yvex_b200_attention_scored_execute.argtypes = [vp, P(AttentionScoredRequest), P(OperationFacts), P(Error)]
+    lib.yvex_b200_attention_row_ranges.argtypes = [P(u64), P(u64), u64, u64, u64, P(C.c_int), P(C.c_int)]
+    lib.yvex_b200_kv8_append_execute.argtypes = [vp, P(Kv8AppendRequest), P(OperationFacts), P(Error)]
+    lib.yvex_b200_kv_pages_copy_execute.argtypes = [vp, P(KvPagesPool), C.c_uint, P(KvCopy), C.c_uint, u64,
+                                                    P(OperationFacts), P(Error)]
+    lib.yvex_b200_kv_pool_session_truncate.argtypes = [vp, C.c_uint, u64]
+    lib.yvex_b200_kv_pool_compact.argtypes = [vp, P(KvCopy), C.c_uint, P(C.c_uint)]
     lib.yvx_cuda_gqa_attention.argtypes = [P(GqaProblem), vp, P(C.c_uint)]
     lib.yvx_cuda_gqa_attention_profiled.argtypes = [P(GqaProblem), vp, vp * 3, P(C.c_uint)]
     lib.yvx_cuda_fill_normal.argtypes = [vp, C.c_int, u64, u64, C.c_float, vp]

@@ -1,0 +1,105 @@
+// Checks, kernel selection and split planning of scored attention.
+#include "scored.cuh"
+
+namespace yvx {
+
+static int scored_refuse(int code, const char *text)
+{
+    yvx_cuda_set_error_text(text);
+    return code;
+}
+
+static int scored_check(const yvx_scored_problem *p)
+{
+    if (!p || !p->query || !p->output || !p->key || !p->value || !p->status)
+        return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: query, output, key, value and status are required");
+    if (!p->sessions || !p->query_rows || !p->query_heads || !p->kv_heads || !p->head_dim ||
+        p->query_heads % p->kv_heads || !p->kv_tokens_max || (!p->kv_tokens && p->kv_tokens_uniform > p->kv_tokens_max) ||
+        !(p->scale > 0.0f) || !isfinite(p->scale) || !(p->cap >= 0.0f) || !isfinite(p->cap))
+        return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: inconsistent geometry, scale or cap");
+    if (p->head_dim > 256u || (p->query_dtype != YVEX_DTYPE_F32 && p->query_dtype != YVEX_DTYPE_BF16) ||
+        (p->output_dtype != YVEX_DTYPE_F32 && p->output_dtype != YVEX_DTYPE_BF16) || p->kv_code < YVX_KV_PLAIN ||
+        p->kv_code > YVX_KV_I8 ||
+        (p->kv_code == YVX_KV_PLAIN && p->kv_dtype != YVEX_DTYPE_F32 && p->kv_dtype != YVEX_DTYPE_BF16))
+        return scored_refuse(YVEX_ERR_UNSUPPORTED, "scored attention: head_dim above 256 or a type it does not read");
+    if (p->kv_code != YVX_KV_PLAIN && (!p->block_table || !p->key_scales || !p->value_scales))
+        return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: codes need a block table and scales");
+    if (p->block_table && (!p->block_tokens || !p->pool_blocks || p->pool_blocks > 0x7fffffffu ||
+                           (unsigned long long)p->block_table_stride * p->block_tokens < p->kv_tokens_max))
+        return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: the block table does not cover kv_tokens_max");
+    if (!p->chunk_tokens || (p->chunk_tokens & 63u) || !p->max_splits)
+        return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: yvx_cuda_scored_plan has not been called");
+    if (p->kv_tokens_max > 0x7fffffffu - 1024u || p->sessions > 65535u || p->max_splits > 65535u)
+        return scored_refuse(YVEX_ERR_BOUNDS, "scored attention: lengths below 2^31 - 1024, at most 65535 sessions and splits");
+    return 0;
+}
+
+// Tokens a call's rows can see, as far as the host knows: a causal window bounds them.
+static unsigned long long scored_span(const yvx_scored_problem *p)
+{
+    const unsigned long long all = ((unsigned long long)p->kv_tokens_max + 63ull) / 64ull * 64ull;
+    if (!p->window || !p->causal || p->row_end) return all;
+    const unsigned long long seen = (unsigned long long)p->window + p->query_rows + 62ull;
+    return seen < all ? (seen + 63ull) / 64ull * 64ull : all;
+}
+
+}  // namespace yvx
+
+extern "C" {
+
+// Splits fill the machine: two CTAs of the split kernels run on an SM, so a wave is 2 * sm_count
+// items. The chunk is the largest multiple of 64 tokens, at most 4096, whose items fill their
+// last wave to 90 %; else the best-filled one with at least a wave; else 64.
+void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
+{
+    if (!p || !p->kv_heads || !p->query_rows || !p->kv_tokens_max) return;
+    const unsigned long long wave = 2ull * (unsigned long long)(sm_count > 0 ? sm_count : 148);
+    const unsigned long long vectors = (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads);
+    const unsigned long long span = yvx::scored_span(p);
+    const unsigned long long lanes = (unsigned long long)p->sessions * p->kv_heads * ((vectors + 15ull) / 16ull);
+    unsigned int best = 64u;
+    double best_fill = -1.0;
+    for (unsigned int chunk = 4096u; chunk >= 64u; chunk -= 64u) {
+        const unsigned long long items = lanes * ((span + chunk - 1ull) / chunk);
+        if (items < wave) continue;
+        const double fill = (double)items / (double)((items + wave - 1ull) / wave * wave);
+        if (fill > best_fill) {
+            best_fill = fill;
+            best = chunk;
+        }
+        if (fill >= 0.9) break;
+    }
+    while ((span + best - 1ull) / best > 65535ull) best += 64u;
+    if (lanes >= wave && vectors > 64ull) best = (unsigned int)span;  // many rows fill the machine by themselves
+    p->chunk_tokens = best;
+    p->max_splits = (unsigned int)((span + best - 1ull) / best);
+}
+
+unsigned long long yvx_cuda_scored_workspace_bytes(const yvx_scored_problem *p)
+{
+    if (!p || p->max_splits <= 1u) return 0ull;
+    return (unsigned long long)p->sessions * p->query_rows * p->query_heads * p->max_splits * (p->head_dim + 4ull) * 4ull;
+}
+
+int yvx_cuda_scored_attention(const yvx_scored_problem *p, void *stream, unsigned int *launches)
+{
+    if (launches) *launches = 0u;
+    int rc = yvx::scored_check(p);
+    if (rc != 0) return rc;
+    const unsigned long long needed = yvx_cuda_scored_workspace_bytes(p);
+    if (needed && (!p->workspace || p->workspace_bytes < needed || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)))
+        return yvx::scored_refuse(YVEX_ERR_BOUNDS, "scored attention: the workspace is missing, misaligned or too small");
+    cudaStream_t s = (cudaStream_t)stream;
+    rc = yvx::scored_general_launch(*p, s);
+    if (rc != 0) return rc;
+    unsigned int count = 1u;
+    if (p->max_splits > 1u) {
+        rc = yvx::scored_combine_launch(*p, s);
+        if (rc != 0) return rc;
+        ++count;
+    }
+    if (launches) *launches = count;
+    return 0;
+}
+
+}  // extern "C"

@@ -210,6 +210,14 @@ int yvx_backend_status_arm(yvex_backend *backend, const char *where, yvex_error 
     return YVEX_OK;
 }
 
+int yvx_backend_status_join(yvex_backend *backend, const char *where, yvex_error *err)
+{
+    if (backend->synchronous || !backend->status_pending) return yvx_backend_status_arm(backend, where, err);
+    if (injected_failure("YVEX_B200_TEST_LAUNCH_FAILURE", where))
+        return inject(backend, "injected launch failure (test hook)", where, err);
+    return YVEX_OK;
+}
+
 int yvx_backend_status_collect(yvex_backend *backend, yvex_backend_operation_facts *facts,
                                const char *where, yvex_error *err)
 {

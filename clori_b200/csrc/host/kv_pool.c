@@ -205,6 +205,57 @@ int yvex_b200_kv_pool_commit(yvex_b200_kv_pool *pool, unsigned int session, unsi
     return YVEX_OK;
 }
 
+int yvex_b200_kv_pool_session_truncate(yvex_b200_kv_pool *pool, unsigned int session, unsigned long long rows)
+{
+    unsigned int j;
+    int *row;
+    if (!session_ok(pool, session)) return YVEX_ERR_INVALID_ARG;
+    if (rows > pool->committed[session]) return YVEX_ERR_BOUNDS;
+    pool->committed[session] = pool->reserved[session] = rows;
+    row = pool->table + (size_t)session * pool->max_blocks_per_session;
+    for (j = blocks_for(pool, rows); j < pool->max_blocks_per_session; ++j) {
+        release_block(pool, row[j]);
+        row[j] = -1;
+    }
+    return YVEX_OK;
+}
+
+/* The n blocks in use end as [0, n): the used blocks at or behind n and the free ones in front of it are
+ * equally many, and the i-th of one goes to the i-th of the other. */
+int yvex_b200_kv_pool_compact(yvex_b200_kv_pool *pool, yvex_b200_kv_copy *copies, unsigned int capacity,
+                              unsigned int *count)
+{
+    unsigned int used, moves = 0u, hole = 0u, block;
+    size_t cell;
+    int *moved_to;
+    if (!pool || !count || (capacity && !copies)) return YVEX_ERR_INVALID_ARG;
+    used = pool->blocks - pool->free_count;
+    for (block = used; block < pool->blocks; ++block) moves += pool->refcount[block] != 0u;
+    *count = moves;
+    if (moves > capacity) return YVEX_ERR_BOUNDS;
+    if (moves) {
+        moved_to = (int *)malloc(sizeof(int) * (pool->blocks - used));
+        if (!moved_to) return YVEX_ERR_NOMEM;
+        moves = 0u;
+        for (block = used; block < pool->blocks; ++block) {
+            if (!pool->refcount[block]) continue;
+            while (pool->refcount[hole]) ++hole;
+            copies[moves].needed = 1;
+            copies[moves].source_block = (int)block;
+            copies[moves].destination_block = (int)hole;
+            copies[moves++].rows = pool->block_tokens;
+            pool->refcount[hole] = pool->refcount[block];
+            pool->refcount[block] = 0u;
+            moved_to[block - used] = (int)hole;
+        }
+        for (cell = 0; cell < (size_t)pool->max_sessions * pool->max_blocks_per_session; ++cell)
+            if (pool->table[cell] >= (int)used) pool->table[cell] = moved_to[pool->table[cell] - (int)used];
+        free(moved_to);
+    }
+    for (block = 0; block < pool->free_count; ++block) pool->free_list[block] = pool->blocks - 1u - block;
+    return YVEX_OK;
+}
+
 const int *yvex_b200_kv_pool_table(const yvex_b200_kv_pool *pool, unsigned int session)
 {
     return session_ok(pool, session) ? pool->table + (size_t)session * pool->max_blocks_per_session : NULL;

@@ -81,6 +81,10 @@ int yvx_backend_device_fail(yvex_backend *backend, int rc, const char *where, yv
 /* Clears the status word before an operator and reads it back after: returns
  * YVEX_ERR_FORMAT when a kernel published a non-finite or contract failure. */
 int yvx_backend_status_arm(yvex_backend *backend, const char *where, yvex_error *err);
+/* The same for operators that may be enqueued one behind another: on an asynchronous backend whose status
+ * word already waits to be read, the word is left as it is (its first failure stays) and nothing is
+ * synchronised. */
+int yvx_backend_status_join(yvex_backend *backend, const char *where, yvex_error *err);
 int yvx_backend_status_collect(yvex_backend *backend, yvex_backend_operation_facts *facts,
                                const char *where, yvex_error *err);
 int yvx_tensor_owned(const yvex_backend *backend, const yvex_device_tensor *tensor);

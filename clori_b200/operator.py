@@ -58,6 +58,18 @@ def attention_requirement(query_tokens, key_value_tokens, query_start, query_hea
     return r
 
 
+def row_ranges(document_lengths, rows, query_start=0, prefix_lengths=None):
+    """yvex_b200_attention_row_ranges: (row_first, row_end) int32 arrays of `rows` query rows over documents laid
+    end to end, each with a bidirectional prefix."""
+    lengths = (abi.u64 * max(1, len(document_lengths)))(*document_lengths)
+    prefixes = (abi.u64 * max(1, len(document_lengths)))(*prefix_lengths) if prefix_lengths is not None else None
+    first, end = (C.c_int * max(1, rows))(), (C.c_int * max(1, rows))()
+    if not abi.load().yvex_b200_attention_row_ranges(lengths, prefixes, len(document_lengths), query_start, rows,
+                                                     first, end):
+        raise ValueError("bad documents or rows")
+    return np.array(first, np.int32), np.array(end, np.int32)
+
+
 _NP_DTYPES = {abi.DTYPE_F32: np.float32, abi.DTYPE_BF16: np.uint16, abi.DTYPE_F16: np.uint16,
               abi.DTYPE_I32: np.int32, abi.DTYPE_I8: np.int8, abi.DTYPE_I64: np.int64,
               abi.DTYPE_F64: np.float64}
@@ -262,6 +274,57 @@ class Backend:
             _raise(err)
         return rc, facts
 
+    def _extension(self, function, request, fields, check):
+        """Fill a request from keyword fields (Tensors become pointers, None stays NULL) and call it."""
+        for name, value in fields.items():
+            setattr(request, name, C.cast(value.ptr, C.c_void_p) if isinstance(value, Tensor) else value)
+        facts, err = abi.OperationFacts(), abi.Error()
+        rc = function(self.handle, C.byref(request), C.byref(facts), C.byref(err))
+        if rc and check:
+            _raise(err)
+        return rc, facts
+
+    def attention_scored(self, query, key, value, kv_tokens, output, *, kv_heads, head_dim, max_kv_tokens,
+                         causal=True, scale=0.0, score_cap=0.0, block_table=None, check=True, **fields):
+        """yvex_b200_attention_scored_execute over a query [sessions, rows, heads*head_dim]: capped scores
+        (score_cap), distance bias (slopes), window, row_first / row_end, pages (block_table, block_tokens) and
+        8-bit codes (kv_code, key_scales, value_scales). Other fields as in yvex_b200_attention_scored_request."""
+        fields = {"session_count": query.shape[0], "query_tokens": query.shape[1],
+                  "query_heads": output.shape[2] // head_dim, "key_value_heads": kv_heads, "head_dimension": head_dim,
+                  "key_value_tokens": max_kv_tokens, "causal": int(causal), "scale": scale, "score_cap": score_cap,
+                  "query": query, "key": key, "value": value, "kv_tokens": kv_tokens, "output": output, **fields}
+        if block_table is not None:
+            fields = {"kv_layout": abi.KV_BLOCK_TABLE, "block_table": block_table,
+                      "max_blocks_per_session": block_table.shape[1], **fields}
+        return self._extension(self.lib.yvex_b200_attention_scored_execute, abi.AttentionScoredRequest(),
+                               {k: v for k, v in fields.items() if v is not None}, check)
+
+    def kv8_append(self, key, value, key_codes, value_codes, key_scales, value_scales, block_table, *, kv_code,
+                   max_kv_tokens, kv_tokens=None, new_tokens=None, check=True, **fields):
+        """yvex_b200_kv8_append_execute: rows [sessions, tokens, kv_heads*head_dim] into pages of codes
+        [page, kv_heads, block_tokens, head_dim] with scales [page, kv_heads]."""
+        fields = {"session_count": key.shape[0], "token_count": key.shape[1], "key_value_heads": key_codes.shape[1],
+                  "head_dimension": key_codes.shape[3], "kv_code": kv_code, "key": key, "value": value,
+                  "kv_tokens": kv_tokens, "max_kv_tokens": max_kv_tokens, "new_tokens": new_tokens,
+                  "block_table": block_table, "block_tokens": key_codes.shape[2],
+                  "max_blocks_per_session": block_table.shape[1], "key_codes": key_codes, "value_codes": value_codes,
+                  "key_scales": key_scales, "value_scales": value_scales, **fields}
+        return self._extension(self.lib.yvex_b200_kv8_append_execute, abi.Kv8AppendRequest(),
+                               {k: v for k, v in fields.items() if v is not None}, check)
+
+    def kv_pages_copy(self, pools, copies, block_tokens, check=True):
+        """yvex_b200_kv_pages_copy_execute. pools: (tensor, segments) for rows, (tensor, None) for pages copied
+        whole; copies: (source, destination, rows) triples as KvPool.reserve and KvPool.compact return them."""
+        described = (abi.KvPagesPool * max(1, len(pools)))(
+            *[abi.KvPagesPool(C.cast(t.ptr, C.c_void_p), s or 1, int(s is None)) for t, s in pools])
+        listed = (abi.KvCopy * max(1, len(copies)))(*[abi.KvCopy(1, *copy) for copy in copies])
+        facts, err = abi.OperationFacts(), abi.Error()
+        rc = self.lib.yvex_b200_kv_pages_copy_execute(self.handle, described, len(pools), listed, len(copies),
+                                                      block_tokens, C.byref(facts), C.byref(err))
+        if rc and check:
+            _raise(err)
+        return rc, facts
+
     def mla_decode(self, q_nope, q_rope, w_uk, latent, rope_key, output, *, max_kv_tokens, scale,
                    kv_tokens=None, check=True):
         """yvex_b200_mla_decode_execute: bf16 tensors [sessions, 128, 128 | 64], [128, 128, 512],
@@ -401,6 +464,20 @@ class KvPool:
 
     def commit(self, session, accepted):
         self._check(self.lib.yvex_b200_kv_pool_commit(self.handle, session, accepted))
+
+    def truncate(self, session, rows):
+        """Forget the session's rows from `rows` on and free the blocks behind them."""
+        self._check(self.lib.yvex_b200_kv_pool_session_truncate(self.handle, session, rows))
+
+    def compact(self):
+        """Move the blocks in use to the front; returns the (source_block, destination_block, rows) copies to make
+        in every layer's pools before a table is used again."""
+        count = C.c_uint()
+        if self.lib.yvex_b200_kv_pool_compact(self.handle, None, 0, C.byref(count)) == 0:
+            return []
+        copies = (abi.KvCopy * count.value)()
+        self._check(self.lib.yvex_b200_kv_pool_compact(self.handle, copies, count.value, C.byref(count)))
+        return [(c.source_block, c.destination_block, c.rows) for c in copies]
 
     def table(self, session):
         row = self.lib.yvex_b200_kv_pool_table(self.handle, session)

@@ -139,6 +139,74 @@ int yvex_b200_attention_batch_execute(yvex_backend *backend,
                                       const yvex_b200_attention_batch_request *request,
                                       yvex_backend_operation_facts *facts, yvex_error *err);
 
+/* ---- scored attention (extension) --------------------------------------------
+ * Grouped-query attention with capped scores, a bias that depends on distance, a sliding
+ * window and a run of visible tokens for each row (packed documents, padding, bidirectional
+ * prefixes), over F32 / bf16 rows or over pages of 8-bit codes. The mathematics, the layouts
+ * and what masked places may hold stand at yvx_scored_problem (yvex_b200/cuda_shim.h). No
+ * counterpart in the reference. Refusals: missing tensors, inconsistent geometry ->
+ * YVEX_ERR_INVALID_ARG; types, head_dimension above 256, unknown layouts ->
+ * YVEX_ERR_UNSUPPORTED; views that do not hold the declared geometry -> YVEX_ERR_FORMAT;
+ * sizes beyond the launch limits -> YVEX_ERR_BOUNDS.
+ * On a backend bound asynchronously (yvex_b200_backend_bind_stream with synchronous = 0) this
+ * operator, yvex_b200_kv8_append_execute and yvex_b200_kv_pages_copy_execute enqueue without
+ * reading the status word back: a failure of any of them is reported by yvex_backend_sync.
+ * Operators of one backend share its scratch: calls on several streams are ordered by the
+ * caller. */
+typedef struct yvex_b200_attention_scored_request {
+    unsigned long long session_count, query_tokens, query_heads, key_value_heads, head_dimension;
+    unsigned long long key_value_tokens;   /* the longest session */
+    int causal;
+    float scale, score_cap;                /* 0: 1 / sqrt(head_dimension); 0: no cap */
+    unsigned long long window;             /* 0: none */
+    int kv_code;                           /* 0: key / value are F32 or BF16; 1 e4m3, 2 integer codes (I8 tensors) */
+    yvex_b200_kv_layout kv_layout;         /* codes: YVEX_B200_KV_BLOCK_TABLE */
+    const yvex_device_tensor *query;       /* F32 / BF16 [session][row][query_heads*head_dim] */
+    const yvex_device_tensor *key, *value;
+    const yvex_device_tensor *key_scales, *value_scales; /* F32 [page][kv_heads]; codes only */
+    const yvex_device_tensor *kv_tokens;   /* I32 [session] */
+    const yvex_device_tensor *query_start; /* I32 [session] position of each session's first row;
+                                              NULL: the rows are the session's last */
+    const yvex_device_tensor *block_table; /* I32 [session][max_blocks_per_session] */
+    unsigned long long block_tokens, max_blocks_per_session;
+    const yvex_device_tensor *row_first, *row_end; /* I32 [session][row] or NULL */
+    const yvex_device_tensor *slopes;      /* F32 [query_heads] or NULL */
+    /* element strides (bytes for codes); 0: packed. Rows are [token][head][dim], pages of codes
+     * [head][token][dim]; kv_outer_stride is between sessions or pages and has no default for
+     * more than one contiguous session */
+    unsigned long long query_token_stride, kv_token_stride, kv_head_stride, kv_outer_stride;
+    yvex_device_tensor *output;            /* F32 / BF16 [session][row][query_heads*head_dim] */
+} yvex_b200_attention_scored_request;
+int yvex_b200_attention_scored_execute(yvex_backend *backend, const yvex_b200_attention_scored_request *request,
+                                       yvex_backend_operation_facts *facts, yvex_error *err);
+/* The runs of visible tokens of `rows` query rows, the first at position query_start, in a sequence of
+ * documents laid end to end from token 0: a row sees its own document up to itself and all of the
+ * document's first prefix_lengths[d] tokens (NULL: no prefixes). Rows behind the last document are padding
+ * and see nothing. One document with a prefix is a prefix mask. Host arithmetic; returns 1, or 0 on bad
+ * arguments or positions beyond 2^31 - 1024. */
+int yvex_b200_attention_row_ranges(const unsigned long long *document_lengths, const unsigned long long *prefix_lengths,
+                                   unsigned long long documents, unsigned long long query_start,
+                                   unsigned long long rows, int *row_first, int *row_end);
+
+/* New rows into a cache of 8-bit codes (yvx_cuda_kv8_append, where scales and rounding are described).
+ * Pages are I8 [page][kv_heads][block_tokens][head_dimension], scales F32 [page][kv_heads]. Refusals:
+ * YVEX_ERR_INVALID_ARG, YVEX_ERR_UNSUPPORTED, YVEX_ERR_FORMAT as above; rows that the block table cannot
+ * hold -> YVEX_ERR_BOUNDS. */
+typedef struct yvex_b200_kv8_append_request {
+    unsigned long long session_count, token_count, key_value_heads, head_dimension;
+    int kv_code;                                      /* 1 e4m3, 2 integer codes */
+    const yvex_device_tensor *key, *value;            /* F32 / BF16 [session][token][kv_heads*hd] */
+    unsigned long long token_stride, session_stride;  /* elements; 0: packed */
+    const yvex_device_tensor *kv_tokens;              /* I32 [session] rows present; NULL: max_kv_tokens for all */
+    unsigned long long max_kv_tokens;                 /* upper bound of every session's rows present */
+    const yvex_device_tensor *new_tokens;             /* I32 [session]; NULL: token_count for all */
+    const yvex_device_tensor *block_table;            /* I32 [session][max_blocks_per_session] */
+    unsigned long long block_tokens, max_blocks_per_session;
+    yvex_device_tensor *key_codes, *value_codes, *key_scales, *value_scales;
+} yvex_b200_kv8_append_request;
+int yvex_b200_kv8_append_execute(yvex_backend *backend, const yvex_b200_kv8_append_request *request,
+                                 yvex_backend_operation_facts *facts, yvex_error *err);
+
 /* ---- latent attention: the reduce stage of the encoded attention job ---------
  * The reference reaches this stage inside yvex_backend_attention_execute
  * (include/yvex/internal/backend.h:193-195; src/backend/cuda/attention.c:1386-1422).
@@ -423,11 +491,35 @@ int yvex_b200_kv_pool_session_close(yvex_b200_kv_pool *pool, unsigned int sessio
 int yvex_b200_kv_pool_reserve(yvex_b200_kv_pool *pool, unsigned int session, unsigned int new_rows,
                               yvex_b200_kv_copy *copy);
 int yvex_b200_kv_pool_commit(yvex_b200_kv_pool *pool, unsigned int session, unsigned int accepted_rows);
+/* Forgets the session's rows from `rows` on (candidates too) and frees the blocks behind them: a
+ * conversation taken back to an earlier turn. YVEX_ERR_BOUNDS beyond the committed rows. */
+int yvex_b200_kv_pool_session_truncate(yvex_b200_kv_pool *pool, unsigned int session, unsigned long long rows);
+/* Moves the blocks in use to the front: afterwards they are [0, blocks in use), every session's table says
+ * so, and the pools may be cut or handed back behind them. `copies` receives the whole-block copies that
+ * the caller makes in every layer's pools (yvex_b200_kv_pages_copy_execute) before it uses a table again;
+ * no copy's source or destination is another's destination. *count is their number; when `capacity` is too
+ * small it still is, nothing changes, and the call is YVEX_ERR_BOUNDS. */
+int yvex_b200_kv_pool_compact(yvex_b200_kv_pool *pool, yvex_b200_kv_copy *copies, unsigned int capacity,
+                              unsigned int *count);
 const int *yvex_b200_kv_pool_table(const yvex_b200_kv_pool *pool, unsigned int session);
 unsigned long long yvex_b200_kv_pool_committed(const yvex_b200_kv_pool *pool, unsigned int session);
 unsigned long long yvex_b200_kv_pool_reserved(const yvex_b200_kv_pool *pool, unsigned int session);
 unsigned int yvex_b200_kv_pool_free_blocks(const yvex_b200_kv_pool *pool);
 unsigned int yvex_b200_kv_pool_block_refcount(const yvex_b200_kv_pool *pool, unsigned int block);
+/* The copies of a reserve, a fork or a compaction, made in several pools at once (every layer's K and V,
+ * codes and their scales): yvx_cuda_kv_pages_copy. A pool tensor's first dimension counts its blocks; a
+ * block is `segments` runs of block_tokens rows (1 for [token][head][dim], kv_heads for
+ * [head][token][dim]), or is copied whole whatever a copy's rows (scales). A destination that is the source
+ * or destination of another copy is YVEX_ERR_INVALID_ARG. Lists are read before the call returns. */
+typedef struct {
+    yvex_device_tensor *tensor;
+    unsigned long long segments;
+    int whole;
+} yvex_b200_kv_pages_pool;
+int yvex_b200_kv_pages_copy_execute(yvex_backend *backend, const yvex_b200_kv_pages_pool *pools,
+                                    unsigned int pool_count, const yvex_b200_kv_copy *copies,
+                                    unsigned int copy_count, unsigned long long block_tokens,
+                                    yvex_backend_operation_facts *facts, yvex_error *err);
 unsigned long long yvex_b200_kv_block_row(const int *block_table,
                                           unsigned long long block_tokens,
                                           unsigned long long row);

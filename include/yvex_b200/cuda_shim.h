@@ -157,6 +157,131 @@ int yvx_cuda_gqa_attention(const yvx_gqa_problem *problem, void *stream,
 int yvx_cuda_gqa_attention_profiled(const yvx_gqa_problem *problem, void *stream,
                                     void *events[3], unsigned int *launches);
 
+/* ---- scored attention over plain or 8-bit KV caches ---------------------------
+ * Grouped-query attention whose scores are more than a scaled product, over rows of F32 or
+ * bf16 (strided, or pages behind a block table) or over pages of 8-bit codes. The reference
+ * has none of this (its exact operator admits one score and two masks,
+ * src/backend/cuda/exact_attention.c:35-53); the semantics beyond that are those of
+ * yvx_gqa_problem above.
+ *
+ *   z         = scale * Q[b,t,h,:] . K[b,s,h/g,:]
+ *   z         = cap * tanh(z / cap)                       when cap > 0
+ *   z        -= slopes[h] * |position(t) - s|             when slopes are given
+ *   O[b,t,h,:] = softmax over the visible s of z, times V[b,s,h/g,:]
+ *
+ * position(t) = query_start[b] + t. Row t sees the tokens s of [first, end) with
+ *   first = max(row_first[b][t], position(t) + 1 - window)    (0 without either)
+ *   end   = row_end[b][t], else position(t) + 1 when causal, else the session's length
+ * both clipped to [0, kv_tokens[b]]. Packed documents, padding, bidirectional prefixes and
+ * any other mask whose rows see one run of tokens are such arrays
+ * (yvex_b200_attention_row_ranges writes the usual ones). A row that sees nothing is written
+ * as zeros, and what lies in K and V where no row looks (beyond a session's length, in the
+ * rest of a page, in padding) may be anything, NaN included. A NaN or infinity that a row
+ * does see is reported in the status word (1).
+ *
+ * kv_code != YVX_KV_PLAIN: key and value are 8-bit codes in pages (block_table is required;
+ * strides are in bytes) and a lane stands for code * scale, with one float scale for each
+ * page and KV head: scales[page * scale_block_stride + head]. Codes are e4m3 (4 exponent, 3
+ * fraction bits, largest 448) or signed 8-bit integers.
+ *
+ * Everything is accumulated in F32. On the matrix units (head_dim 128 and bf16 queries) the
+ * weights of the softmax are rounded once to 11 bits (codes), 16 bits (bf16 decode) or 8 bits
+ * (prompt-sized calls), like their operands; other shapes run in F32 throughout. Results
+ * repeat bit for bit. Offsets are 64 bits wide; lengths are below 2^31 - 1024. */
+typedef enum { YVX_KV_PLAIN = 0, YVX_KV_E4M3 = 1, YVX_KV_I8 = 2 } yvx_kv_code;
+typedef struct yvx_scored_problem {
+    unsigned int sessions, query_rows;        /* rows per session (uniform) */
+    unsigned int query_heads, kv_heads, head_dim; /* head_dim at most 256 */
+    unsigned int causal;
+    float scale, cap;                         /* scale > 0; cap 0: none */
+    unsigned int window;                      /* 0: none */
+    int query_dtype, kv_dtype, output_dtype;  /* F32 or BF16; kv_dtype is ignored for codes */
+    int kv_code;                              /* yvx_kv_code */
+    const void *query;                        /* [session][row][head][head_dim] by strides */
+    unsigned long long query_row_stride, query_session_stride, query_head_stride; /* elements; head 0 = head_dim */
+    void *output;                             /* packed [session][row][query_heads * head_dim] */
+    const void *key, *value;
+    unsigned long long key_token_stride, value_token_stride; /* elements (bytes for codes) */
+    unsigned long long key_head_stride, value_head_stride;
+    unsigned long long key_outer_stride, value_outer_stride; /* between sessions, or between pages */
+    const float *key_scales, *value_scales;   /* codes only */
+    unsigned long long scale_block_stride;    /* floats between pages; 0 = kv_heads */
+    const int *block_table;                   /* device [sessions][block_table_stride]; NULL = contiguous */
+    unsigned int block_tokens, block_table_stride, pool_blocks;
+    const unsigned int *kv_tokens;            /* device [sessions]; NULL = uniform */
+    unsigned int kv_tokens_uniform, kv_tokens_max;
+    const unsigned int *query_start;          /* device [sessions]; NULL = uniform / from the end */
+    unsigned int query_start_uniform, query_start_from_end;
+    const int *row_first, *row_end;           /* device [sessions][query_rows] or NULL */
+    const float *slopes;                      /* device [query_heads] or NULL */
+    unsigned int chunk_tokens, max_splits;    /* yvx_cuda_scored_plan */
+    void *workspace;                          /* yvx_cuda_scored_workspace_bytes(), 256-byte aligned; calls
+                                                 that may overlap on the GPU must not share one */
+    unsigned long long workspace_bytes;
+    int *status;                              /* device status word as in yvx_gqa_problem */
+    int force_general;                        /* 1: the general kernel whatever the shape */
+} yvx_scored_problem;
+/* Splits of the KV sequence for a device with `sm_count` SMs; call it after every other field
+ * is set. It depends on the problem's shape, types, strides and alignment only. */
+void yvx_cuda_scored_plan(yvx_scored_problem *problem, int sm_count);
+unsigned long long yvx_cuda_scored_workspace_bytes(const yvx_scored_problem *problem);
+/* Enqueues the attention on `stream` (1 to 3 launches, reported in `launches` when given). No
+ * allocation and no synchronisation: it may be captured into a graph. Refusals, before anything
+ * is enqueued: YVEX_ERR_INVALID_ARG (missing pointers, inconsistent geometry),
+ * YVEX_ERR_UNSUPPORTED (types, head_dim above 256), YVEX_ERR_BOUNDS (launch limits, workspace). */
+int yvx_cuda_scored_attention(const yvx_scored_problem *problem, void *stream, unsigned int *launches);
+
+/* ---- appending rows to a cache of 8-bit codes --------------------------------------
+ * Rows [kv_tokens[b], kv_tokens[b] + new_tokens[b]) of every session, as codes in the pages that
+ * block_table names, K and V alike. Per page and head the scale is the smallest power of two
+ * s >= 2^-126 with max|x| <= s * limit over the page's new rows (limit 448 for e4m3, 127 for
+ * integers); a page that held rows keeps its scale when that is larger, else its old codes are
+ * brought to the new scale. Codes are rounded to nearest even; divisions by s are exact. What a
+ * page holds behind the last row is left as it was. A lane that is not finite is stored as 0
+ * and recorded in the status word (1); a table entry outside the pool, or a session whose rows do
+ * not fit its table row, is recorded (2) and skipped. A page belongs to one session of a call: a
+ * shared one is copied first (yvex_b200_kv_pool_reserve). No counterpart in the reference. */
+typedef struct yvx_kv8_append_args {
+    unsigned int sessions, tokens;            /* tokens: the largest number of new rows of a session */
+    unsigned int kv_heads, head_dim;          /* head_dim a multiple of 16, at most 256 */
+    int code;                                 /* YVX_KV_E4M3 or YVX_KV_I8 */
+    int dtype;                                /* of key and value: F32 or BF16 */
+    const void *key, *value;                  /* [session][token][kv_heads * head_dim] by strides */
+    unsigned long long token_stride, session_stride; /* elements */
+    const unsigned int *kv_tokens;            /* device [sessions]; NULL = kv_tokens_uniform for all */
+    unsigned int kv_tokens_uniform;
+    const unsigned int *new_tokens;           /* device [sessions], at most `tokens`; NULL = tokens for all */
+    const int *block_table;                   /* device [sessions][block_table_stride] */
+    unsigned int block_tokens, block_table_stride, pool_blocks; /* block_tokens at most 256 */
+    void *key_codes, *value_codes;
+    unsigned long long code_token_stride, code_head_stride, code_block_stride; /* bytes, multiples of 16 */
+    float *key_scales, *value_scales;
+    unsigned long long scale_block_stride;    /* floats between pages; 0 = kv_heads */
+    int *status;
+} yvx_kv8_append_args;
+int yvx_cuda_kv8_append(const yvx_kv8_append_args *args, void *stream);
+
+/* ---- copying pages of every layer's pool -------------------------------------------
+ * For each pool and each copy: rows [0, rows) of page `source` to page `destination` (the copies
+ * yvex_b200_kv_pool_reserve and _compact report; entries with needed == 0 are skipped). A page is
+ * `segments` runs of rows `segment_stride` bytes apart (1 for [token][head][dim], kv_heads for
+ * [head][token][dim]); with fixed_bytes a segment is copied whole whatever the rows (scales).
+ * The copies of a call are made in no order: a destination must not be the source or the
+ * destination of another copy (YVEX_ERR_INVALID_ARG). Lists are host memory, read before the
+ * call returns; it may be captured. One launch for up to 512 copies and 128 pools. */
+typedef struct yvx_kv_page_pool {
+    void *base;
+    unsigned long long block_stride, segment_stride, row_bytes, fixed_bytes; /* bytes */
+    unsigned int blocks, segments;
+} yvx_kv_page_pool;
+struct yvx_kv_page_copy { int needed, source_block, destination_block; unsigned int rows; };
+typedef struct yvx_kv_pages_args {
+    const yvx_kv_page_pool *pools;            /* host [pool_count] */
+    const struct yvx_kv_page_copy *copies;    /* host [copy_count]; layout of yvex_b200_kv_copy */
+    unsigned int pool_count, copy_count, block_tokens;
+} yvx_kv_pages_args;
+int yvx_cuda_kv_pages_copy(const yvx_kv_pages_args *args, void *stream, unsigned int *launches);
+
 /* ---- split attention + cross-GPU fold over NVLink peer memory -------------------
  * For one session whose KV sequence is sharded over `ranks` GPUs (one process per
  * GPU): the attention kernel, then ONE kernel that folds this rank's splits, stores

@@ -1,0 +1,72 @@
+"""Scored attention on a B200 against float64: caps, distance bias, windows, visible runs, caches of every kind. What no
+row sees holds NaN in every case; results repeat bit for bit; tolerances are derived in scored_cases.tolerance."""
+import numpy as np
+import pytest
+
+import clori_b200
+from clori_b200 import abi
+from tests.scored_cases import Case, documents
+
+pytestmark = pytest.mark.gpu
+E4M3, I8, PLAIN = abi.KV_E4M3, abi.KV_I8, abi.KV_PLAIN
+F32, BF16 = abi.DTYPE_F32, abi.DTYPE_BF16
+
+
+GENERAL = [
+    # lengths, rows, heads, kv_heads, hd, fields
+    ([1], 1, 1, 1, 128, {}),
+    ([0, 1, 33, 300], 1, 8, 2, 128, dict(kv_dtype=F32, q_dtype=F32)),
+    ([5, 70, 129], 3, 6, 3, 64, dict(cap=20.0, q_scale=6.0)),
+    ([200, 31], 5, 4, 1, 80, dict(slopes=True, out_dtype=BF16)),
+    ([100, 257], 17, 4, 4, 256, dict(kv_dtype=F32, q_dtype=F32, slopes=True, cap=5.0, q_scale=3.0)),
+    ([90, 90], 90, 5, 1, 40, dict(causal=False, slopes=True)),
+    ([300, 129, 64], 4, 8, 2, 128, dict(page=16, window=70)),
+    ([300, 129, 64], 2, 5, 1, 96, dict(page=48, kv_dtype=F32)),
+    ([64, 130, 1], 2, 8, 2, 64, dict(cache=E4M3, page=16, cap=30.0, q_scale=4.0)),
+    ([64, 130, 1], 2, 8, 2, 128, dict(cache=I8, page=24, slopes=True)),
+    ([33], 33, 2, 2, 16, dict(cache=E4M3, page=7, pad=3)),
+    ([40, 41], 8, 4, 2, 33, dict(head_major=True, window=5, pad=1)),
+]
+
+
+@pytest.mark.parametrize("lengths,rows,heads,kv_heads,hd,fields", GENERAL)
+@pytest.mark.parametrize("chunk", [None, 64])
+def test_general_kernel(backend, lengths, rows, heads, kv_heads, hd, fields, chunk):
+    Case(11, lengths, rows, heads, kv_heads, hd, **fields).check(backend, "general", force_general=True, chunk=chunk)
+
+
+def test_rows_in_front_of_the_session_and_empty_sessions_are_zero(backend):
+    c = Case(5, [2, 0, 7], 4, 4, 2, 128)
+    p = c.plan(backend, c.problem(backend))
+    got, status = c.launch(backend, p)
+    assert status == 0
+    assert not got[0, :2].any() and got[0, 2:].any() and not got[1].any() and got[2].any()
+
+
+def test_row_runs_with_gaps_padding_and_reversed_bounds(backend):
+    rng = np.random.default_rng(3)
+    first = rng.integers(-5, 180, (2, 9))
+    end = first + rng.integers(-20, 80, (2, 9))
+    c = Case(6, [190, 150], 9, 4, 2, 128, ranges=(first, end), slopes=True)
+    for general in (False, True):
+        c.check(backend, "general" if general else "decode_bf16", force_general=general)
+
+
+def test_a_nan_that_is_seen_is_reported(backend):
+    for x in ("k", "v"):
+        for fields in (dict(), dict(kv_dtype=F32, q_dtype=F32)):
+            c = Case(7, [100], 1, 4, 2, 128, garbage=False, **fields)
+            c.arrays[x][0, 50] = np.nan
+            assert c.launch(backend, c.plan(backend, c.problem(backend)))[1] == 1
+
+
+def test_bad_lengths_and_table_entries_are_reported(backend):
+    c = Case(8, [100, 90], 1, 4, 2, 128, page=64, cache=E4M3)
+    c.table[1, 0] = 9999
+    assert c.launch(backend, c.plan(backend, c.problem(backend)))[1] == 2
+    c = Case(8, [100, 90], 1, 4, 2, 128, page=64)
+    p = c.plan(backend, c.problem(backend))
+    too_long = backend.tensor("lens", np.array([100, 2000], np.int32))
+    p.kv_tokens = too_long.data_ptr
+    got, status = c.launch(backend, p)
+    assert status == 2 and not got[1].any()
