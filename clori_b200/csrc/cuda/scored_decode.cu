@@ -1,0 +1,561 @@
+// Scored attention for few query rows over long caches: decode and verify, head_dim 128, bf16
+// queries, K and V as bf16 rows or 8-bit codes, contiguous or in pages of 16, 32 or 64 n tokens.
+//
+// Bandwidth-shaped split-KV kernel. A CTA owns up to 16 vectors (query rows x heads of one KV
+// head) and one split; a producer warp streams 64-token tiles of K and V into a ring with tiled
+// copies (one per page and operand; 128-byte swizzle, so every shared-memory read below is free of
+// bank conflicts) together with the pages' scales, and four consumer warps own 16 tokens of each
+// tile: S = Q K^T and O += P V as mma.sync m16n8k16 with the vectors in M. M is at most 16, so the
+// 5th-generation tensor cores have nothing to win: the memory system is the bound.
+//
+// Codes. A lane of 8 bits becomes an exact f16. A page's K scale multiplies the scores; its V scale
+// multiplies the weights, relative to the largest V scale the warp has met (the accumulator is
+// brought along when that grows), so the operand of P V stays inside f16: the arithmetic of a code
+// costs one conversion and nothing else. Queries are brought to f16 by a power of two per vector
+// (exact but for lanes below 2^-29 of the vector's largest). The order of head dimensions inside a
+// k-step is free, so a thread takes 32 adjacent dims of its token with two 16-byte reads.
+// Weights: the maximum is lazy, it moves when a score exceeds it by 2^4 (codes) or 2^8, and the
+// weights of codes carry a factor 2^11 (at most 2^15): one rounding to 11 bits, full precision down
+// to 2^-25 of the largest. bf16 caches carry a weight as head + tail, 16 bits.
+#include "scored.cuh"
+
+namespace yvx {
+
+constexpr int kSdTokens = 64, kSdDim = 128, kSdWarps = 4, kSdThreads = (kSdWarps + 1) * 32;
+constexpr int kSdQRowBytes = kSdDim * 2 + 16;          // padded rows
+constexpr int kSdMergeFloats = kSdDim + 4;
+constexpr int kSdRingBytes = 96 * 1024;
+
+struct SdMaps {
+    CUtensorMap key, value;
+};
+
+template <int CODE>
+struct SdShape {
+    static constexpr int operand_bytes = kSdTokens * kSdDim * (CODE ? 1 : 2);  // one K or V tile
+    static constexpr int stages = kSdRingBytes / (2 * operand_bytes);
+};
+constexpr int kSdMaxStages = SdShape<1>::stages;
+constexpr int kSdSmemBytes = kSdRingBytes + 16 * kSdQRowBytes + kSdMaxStages * kSdWarps * 8 + kSdMaxStages * 16 + 64 + 64 + 1024;
+
+// 16 bits of code (two lanes) -> f16x2, four lanes -> two of them.
+template <int CODE>
+__device__ __forceinline__ void sd_codes(uint32_t word, uint32_t &lo, uint32_t &hi)
+{
+    if (CODE == YVX_KV_E4M3) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(word));
+    } else {
+        // a byte u under the exponent 0x64 reads 1024 + u; u = lane + 128
+        uint32_t a, b;
+        const uint32_t biased = word ^ 0x80808080u;
+        asm("prmt.b32 %0, %1, %2, 0x4140;" : "=r"(a) : "r"(biased), "r"(0x64646464u));
+        asm("prmt.b32 %0, %1, %2, 0x4342;" : "=r"(b) : "r"(biased), "r"(0x64646464u));
+        asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+        asm("sub.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+    }
+}
+
+// grid: x = split, y = kv_head * row_tiles + row_tile, z = session. `unit`: tokens of one tiled copy
+// (a page or 64). `head_inner`: the maps order their middle dimensions (head, token).
+template <int CODE>
+__global__ void __launch_bounds__(kSdThreads, 2)
+scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps maps, const int unit, const int head_inner)
+{
+    typedef SdShape<CODE> Shape;
+    constexpr int kStages = Shape::stages, kOperand = Shape::operand_bytes;
+    extern __shared__ unsigned char sd_raw[];
+    // the 128-byte swizzle is a function of address bits 4..9
+    unsigned char *ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(sd_raw) + 1023u) & ~uintptr_t(1023));
+    unsigned char *q_smem = ring + kSdRingBytes;
+    float2 *scale_smem = reinterpret_cast<float2 *>(q_smem + 16 * kSdQRowBytes);   // [stage][warp]: K, V
+    uint64_t *full = reinterpret_cast<uint64_t *>(scale_smem + kSdMaxStages * kSdWarps);
+    uint64_t *empty = full + kSdMaxStages;
+    float *q_unscale = reinterpret_cast<float *>(empty + kSdMaxStages);            // [16]
+
+    const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const unsigned int group = p.query_heads / p.kv_heads, vectors = p.query_rows * group;
+    const unsigned int row_tiles = (vectors + 15u) / 16u;
+    const unsigned int kv_head = blockIdx.y / row_tiles, row_tile = blockIdx.y % row_tiles;
+    const unsigned int b = blockIdx.z, split = blockIdx.x;
+    const unsigned int kv_tokens = admitted_kv_tokens(p.kv_tokens, b, p.kv_tokens_uniform, p.kv_tokens_max, p.status);
+    const long long query_start = scored_query_start(p, b, kv_tokens);
+    const unsigned int vector_base = row_tile * 16u, live = min(16u, vectors - vector_base);
+    int hull_first, hull_end, t0, t1;
+    scored_hull(p, b, vector_base / group, (vector_base + live - 1u) / group + 1u, kv_tokens, query_start, hull_first, hull_end);
+    scored_split(p, split, hull_first, hull_end, t0, t1);
+    auto item_of = [&](unsigned int i) {
+        const unsigned int v = vector_base + i;
+        return ((unsigned long long)b * p.query_rows + v / group) * p.query_heads + kv_head * group + v % group;
+    };
+    if (t0 >= t1) {
+        for (unsigned int i = warp; i < live; i += kSdThreads / 32) scored_store_empty(p, item_of(i), split, lane, 32u);
+        return;
+    }
+    const unsigned int tiles = (unsigned int)(t1 - t0 + kSdTokens - 1) / kSdTokens;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kSdWarps);
+        }
+        fence_barrier_init();
+    }
+    __syncthreads();
+
+    if (warp == kSdWarps) {
+        // ---- producer: 32 table entries (and scales) at a time, a lane each ----------------------
+        const unsigned int per_tile = (unsigned int)(kSdTokens / unit), batch_tiles = 32u / per_tile;
+        int page = 0, inner = 0;
+        float key_scale = 0.0f, value_scale = 0.0f;
+        for (unsigned int i = 0; i < tiles; ++i) {
+            const unsigned int slot = i % batch_tiles;
+            if (slot == 0u) {
+                const int token = t0 + (int)(i * kSdTokens) + (int)lane * unit;
+                page = -1;
+                if (token < t1) {
+                    if (p.block_table) {
+                        page = scored_page(p, b, (unsigned int)token / p.block_tokens);
+                        if (page < 0) page = 0;
+                        inner = (int)((unsigned int)token % p.block_tokens);
+                        if (CODE) {
+                            const unsigned long long at =
+                                (unsigned long long)page * (p.scale_block_stride ? p.scale_block_stride : p.kv_heads) + kv_head;
+                            key_scale = p.key_scales[at];
+                            value_scale = p.value_scales[at];
+                        }
+                    } else {
+                        page = (int)b;
+                        inner = token;
+                    }
+                }
+            }
+            const unsigned int stage = i % kStages;
+            if (i >= (unsigned int)kStages && !__all_sync(0xffffffffu, mbar_wait(&empty[stage], ((i / kStages) - 1u) & 1u))) {
+                if (lane == 0) atomicCAS(p.status, 0, YVX_STATUS_TIMEOUT);
+                return;
+            }
+            const unsigned int mine = slot * per_tile + min(lane, per_tile - 1u);
+            const int unit_page = __shfl_sync(0xffffffffu, page, mine), unit_inner = __shfl_sync(0xffffffffu, inner, mine);
+            const unsigned int loaded = __ballot_sync(0xffffffffu, lane < per_tile && unit_page >= 0);
+            if (CODE) {
+                // the scales of the 16 tokens of consumer warp `lane`; a unit behind the split's end: 0
+                const unsigned int of_warp = slot * per_tile + (16u * min(lane, 3u)) / (unsigned int)unit;
+                const float ks = __shfl_sync(0xffffffffu, key_scale, of_warp), vs = __shfl_sync(0xffffffffu, value_scale, of_warp);
+                const int there = __shfl_sync(0xffffffffu, page, of_warp);
+                if (lane < (unsigned int)kSdWarps)
+                    scale_smem[stage * kSdWarps + lane] = there >= 0 ? make_float2(ks, vs) : make_float2(0.0f, 0.0f);
+                __syncwarp();
+            }
+            unsigned char *k_dst = ring + stage * 2 * kOperand, *v_dst = k_dst + kOperand;
+            if (lane == 0) mbar_expect_tx(&full[stage], (uint32_t)__popc(loaded) * (uint32_t)unit * kSdDim * 2u * (CODE ? 1u : 2u));
+            __syncwarp();
+            if (lane < per_tile && unit_page >= 0) {
+                const int c1 = head_inner ? (int)kv_head : unit_inner, c2 = head_inner ? unit_inner : (int)kv_head;
+                const uint32_t at = lane * (uint32_t)unit * 128u;
+                tma_load_4d(k_dst + at, &maps.key, &full[stage], 0, c1, c2, unit_page);
+                if (!CODE) tma_load_4d(k_dst + kOperand / 2 + at, &maps.key, &full[stage], 64, c1, c2, unit_page);
+                tma_load_4d(v_dst + at, &maps.value, &full[stage], 0, c1, c2, unit_page);
+                if (!CODE) tma_load_4d(v_dst + kOperand / 2 + at, &maps.value, &full[stage], 64, c1, c2, unit_page);
+            }
+        }
+        return;
+    }
+
+    // ---- consumers ------------------------------------------------------------------------------
+    const unsigned int g = lane >> 2, c = lane & 3u;
+    // queries into shared memory: bf16 as they are, or f16 after a power of two that brings the vector's
+    // largest lane to [2^14, 2^15); a warp per row, 4 dims per lane
+    for (unsigned int row = warp; row < 16u; row += kSdWarps) {
+        uint2 raw = make_uint2(0u, 0u);
+        if (row < live) {
+            const unsigned int v = vector_base + row;
+            raw = *reinterpret_cast<const uint2 *>(
+                reinterpret_cast<const __nv_bfloat16 *>(p.query) + (unsigned long long)b * p.query_session_stride +
+                (unsigned long long)(v / group) * p.query_row_stride +
+                (unsigned long long)(kv_head * group + v % group) * (p.query_head_stride ? p.query_head_stride : kSdDim) + 4u * lane);
+        }
+        if (CODE) {
+            const float x0 = __uint_as_float(raw.x << 16), x1 = __uint_as_float(raw.x & 0xffff0000u);
+            const float x2 = __uint_as_float(raw.y << 16), x3 = __uint_as_float(raw.y & 0xffff0000u);
+            const float top = warp_max(fmaxf(fmaxf(fabsf(x0), fabsf(x1)), fmaxf(fabsf(x2), fabsf(x3))));
+            // exponent field of the largest lane, kept where the factor and its inverse are normal numbers
+            const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);
+            const float up = __uint_as_float((unsigned int)min(127 + 14 + 127 - e, 254) << 23);
+            raw.x = pack_f16(x0 * up, x1 * up);
+            raw.y = pack_f16(x2 * up, x3 * up);
+            if (lane == 0) q_unscale[row] = 1.0f / up;
+        }
+        *reinterpret_cast<uint2 *>(q_smem + row * kSdQRowBytes + 8u * lane) = raw;
+    }
+    named_barrier(1, kSdWarps * 32);
+    uint32_t qa[8][4];
+    float mul[2] = {p.scale, p.scale};    // raw product -> logit (natural units)
+    if (CODE) {
+        // dims 32c .. 32c+31 of rows g and g + 8; k-step s takes the four at 32c + 4s
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 a = *reinterpret_cast<const uint4 *>(q_smem + g * kSdQRowBytes + 64u * c + 16u * i);
+            const uint4 d = *reinterpret_cast<const uint4 *>(q_smem + (g + 8u) * kSdQRowBytes + 64u * c + 16u * i);
+            qa[2 * i][0] = a.x, qa[2 * i][2] = a.y, qa[2 * i + 1][0] = a.z, qa[2 * i + 1][2] = a.w;
+            qa[2 * i][1] = d.x, qa[2 * i][3] = d.y, qa[2 * i + 1][1] = d.z, qa[2 * i + 1][3] = d.w;
+        }
+        mul[0] *= q_unscale[g];
+        mul[1] *= q_unscale[g + 8u];
+    } else {
+        const unsigned int j = lane >> 3, i = lane & 7u;
+        const uint32_t base = smem_u32(q_smem) + (8u * (j & 1u) + i) * kSdQRowBytes + 16u * (j >> 1);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) ldmatrix_x4(qa[ks], base + ks * 32u);
+    }
+    // this thread's rows, and the tokens that every live row of the CTA sees
+    int first[2], end[2], position[2];
+    float slope[2];
+    int inner_first = 0, inner_end = 0x7fffffff;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const unsigned int row = g + 8u * h;
+        first[h] = 0x7fffffff, end[h] = 0, position[h] = 0, slope[h] = 0.0f;
+        if (row < live) {
+            const unsigned int v = vector_base + row;
+            const ScoredRange r = scored_range(p, b, v / group, kv_tokens, query_start);
+            first[h] = r.first, end[h] = r.end, position[h] = (int)min(r.position, 0x7fffffffll);
+            if (p.slopes) slope[h] = p.slopes[kv_head * group + v % group];
+            inner_first = max(inner_first, r.first);
+            inner_end = min(inner_end, r.end);
+        }
+    }
+    inner_first = __reduce_max_sync(0xffffffffu, inner_first);
+    inner_end = __reduce_min_sync(0xffffffffu, inner_end);
+
+    constexpr float kSlack = CODE ? 4.0f : 8.0f, kLift = CODE ? 11.0f : 0.0f;
+    const bool capped = p.cap > 0.0f, biased = p.slopes != nullptr;
+    const float inverse_cap = capped ? 1.0f / p.cap : 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float v_ref = 1.17549435e-38f, v_inverse = 8.50705917e37f;  // 2^-126: no V scale is smaller and counts
+    float o[16][4];
+#pragma unroll
+    for (int n = 0; n < 16; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
+
+    for (unsigned int i = 0; i < tiles; ++i) {
+        const unsigned int stage = i % kStages;
+        if (!mbar_wait(&full[stage], (i / kStages) & 1u)) {
+            atomicCAS(p.status, 0, YVX_STATUS_TIMEOUT);
+            break;
+        }
+        const unsigned char *k_tile = ring + stage * 2 * kOperand;
+        const uint32_t k_base = smem_u32(k_tile), v_base = k_base + kOperand;
+        const int token0 = t0 + (int)(i * kSdTokens) + 16 * (int)warp;
+        float2 scales = make_float2(1.0f, 1.0f);
+        if (CODE) scales = scale_smem[stage * kSdWarps + warp];
+
+        // ---- S = Q K^T over 16 tokens: column 8 n + j of the tile is token 8 n + j ----------------
+        float sc[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
+        if (CODE) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const unsigned int row = 16u * warp + 8u * n + g;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint4 kq = *reinterpret_cast<const uint4 *>(k_tile + row * 128u + (((2u * c + half) ^ (row & 7u)) << 4));
+                    const uint32_t words[4] = {kq.x, kq.y, kq.z, kq.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t b0, b1;
+                        sd_codes<CODE>(words[w], b0, b1);
+                        mma_f16(sc[n], qa[4 * half + w], b0, b1);
+                    }
+                }
+            }
+        } else {
+            const unsigned int j = lane >> 3, r = lane & 7u;
+            const unsigned int token = 16u * warp + 8u * (j >> 1) + r;
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                const unsigned int chunk = 2u * (ks & 3) + (j & 1u);
+                uint32_t kb[4];
+                ldmatrix_x4(kb, k_base + (ks >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
+                mma_bf16(sc[0], qa[ks], kb[0], kb[1]);
+                mma_bf16(sc[1], qa[ks], kb[2], kb[3]);
+            }
+        }
+        // ---- the score rule, in log2 units --------------------------------------------------------
+        const float unit0 = mul[0] * scales.x, unit1 = mul[1] * scales.x;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float z = sc[n][e] * (e < 2 ? unit0 : unit1);
+                if (capped) {
+                    // tanh from one exponential: 1 - 2 / (e^2x + 1), absolute error a few 2^-24
+                    const float t = exp2_approx(z * inverse_cap * (2.0f * kScoredLog2e));
+                    z = p.cap - 2.0f * p.cap * __frcp_rn(t + 1.0f);
+                }
+                if (biased) {
+                    const int distance = position[e >> 1] - (token0 + 8 * n + 2 * (int)c + (e & 1));
+                    z = fmaf(-slope[e >> 1], fabsf((float)distance), z);
+                }
+                sc[n][e] = z * kScoredLog2e;
+            }
+        // ---- visibility: tokens that no row of the CTA sees may hold anything in V ----------------
+        uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;
+        if (token0 < inner_first || token0 + 16 > inner_end) {
+            uint32_t seen = 0u;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int token = token0 + 8 * n + 2 * (int)c + (e & 1);
+                    const bool visible = token >= first[e >> 1] && token < end[e >> 1];
+                    if (!visible) sc[n][e] = -INFINITY;
+                    seen |= (visible ? 1u : 0u) << (2 * n + (e & 1));
+                }
+#pragma unroll
+            for (int offset = 4; offset < 32; offset <<= 1) seen |= __shfl_xor_sync(0xffffffffu, seen, offset);
+            keep_lo = (seen & 1u ? 0x0000ffffu : 0u) | (seen & 2u ? 0xffff0000u : 0u);
+            keep_hi = (seen & 4u ? 0x0000ffffu : 0u) | (seen & 8u ? 0xffff0000u : 0u);
+        }
+        // ---- online softmax with a lazy maximum ----------------------------------------------------
+        bool grow = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float bound = m[h] + kSlack;  // -inf while the row has seen nothing
+#pragma unroll
+            for (int n = 0; n < 2; ++n) grow = grow || sc[n][2 * h] > bound || sc[n][2 * h + 1] > bound;
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+            float keep[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float fresh = fmaxf(m[h], top);
+                keep[h] = fresh == -INFINITY ? 1.0f : exp2_approx(m[h] - fresh);
+                m[h] = fresh;
+                l[h] *= keep[h];
+            }
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+                o[n][0] *= keep[0];
+                o[n][1] *= keep[0];
+                o[n][2] *= keep[1];
+                o[n][3] *= keep[1];
+            }
+        }
+        float ratio = 1.0f;
+        if (CODE) {
+            const float size = fabsf(scales.y);
+            if (size > v_ref) {  // the warp's 16 tokens share a page: uniform
+                const float factor = v_ref / size;
+#pragma unroll
+                for (int n = 0; n < 16; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][e] *= factor;
+                v_ref = size;
+                v_inverse = 1.0f / size;
+            }
+            ratio = scales.y * v_inverse;
+        }
+        float offset[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) offset[h] = m[h] == -INFINITY ? 0.0f : kLift - m[h];
+        uint32_t p_head[4], p_tail[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float p0 = exp2_approx(sc[n][2 * h] + offset[h]), p1 = exp2_approx(sc[n][2 * h + 1] + offset[h]);
+                l[h] += p0 + p1;
+                if (CODE) {
+                    p_head[2 * n + h] = pack_f16(p0 * ratio, p1 * ratio);
+                } else {
+                    const uint32_t head = pack_bf16(p0, p1);
+                    p_head[2 * n + h] = head;
+                    p_tail[2 * n + h] = pack_bf16(p0 - __uint_as_float(head << 16), p1 - __uint_as_float(head & 0xffff0000u));
+                }
+            }
+        // ---- O += P V -------------------------------------------------------------------------------
+        const unsigned int j = lane >> 3, r = lane & 7u;
+        const unsigned int token = 16u * warp + 8u * (j & 1u) + r;
+        if (CODE) {
+            // A transposed 8x8 block of 16-bit pairs gives a thread two tokens of two adjacent dims; columns of
+            // the accumulator tile 2 ch + parity are the dims 16 ch + 2 g + parity.
+#pragma unroll
+            for (int np = 0; np < 4; ++np) {
+                uint32_t raw[4];
+                ldmatrix_x4_trans(raw, v_base + token * 128u + (((2u * np + (j >> 1)) ^ (token & 7u)) << 4));
+#pragma unroll
+                for (int ch = 0; ch < 2; ++ch) {
+                    uint32_t lo, hi, lo_even, lo_odd, hi_even, hi_odd;
+                    asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(lo) : "r"(raw[2 * ch]));
+                    asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(hi) : "r"(raw[2 * ch + 1]));
+                    sd_codes<CODE>(lo, lo_even, lo_odd);
+                    sd_codes<CODE>(hi, hi_even, hi_odd);
+                    mma_f16(o[4 * np + 2 * ch], p_head, lo_even & keep_lo, hi_even & keep_hi);
+                    mma_f16(o[4 * np + 2 * ch + 1], p_head, lo_odd & keep_lo, hi_odd & keep_hi);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int np = 0; np < 8; ++np) {
+                const unsigned int chunk = 2u * (np & 3) + (j >> 1);
+                uint32_t vb[4];
+                ldmatrix_x4_trans(vb, v_base + (np >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
+                mma_bf16(o[2 * np], p_head, vb[0] & keep_lo, vb[1] & keep_hi);
+                mma_bf16(o[2 * np], p_tail, vb[0] & keep_lo, vb[1] & keep_hi);
+                mma_bf16(o[2 * np + 1], p_head, vb[2] & keep_lo, vb[3] & keep_hi);
+                mma_bf16(o[2 * np + 1], p_tail, vb[2] & keep_lo, vb[3] & keep_hi);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+    }
+
+    // ---- merge the four warps and publish ------------------------------------------------------------
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    pdl_launch_dependents();
+    named_barrier(1, kSdWarps * 32);   // every warp is done reading the ring
+    float *merge_o = reinterpret_cast<float *>(ring);                      // [4][16][132]
+    float *merge_m = merge_o + kSdWarps * 16 * kSdMergeFloats;             // [4][16]
+    float *merge_l = merge_m + kSdWarps * 16;                              // [4][16]
+    const float out_scale = CODE ? v_ref : 1.0f;
+#pragma unroll
+    for (int n = 0; n < 16; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float *row = merge_o + (warp * 16u + g + 8u * h) * kSdMergeFloats;
+            const float x0 = o[n][2 * h] * out_scale, x1 = o[n][2 * h + 1] * out_scale;
+            if (CODE) {
+                row[16 * (n >> 1) + 4 * c + (n & 1)] = x0;
+                row[16 * (n >> 1) + 4 * c + 2 + (n & 1)] = x1;
+            } else {
+                *reinterpret_cast<float2 *>(row + 8 * n + 2 * c) = make_float2(x0, x1);
+            }
+        }
+    if (c == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            merge_m[warp * 16u + g + 8u * h] = m[h] - kLift;
+            merge_l[warp * 16u + g + 8u * h] = l[h];
+        }
+    }
+    named_barrier(1, kSdWarps * 32);
+    const unsigned int d = threadIdx.x;  // one head dimension per consumer thread
+    for (unsigned int row = 0; row < live; ++row) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kSdWarps; ++w) top = fmaxf(top, merge_m[w * 16 + row]);
+        float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kSdWarps; ++w) {
+            const float mw = merge_m[w * 16 + row];
+            const float weight = mw == -INFINITY ? 0.0f : exp2_approx(mw - top);
+            sum += merge_l[w * 16 + row] * weight;
+            acc += merge_o[(w * 16 + row) * kSdMergeFloats + d] * weight;
+        }
+        const unsigned long long item = item_of(row);
+        if (p.max_splits > 1u) {
+            float *part = scored_partial(p, item, split);
+            part[d] = acc;
+            if (d == 0) {
+                part[kSdDim] = top;
+                part[kSdDim + 1] = sum;
+            }
+        } else {
+            const float value = sum == 0.0f ? 0.0f : acc / sum;
+            if (!isfinite(value)) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
+            store_output(p.output, p.output_dtype, item * kSdDim + d, value);
+        }
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------
+
+typedef CUresult (*ScoredEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static ScoredEncodeFn scored_encode_entry()
+{
+    static ScoredEncodeFn entry = [] {
+        void *symbol = nullptr;
+        cudaDriverEntryPointQueryResult query;
+        const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &symbol, cudaEnableDefault, &query) == cudaSuccess &&
+                           query == cudaDriverEntryPointSuccess;
+        return found ? reinterpret_cast<ScoredEncodeFn>(symbol) : nullptr;
+    }();
+    return entry;
+}
+
+// {128 lanes, two middle dimensions by ascending stride, outer}; the box is 128 bytes of `box_tokens` rows.
+// Returns false when tiled copies cannot describe the layout.
+bool scored_encode_rows(CUtensorMap *map, const void *base, int element_bytes, unsigned long long token_stride,
+                        unsigned long long head_stride, unsigned long long outer_stride, unsigned long long tokens,
+                        unsigned long long heads, unsigned long long outer, bool head_inner, unsigned int box_tokens)
+{
+    ScoredEncodeFn encode = scored_encode_entry();
+    const unsigned long long tb = token_stride * element_bytes, hb = head_stride * element_bytes;
+    unsigned long long ob = outer_stride * element_bytes;
+    if (outer == 1ull) ob = ((head_inner ? tb * tokens : hb * heads) + 15ull) & ~15ull;
+    if (!encode || (reinterpret_cast<uintptr_t>(base) & 15u) || (tb & 15ull) || (hb & 15ull) || (ob & 15ull) || !tb || !hb ||
+        !ob || tb >= (1ull << 40) || hb >= (1ull << 40) || ob >= (1ull << 40))
+        return false;
+    const cuuint64_t dims[4] = {kSdDim, head_inner ? heads : tokens, head_inner ? tokens : heads, outer};
+    const cuuint64_t strides[3] = {head_inner ? hb : tb, head_inner ? tb : hb, ob};
+    const cuuint32_t box[4] = {128u / (unsigned int)element_bytes, head_inner ? 1u : box_tokens, head_inner ? box_tokens : 1u, 1u};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    return encode(map, element_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                  const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// 1: launched, 0: not this kernel's shape, negative: an error.
+int scored_decode_launch(const yvx_scored_problem &p, cudaStream_t stream)
+{
+    const int element_bytes = p.kv_code == YVX_KV_PLAIN ? 2 : 1;
+    const unsigned long long vectors = (unsigned long long)p.query_rows * (p.query_heads / p.kv_heads);
+    const unsigned long long head_stride = p.query_head_stride ? p.query_head_stride : kSdDim;
+    if (p.head_dim != (unsigned)kSdDim || p.query_dtype != YVEX_DTYPE_BF16 ||
+        (p.kv_code == YVX_KV_PLAIN && p.kv_dtype != YVEX_DTYPE_BF16) || (reinterpret_cast<uintptr_t>(p.query) & 7u) ||
+        (p.query_row_stride & 3ull) || (p.query_session_stride & 3ull) || (head_stride & 3ull) ||
+        (vectors + 15ull) / 16ull * p.kv_heads > 65535ull)
+        return 0;
+    unsigned int unit = kSdTokens;
+    if (p.block_table && p.block_tokens % kSdTokens) {
+        if (p.block_tokens != 16u && p.block_tokens != 32u) return 0;
+        unit = p.block_tokens;
+    }
+    const bool head_inner = p.key_head_stride < p.key_token_stride;
+    if ((p.value_head_stride < p.value_token_stride) != head_inner) return 0;
+    const unsigned long long tokens = p.block_table ? p.block_tokens : p.kv_tokens_max;
+    const unsigned long long outer = p.block_table ? p.pool_blocks : p.sessions;
+    SdMaps maps;
+    if (!scored_encode_rows(&maps.key, p.key, element_bytes, p.key_token_stride, p.key_head_stride, p.key_outer_stride, tokens,
+                            p.kv_heads, outer, head_inner, unit) ||
+        !scored_encode_rows(&maps.value, p.value, element_bytes, p.value_token_stride, p.value_head_stride,
+                            p.value_outer_stride, tokens, p.kv_heads, outer, head_inner, unit))
+        return 0;
+    void (*const kernels[3])(const yvx_scored_problem, const SdMaps, const int, const int) = {
+        scored_decode_kernel<YVX_KV_PLAIN>, scored_decode_kernel<YVX_KV_E4M3>, scored_decode_kernel<YVX_KV_I8>};
+    YVX_CUDA_TRY(cudaFuncSetAttribute((const void *)kernels[p.kv_code], cudaFuncAttributeMaxDynamicSharedMemorySize, kSdSmemBytes));
+    const dim3 grid(p.max_splits, p.kv_heads * (unsigned int)((vectors + 15ull) / 16ull), p.sessions);
+    kernels[p.kv_code]<<<grid, kSdThreads, kSdSmemBytes, stream>>>(p, maps, (int)unit, head_inner ? 1 : 0);
+    const int rc = yvx_cuda_check(cudaGetLastError(), "scored_decode_kernel");
+    return rc != 0 ? rc : 1;
+}
+
+}  // namespace yvx

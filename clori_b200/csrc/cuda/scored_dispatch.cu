@@ -90,7 +90,11 @@ int yvx_cuda_scored_attention(const yvx_scored_problem *p, void *stream, unsigne
     if (needed && (!p->workspace || p->workspace_bytes < needed || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)))
         return yvx::scored_refuse(YVEX_ERR_BOUNDS, "scored attention: the workspace is missing, misaligned or too small");
     cudaStream_t s = (cudaStream_t)stream;
-    rc = yvx::scored_general_launch(*p, s);
+    const unsigned long long vectors = (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads);
+    // specialised kernels answer 1 when they took the call, 0 when its shape is not theirs
+    rc = !p->force_general && vectors <= 64ull ? yvx::scored_decode_launch(*p, s) : 0;
+    if (rc == 0) rc = yvx::scored_general_launch(*p, s);
+    else if (rc == 1) rc = 0;
     if (rc != 0) return rc;
     unsigned int count = 1u;
     if (p->max_splits > 1u) {

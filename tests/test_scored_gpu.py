@@ -35,6 +35,53 @@ def test_general_kernel(backend, lengths, rows, heads, kv_heads, hd, fields, chu
     Case(11, lengths, rows, heads, kv_heads, hd, **fields).check(backend, "general", force_general=True, chunk=chunk)
 
 
+LENGTHS = [1, 15, 16, 17, 63, 64, 65, 130, 0, 700]
+DECODE = [
+    # lengths, rows, heads, kv_heads, fields
+    ([1], 1, 1, 1, {}),
+    (LENGTHS, 1, 8, 2, dict(page=64)),
+    (LENGTHS, 1, 5, 1, dict(page=128, cap=30.0, q_scale=6.0)),
+    (LENGTHS, 3, 8, 2, dict(out_dtype=BF16, slopes=True)),
+    ([500, 333], 8, 16, 2, dict(head_major=True, window=100)),
+    ([500, 333], 2, 16, 1, dict(causal=False, slopes=True, cap=5.0, pad=8)),
+    (LENGTHS, 1, 8, 2, dict(cache=E4M3, page=64)),
+    (LENGTHS, 4, 4, 1, dict(cache=E4M3, page=16, cap=50.0, q_scale=8.0)),
+    (LENGTHS, 1, 10, 2, dict(cache=I8, page=32, slopes=True, out_dtype=BF16)),
+    (LENGTHS, 8, 16, 2, dict(cache=I8, page=128, window=90, cap=2.0)),
+    (LENGTHS, 2, 2, 2, dict(cache=E4M3, page=64, q_scale=1e-30, k_scale=1e20)),
+    ([200, 129], 3, 4, 2, dict(cache=E4M3, page=16, q_scale=3e5, k_scale=1e-7, outlier=40.0)),
+    ([900, 64], 1, 4, 2, dict(cache=I8, page=64, query_start=[1000, 20])),
+]
+
+
+@pytest.mark.parametrize("lengths,rows,heads,kv_heads,fields", DECODE)
+@pytest.mark.parametrize("chunk", [None, 64, 128])
+def test_decode_kernel(backend, lengths, rows, heads, kv_heads, fields, chunk):
+    path = "decode_codes" if fields.get("cache") else "decode_bf16"
+    Case(12, lengths, rows, heads, kv_heads, 128, **fields).check(backend, path, chunk=chunk)
+
+
+def test_one_loud_token_does_not_hide_many_quiet_ones(backend):
+    # weights far below the largest carry half of the result: they have to survive their rounding
+    for fields, path in ((dict(page=64), "decode_bf16"), (dict(cache=E4M3, page=64), "decode_codes")):
+        c = Case(13, [6000], 1, 2, 1, 128, q_scale=0.0, garbage=False, **fields)
+        c.slope = np.array([0.0, 0.0], np.float32)
+        c.q[:] = 1.0
+        a, s = c.arrays["k"], c.arrays["k_scales"]
+        block, slot = int(c.table[0, 0]), 3
+        if fields.get("cache"):
+            a[:], s[:] = 0, 2.0 ** -126
+            s[block] = 1.0
+            a[block, :, slot] = 0x38            # 1.0 in every lane: the score is sqrt(128), 2^16 times the others' weight
+            c.values["k"][:] = 0.0
+        else:
+            a[:] = 0.0
+            a[block, slot] = 1.0
+            c.values["k"][:] = 0.0
+        c.values["k"][0, 3] = 1.0
+        c.check(backend, path)
+
+
 def test_rows_in_front_of_the_session_and_empty_sessions_are_zero(backend):
     c = Case(5, [2, 0, 7], 4, 4, 2, 128)
     p = c.plan(backend, c.problem(backend))
