@@ -166,6 +166,13 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
+__device__ __forceinline__ float min3(float a, float b, float c)
+{
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // (lo, hi) -> packed bf16x2 with lo in the low half, round to nearest even.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
 {

@@ -115,7 +115,8 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
             if (slot == 0u) {
                 const int token = t0 + (int)(i * kSdTokens) + (int)lane * unit;
                 page = -1;
-                if (token < t1) {
+                // pages in front of the first visible token may be gone: not looked up, not loaded
+                if (token < t1 && token + unit > hull_first) {
                     if (p.block_table) {
                         page = scored_page(p, b, (unsigned int)token / p.block_tokens);
                         if (page < 0) page = 0;

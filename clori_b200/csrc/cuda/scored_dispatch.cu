@@ -43,6 +43,28 @@ static unsigned long long scored_span(const yvx_scored_problem *p)
     return seen < all ? (seen + 63ull) / 64ull * 64ull : all;
 }
 
+// Calls of more than 64 vectors (query rows x heads of a KV head) on the shapes of the tensor cores: the
+// rows fill 128-row tiles by themselves and the KV sequence is not split. Decided by the shape, types and
+// alignment alone, before the plan.
+static bool scored_prompt_shape(const yvx_scored_problem *p)
+{
+    const unsigned long long bytes = p->kv_code == YVX_KV_PLAIN ? 2ull : 1ull;
+    const unsigned long long strides = p->key_token_stride | p->value_token_stride | p->key_head_stride | p->value_head_stride |
+                                       p->key_outer_stride | p->value_outer_stride;
+    const unsigned long long q_strides = p->query_row_stride | p->query_session_stride | p->query_head_stride;
+    return !p->force_general && p->head_dim == 128u && p->query_dtype == YVEX_DTYPE_BF16 &&
+           (p->kv_code != YVX_KV_PLAIN || p->kv_dtype == YVEX_DTYPE_BF16) &&
+           (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) > 64ull &&
+           !((reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value) |
+              reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->output) | strides * bytes | q_strides * 2ull) & 15ull);
+}
+
+// Caches that the tensor-core kernel does not read in place: codes, and pages that are no multiple of 64 tokens.
+static bool scored_needs_stage(const yvx_scored_problem *p)
+{
+    return p->kv_code != YVX_KV_PLAIN || (p->block_table && p->block_tokens % 64u);
+}
+
 }  // namespace yvx
 
 extern "C" {
@@ -56,6 +78,11 @@ void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
     const unsigned long long wave = 2ull * (unsigned long long)(sm_count > 0 ? sm_count : 148);
     const unsigned long long vectors = (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads);
     const unsigned long long span = yvx::scored_span(p);
+    if (yvx::scored_prompt_shape(p)) {
+        p->chunk_tokens = (unsigned int)span;
+        p->max_splits = 1u;
+        return;
+    }
     const unsigned long long lanes = (unsigned long long)p->sessions * p->kv_heads * ((vectors + 15ull) / 16ull);
     unsigned int best = 64u;
     double best_fill = -1.0;
@@ -77,7 +104,9 @@ void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
 
 unsigned long long yvx_cuda_scored_workspace_bytes(const yvx_scored_problem *p)
 {
-    if (!p || p->max_splits <= 1u) return 0ull;
+    if (!p || !p->kv_heads || !p->query_rows) return 0ull;
+    if (p->max_splits <= 1u)
+        return yvx::scored_prompt_shape(p) && yvx::scored_needs_stage(p) ? yvx::scored_stage_bytes(*p) : 0ull;
     return (unsigned long long)p->sessions * p->query_rows * p->query_heads * p->max_splits * (p->head_dim + 4ull) * 4ull;
 }
 
@@ -90,13 +119,23 @@ int yvx_cuda_scored_attention(const yvx_scored_problem *p, void *stream, unsigne
     if (needed && (!p->workspace || p->workspace_bytes < needed || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)))
         return yvx::scored_refuse(YVEX_ERR_BOUNDS, "scored attention: the workspace is missing, misaligned or too small");
     cudaStream_t s = (cudaStream_t)stream;
-    const unsigned long long vectors = (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads);
-    // specialised kernels answer 1 when they took the call, 0 when its shape is not theirs
-    rc = !p->force_general && vectors <= 64ull ? yvx::scored_decode_launch(*p, s) : 0;
+    unsigned int count = 0u;
+    rc = 0;  // specialised kernels answer 1 or 2 (no fold needed) when they took the call, 0 when its shape is not theirs
+    if (yvx::scored_prompt_shape(p) && p->max_splits == 1u) {
+        yvx_scored_problem staged = *p;
+        if (yvx::scored_needs_stage(p)) {
+            rc = yvx::scored_stage_launch(*p, &staged, s);
+            if (rc != 0) return rc;
+            ++count;
+        }
+        rc = yvx::scored_prompt_launch(staged, s);
+    } else if (!p->force_general && (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) <= 64ull) {
+        rc = yvx::scored_decode_launch(*p, s);
+    }
     if (rc == 0) rc = yvx::scored_general_launch(*p, s);
-    else if (rc == 1) rc = 0;
+    else if (rc > 0) rc = 0;
     if (rc != 0) return rc;
-    unsigned int count = 1u;
+    ++count;
     if (p->max_splits > 1u) {
         rc = yvx::scored_combine_launch(*p, s);
         if (rc != 0) return rc;

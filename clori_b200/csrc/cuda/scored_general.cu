@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kSgThreads) scored_general_kernel(const yvx_sc
             const int t = tile + (int)token;
             const Element *key = nullptr, *value = nullptr;
             float key_scale = 1.0f, value_scale = 1.0f;
-            if (t < t1) {
+            if (t < t1 && t >= hull_first) {  // pages in front of the first visible token may be gone
                 unsigned long long outer = b, inner = (unsigned long long)t;
                 if (p.block_table) {
                     const int page = scored_page(p, b, (unsigned int)t / p.block_tokens);

@@ -1,0 +1,586 @@
+// Scored attention for prompt-sized calls on the 5th-generation tensor cores: bf16 Q / K / V,
+// head_dim 128, contiguous rows or pages of 64 n tokens, any rule and any visible runs.
+//
+// A CTA owns two tiles (A, B) of 128 query rows of one head: while one tile is in its softmax the
+// other is in its matrix products. Warp 8 brings K and V in tiles of 128 tokens (tiled copies,
+// 128-byte swizzle, two stages each), warp 9 issues S = Q K^T (both operands in shared memory) and
+// O += P V (P in tensor memory, where it overwrites its scores), warps 0-3 and 4-7 run the softmax
+// of A and B, a thread per row; warps 10 and 11 only complete the warpgroup that gives its registers
+// to the softmax (224 and 56 a thread of the 168 at launch). A tile walks only the token tiles that some row of it sees.
+//
+// The score rule is applied to the 128 scores that a thread holds in registers, two at a time
+// (f32x2 instructions):
+//   cap    tanh(x) = x p(x^2) with p of degree 5 while all 128 scores of all 32 rows of the warp stay
+//          inside |x| <= 1, absolute error below 3e-7 (p was fitted for this kernel); otherwise
+//          1 - 2 / (e^2x + 1) from the exponential unit. With the latter alone the exponential unit would
+//          do three operations per score instead of one, and it is as loaded as the tensor cores.
+//   bias   slope * (s - position) is linear in the token inside a tile: one multiply-add per score and one
+//          constant per row and tile; tokens behind the row's position (prefixes) take |.| in full.
+// Weights are rounded to bf16, sums and the accumulator are F32.
+#include "scored.cuh"
+#include "tcgen05.cuh"
+
+namespace yvx {
+
+constexpr int kSpM = 128, kSpN = 128, kSpD = 128, kSpStages = 2, kSpThreads = 384;
+constexpr int kSpHalfBytes = kSpM * 64 * 2;        // [128][64] bf16, swizzled
+constexpr int kSpTileBytes = 2 * kSpHalfBytes;     // 32 KB
+constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 1024 + 512;
+constexpr float kSpRescale = 8.0f;                 // log2 units the maximum may lag behind
+constexpr uint32_t kSpTmemColumns = 512;
+
+struct SpMaps {
+    CUtensorMap query, key, value;
+};
+
+struct SpShared {
+    uint64_t q_full;
+    uint64_t k_full[kSpStages], k_empty[kSpStages], v_full[kSpStages], v_empty[kSpStages];
+    uint64_t s_full[2], p_half[2][2], pv_done[2];
+    uint32_t tmem_base;
+    int first[8], end[8];      // visible run of each softmax warp's rows
+};
+static_assert(sizeof(SpShared) <= 512, "the barrier block outgrew its slot");
+
+// ---- two floats at a time -----------------------------------------------------------------------------
+__device__ __forceinline__ unsigned long long f2_pack(float lo, float hi)
+{
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void f2_unpack(unsigned long long v, float &lo, float &hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long f2_fma(unsigned long long a, unsigned long long b, unsigned long long c)
+{
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b)
+{
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsigned long long b)
+{
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// A row of a finite call that came out non-finite: weights of zero met a NaN or infinity in rows of V that
+// this row does not see (between packed documents, say). It is computed again token by token over what it
+// does see. Rare and slow (a thread per row).
+__device__ __noinline__ bool sp_row_again(const yvx_scored_problem &p, unsigned int b, unsigned int qhead,
+                                          const ScoredRange &range, unsigned int row)
+{
+    const unsigned int kv_head = qhead / (p.query_heads / p.kv_heads);
+    const __nv_bfloat16 *q = reinterpret_cast<const __nv_bfloat16 *>(p.query) + (unsigned long long)b * p.query_session_stride +
+                             (unsigned long long)row * p.query_row_stride +
+                             (unsigned long long)qhead * (p.query_head_stride ? p.query_head_stride : kSpD);
+    const unsigned long long item = (((unsigned long long)b * p.query_rows + row) * p.query_heads + qhead) * kSpD;
+    float o[kSpD], m = -INFINITY, l = 0.0f;
+    for (int d = 0; d < kSpD; ++d) o[d] = 0.0f;
+    for (int t = range.first; t < range.end; ++t) {
+        unsigned long long outer = b, inner = (unsigned int)t;
+        if (p.block_table) {
+            const int page = scored_page(p, b, (unsigned int)t / p.block_tokens);
+            outer = (unsigned long long)(page < 0 ? 0 : page);
+            inner = (unsigned int)t % p.block_tokens;
+        }
+        const __nv_bfloat16 *k = reinterpret_cast<const __nv_bfloat16 *>(p.key) + outer * p.key_outer_stride +
+                                 inner * p.key_token_stride + kv_head * p.key_head_stride;
+        const __nv_bfloat16 *v = reinterpret_cast<const __nv_bfloat16 *>(p.value) + outer * p.value_outer_stride +
+                                 inner * p.value_token_stride + kv_head * p.value_head_stride;
+        float z = 0.0f;
+        for (int d = 0; d < kSpD; ++d) z = fmaf(__bfloat162float(q[d]), __bfloat162float(k[d]), z);
+        z *= p.scale;
+        if (p.cap > 0.0f) z = p.cap * tanhf(z / p.cap);
+        if (p.slopes) z -= p.slopes[qhead] * (float)llabs(range.position - (long long)t);
+        z *= kScoredLog2e;
+        const float fresh = z != z ? INFINITY : fmaxf(m, z);
+        const float keep = m == -INFINITY ? 0.0f : exp2f(m - fresh), weight = exp2f(z - fresh);
+        if (z == -INFINITY && fresh == -INFINITY) continue;
+        l = l * keep + weight;
+        for (int d = 0; d < kSpD; ++d) o[d] = fmaf(weight, __bfloat162float(v[d]), o[d] * keep);
+        m = fresh;
+    }
+    bool finite = true;
+    for (int d = 0; d < kSpD; ++d) {
+        const float x = l == 0.0f ? 0.0f : o[d] / l;
+        finite = finite && isfinite(x);
+        store_output(p.output, p.output_dtype, item + d, x);
+    }
+    return finite;
+}
+
+// grid: one dimension. (session, head) lanes in groups whose K and V fit the L2 together; inside a group the
+// pair of row tiles varies slowest, last rows first, and the lane fastest.
+template <bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kSpThreads, 1)
+scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps maps, const int head_inner,
+                     const unsigned int lane_group)
+{
+    extern __shared__ unsigned char sp_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(sp_raw) + 1023u) & ~uintptr_t(1023));
+    unsigned char *q_smem = smem;                                  // tile A, then tile B
+    unsigned char *k_smem = smem + 2 * kSpTileBytes;
+    unsigned char *v_smem = k_smem + kSpStages * kSpTileBytes;
+    SpShared *sh = reinterpret_cast<SpShared *>(v_smem + kSpStages * kSpTileBytes);
+
+    const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const unsigned int pairs = (p.query_rows + 2 * kSpM - 1) / (2 * kSpM);
+    const unsigned long long per_group = (unsigned long long)pairs * lane_group;
+    const unsigned int within = (unsigned int)(blockIdx.x % per_group);
+    const unsigned int work_lane = (unsigned int)(blockIdx.x / per_group) * lane_group + within % lane_group;
+    if (work_lane >= p.query_heads * p.sessions) return;  // the last group may be short; uniform over the CTA
+    const unsigned int q0 = (pairs - 1u - within / lane_group) * 2u * kSpM;
+    const unsigned int qhead = work_lane % p.query_heads, b = work_lane / p.query_heads;
+    const unsigned int kv_head = qhead / (p.query_heads / p.kv_heads);
+    const unsigned int kv_tokens = admitted_kv_tokens(p.kv_tokens, b, p.kv_tokens_uniform, p.kv_tokens_max, p.status);
+    const long long query_start = scored_query_start(p, b, kv_tokens);
+
+    ScoredRange range = {0, 0, 0};
+    const unsigned int my_row = q0 + threadIdx.x;      // softmax threads: A's rows, then B's
+    const bool exists = threadIdx.x < 2 * kSpM && my_row < p.query_rows;
+    if (exists) range = scored_range(p, b, my_row, kv_tokens, query_start);
+    if (warp < 8) {
+        const bool sees = range.first < range.end;
+        const int lo = __reduce_min_sync(0xffffffffu, sees ? range.first : 0x7fffffff);
+        const int hi = __reduce_max_sync(0xffffffffu, sees ? range.end : 0);
+        if (lane == 0) sh->first[warp] = lo, sh->end[warp] = hi;
+    }
+    if (threadIdx.x == 0) {
+        mbar_init(&sh->q_full, 1);
+        for (int i = 0; i < kSpStages; ++i) {
+            mbar_init(&sh->k_full[i], 1);
+            mbar_init(&sh->k_empty[i], 1);
+            mbar_init(&sh->v_full[i], 1);
+            mbar_init(&sh->v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->p_half[i][0], kSpM);
+            mbar_init(&sh->p_half[i][1], kSpM);
+            mbar_init(&sh->pv_done[i], 1);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(&sh->tmem_base, kSpTmemColumns);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh->tmem_base;
+    // token tiles [from[x], until[x]) of the two row tiles; the CTA walks their hull
+    int hull_first = 0x7fffffff, hull_end = 0, from[2], until[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        int lo = 0x7fffffff, hi = 0;
+#pragma unroll
+        for (int w = 4 * x; w < 4 * x + 4; ++w) {
+            lo = min(lo, sh->first[w]);
+            hi = max(hi, sh->end[w]);
+        }
+        from[x] = hi > 0 ? lo / kSpN : 0;
+        until[x] = (hi + kSpN - 1) / kSpN;
+        hull_first = min(hull_first, lo);
+        hull_end = max(hull_end, hi);
+    }
+    const int start = hull_end > 0 ? hull_first / kSpN : 0, stop = (hull_end + kSpN - 1) / kSpN;
+    auto active = [&](int x, int j) { return j >= from[x] && j < until[x]; };
+    auto fail = [&]() { atomicCAS(p.status, 0, YVX_STATUS_TIMEOUT); };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8) {
+            // ------------------------------ tiled copies ----------------------------------------------
+            if (lane == 0 && stop > start) {
+                mbar_expect_tx(&sh->q_full, 2u * kSpTileBytes);
+                for (int x = 0; x < 2; ++x)
+                    for (int h = 0; h < 2; ++h)
+                        tma_load_4d(q_smem + x * kSpTileBytes + h * kSpHalfBytes, &maps.query, &sh->q_full, 64 * h, (int)qhead,
+                                    (int)(q0 + x * kSpM), (int)b);
+                for (int j = start; j < stop; ++j) {
+                    const unsigned int n = (unsigned int)(j - start), stage = n % kSpStages;
+                    const uint32_t parity = ((n / kSpStages) - 1u) & 1u;
+                    // two runs of 64 tokens (a page may end between them); one behind the hull is not loaded
+                    int outer[2], inner[2], runs = 0;
+                    for (int r = 0; r < 2; ++r) {
+                        const int token = j * kSpN + 64 * r;
+                        if (token >= hull_end) break;
+                        outer[r] = (int)b, inner[r] = token;
+                        if (p.block_table) {
+                            const int page = token + 64 > hull_first ? scored_page(p, b, (unsigned int)token / p.block_tokens) : 0;
+                            outer[r] = page < 0 ? 0 : page;
+                            inner[r] = (int)((unsigned int)token % p.block_tokens);
+                        }
+                        ++runs;
+                    }
+                    for (int operand = 0; operand < 2; ++operand) {
+                        uint64_t *full = operand ? &sh->v_full[stage] : &sh->k_full[stage];
+                        uint64_t *empty = operand ? &sh->v_empty[stage] : &sh->k_empty[stage];
+                        unsigned char *dst = (operand ? v_smem : k_smem) + stage * kSpTileBytes;
+                        const CUtensorMap *map = operand ? &maps.value : &maps.key;
+                        if (n >= (unsigned int)kSpStages && !mbar_wait(empty, parity)) {
+                            fail();
+                            j = stop;
+                            break;
+                        }
+                        mbar_expect_tx(full, (uint32_t)runs * (kSpTileBytes / 2));
+                        for (int r = 0; r < runs; ++r) {
+                            const int c1 = head_inner ? (int)kv_head : inner[r], c2 = head_inner ? inner[r] : (int)kv_head;
+                            tma_load_4d(dst + r * 64 * 128, map, full, 0, c1, c2, outer[r]);
+                            tma_load_4d(dst + kSpHalfBytes + r * 64 * 128, map, full, 64, c1, c2, outer[r]);
+                        }
+                    }
+                }
+            }
+        } else if (warp == 9) {
+            // ------------------------------ matrix products -------------------------------------------
+            // all 32 lanes run converged, one elected lane issues
+            if (stop > start) {
+                constexpr uint32_t idesc_qk = idesc_bf16_f32(kSpM, kSpN, false), idesc_pv = idesc_bf16_f32(kSpM, kSpD, true);
+                const uint32_t q_addr = smem_u32(q_smem), k_addr = smem_u32(k_smem), v_addr = smem_u32(v_smem);
+                auto waited = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
+                auto issue_qk = [&](int x, unsigned int stage) {
+                    const uint32_t ka = k_addr + stage * kSpTileBytes, qa = q_addr + x * kSpTileBytes;
+    #pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t off = (ks >> 2) * kSpHalfBytes + (ks & 3) * 32;
+                        tc_mma_ss_elect(tmem + x * kSpN, smem_desc_sw128(qa + off, 16, 1024), smem_desc_sw128(ka + off, 16, 1024),
+                                        idesc_qk, ks ? 1u : 0u);
+                    }
+                    tc_commit_elect(&sh->s_full[x]);
+                };
+                auto issue_pv = [&](int x, unsigned int stage, unsigned int count) -> bool {
+                    const uint32_t va = v_addr + stage * kSpTileBytes;
+    #pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (!waited(&sh->p_half[x][h], count & 1u)) return false;
+                        tc_fence_after_sync();
+    #pragma unroll
+                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                            tc_mma_ts_elect(tmem + (2 + x) * kSpN, tmem + x * kSpN + kk * 8,
+                                            smem_desc_sw128(va + kk * 2048, kSpHalfBytes, 1024), idesc_pv, (count || kk) ? 1u : 0u);
+                    }
+                    tc_commit_elect(&sh->pv_done[x]);
+                    return true;
+                };
+                bool ok = waited(&sh->q_full, 0) && waited(&sh->k_full[0], 0);
+                if (ok) {
+                    tc_fence_after_sync();
+    #pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        if (active(x, start)) issue_qk(x, 0u);
+                    tc_commit_elect(&sh->k_empty[0]);
+                }
+                for (int j = start; ok && j < stop; ++j) {
+                    const unsigned int n = (unsigned int)(j - start), stage = n % kSpStages, next = (n + 1u) % kSpStages;
+                    const bool more = j + 1 < stop;
+                    ok = waited(&sh->v_full[stage], (n / kSpStages) & 1u);
+                    if (ok && more) ok = waited(&sh->k_full[next], ((n + 1u) / kSpStages) & 1u);
+                    if (ok) tc_fence_after_sync();
+    #pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (ok && active(x, j)) ok = issue_pv(x, stage, (unsigned int)(j - from[x]));
+                        if (ok && active(x, j + 1)) issue_qk(x, next);
+                    }
+                    if (!ok) break;
+                    tc_commit_elect(&sh->v_empty[stage]);
+                    if (more) tc_commit_elect(&sh->k_empty[next]);
+                }
+                if (!ok && lane == 0) fail();
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ------------------------------ softmax ----------------------------------------------------
+        const int x = (int)(warp >> 2);
+        const uint32_t lane_base = tmem + (((warp & 3u) * 32u) << 16);
+        const uint32_t s_col = lane_base + x * kSpN, o_col = lane_base + (2u + x) * kSpN;
+        const unsigned int tile_row = threadIdx.x & 127u;
+        const int my_from = from[x], my_until = until[x];
+        const float mul = (CAP ? p.cap : p.scale) * kScoredLog2e;   // what a held score is multiplied with
+        const float slope2 = BIAS && exists ? p.slopes[qhead] * kScoredLog2e : 0.0f;
+        const float slope_held = BIAS ? slope2 / mul : 0.0f;
+        unsigned long long poly[6];
+        float inside = 0.0f, to_unit = 0.0f;
+        if (CAP) {
+            // tanh(x) = x (a0 + a1 x^2 + ...), the powers of scale / cap folded into the coefficients
+            constexpr float a[6] = {0.9999968538734331f,  -0.33324003815111036f, 0.13253525482390585f,
+                                    -0.05097287022853855f, 0.016114189461285185f, -0.0028394691373163504f};
+            to_unit = p.scale / p.cap;
+            inside = p.cap / p.scale;
+            float power = to_unit;
+#pragma unroll
+            for (int i = 0; i < 6; ++i) {
+                poly[i] = f2_pack(a[i] * power, a[i] * power);
+                power *= to_unit * to_unit;
+            }
+        }
+        float m_used = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int j = my_from; j < my_until; ++j) {
+            const uint32_t parity = (unsigned int)(j - my_from) & 1u;
+            if (!mbar_wait(&sh->s_full[x], parity)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_ld32(s_col + 32 * i, s[i]);
+            tmem_wait_ld();
+            const int k0 = j * kSpN;
+            if (k0 < hull_first || k0 + kSpN > hull_end) {
+                // tokens that no row of the CTA sees: their rows of V may hold anything and become zero
+                const unsigned int n = (unsigned int)(j - start), stage = n % kSpStages;
+                if (!mbar_wait(&sh->v_full[stage], (n / kSpStages) & 1u)) {
+                    ok = false;
+                    break;
+                }
+                const int token = k0 + (int)tile_row;
+                if (token < hull_first || token >= hull_end) {
+                    unsigned char *v_row = v_smem + stage * kSpTileBytes + tile_row * 128u;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        *reinterpret_cast<uint4 *>(v_row + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4 *>(v_row + kSpHalfBytes + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                }
+                fence_proxy_async();
+            }
+            float row_top = -INFINITY;
+            if (CAP) {
+                // largest and smallest score; tanh keeps their order
+                float hi[2] = {-INFINITY, -INFINITY}, lo[2] = {INFINITY, INFINITY};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        const float s0 = __uint_as_float(s[i][c]), s1 = __uint_as_float(s[i][c + 1]);
+                        hi[(c >> 1) & 1] = max3(hi[(c >> 1) & 1], s0, s1);
+                        lo[(c >> 1) & 1] = min3(lo[(c >> 1) & 1], s0, s1);
+                    }
+                row_top = fmaxf(hi[0], hi[1]);
+                row_top = fmaf(-2.0f, __frcp_rn(exp2_approx(row_top * to_unit * (2.0f * kScoredLog2e)) + 1.0f), 1.0f);
+                if (__all_sync(0xffffffffu, fmaxf(fmaxf(hi[0], hi[1]), -fminf(lo[0], lo[1])) <= inside)) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            const unsigned long long v = f2_pack(__uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1]));
+                            const unsigned long long w = f2_mul(v, v);
+                            unsigned long long y = f2_fma(poly[5], w, poly[4]);
+                            y = f2_fma(y, w, poly[3]);
+                            y = f2_fma(y, w, poly[2]);
+                            y = f2_fma(y, w, poly[1]);
+                            y = f2_fma(y, w, poly[0]);
+                            y = f2_mul(y, v);
+                            float lo, hi;
+                            f2_unpack(y, lo, hi);
+                            s[i][c] = __float_as_uint(lo);
+                            s[i][c + 1] = __float_as_uint(hi);
+                        }
+                } else {
+                    const float unit = to_unit * (2.0f * kScoredLog2e);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            const float t = exp2_approx(__uint_as_float(s[i][c]) * unit);
+                            s[i][c] = __float_as_uint(fmaf(-2.0f, __frcp_rn(t + 1.0f), 1.0f));
+                        }
+                }
+            }
+            float ahead_f = 0.0f;
+            if (BIAS) {
+                const int ahead = (int)max(min((long long)k0 - range.position, 0x3fffffffll), -0x3fffffffll);
+                if (__all_sync(0xffffffffu, (long long)min(range.end, k0 + kSpN) <= range.position + 1)) {
+                    ahead_f = (float)ahead;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            s[i][c] = __float_as_uint(fmaf((float)(32 * i + c), slope_held, __uint_as_float(s[i][c])));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            s[i][c] = __float_as_uint(fmaf(-slope_held, fabsf((float)(ahead + 32 * i + c)), __uint_as_float(s[i][c])));
+                }
+            }
+            const bool masked = k0 < range.first || k0 + kSpN > range.end;
+            if (masked) {
+                const int lo = range.first - k0, hi = range.end - k0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (32 * i + c < lo || 32 * i + c >= hi) s[i][c] = 0xff800000u;
+            }
+            if (!CAP || BIAS || __any_sync(0xffffffffu, masked)) {
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2)
+                        mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1]));
+                row_top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+            }
+            const float m_tile = fmaf(row_top, mul, slope2 * ahead_f);
+            const bool grow = m_tile > m_used + kSpRescale || (m_used == -INFINITY && m_tile > -INFINITY);
+            if (__any_sync(0xffffffffu, grow)) {
+                const float m_new = fmaxf(m_used, m_tile);
+                const float factor = m_new == -INFINITY ? 1.0f : exp2_approx(m_used - m_new);
+                l *= factor;
+                m_used = m_new;
+                if (j > my_from) {
+                    // O may be touched once the previous tile's P V has landed
+                    if (!mbar_wait(&sh->pv_done[x], parity ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t o[16];
+                        tmem_ld16(o_col + 16 * i, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * factor);
+                        tmem_st16(o_col + 16 * i, o);
+                    }
+                    tmem_wait_st();
+                }
+            }
+            const float offset = m_used == -INFINITY ? 0.0f : fmaf(slope2, ahead_f, -m_used);
+            const unsigned long long mul2 = f2_pack(mul, mul), offset2 = f2_pack(offset, offset);
+            unsigned long long sum2 = 0ull;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t packed[32];
+#pragma unroll
+                for (int i = 2 * h; i < 2 * h + 2; ++i)
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        float e0, e1;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1])), mul2, offset2), e0, e1);
+                        e0 = exp2_approx(e0);
+                        e1 = exp2_approx(e1);
+                        sum2 = f2_add(sum2, f2_pack(e0, e1));
+                        packed[(i & 1) * 16 + (c >> 1)] = pack_bf16(e0, e1);
+                    }
+                tmem_st32(s_col + 32 * h, packed);
+                tmem_wait_st();
+                tc_fence_before_sync();
+                mbar_arrive(&sh->p_half[x][h]);   // weights of tokens 64 h .. 64 h + 63
+            }
+            float sum_lo, sum_hi;
+            f2_unpack(sum2, sum_lo, sum_hi);
+            l += sum_lo + sum_hi;
+        }
+        // ------------------------------ epilogue ----------------------------------------------------
+        const bool any = my_until > my_from;
+        if (ok && any) ok = mbar_wait(&sh->pv_done[x], (unsigned int)(my_until - my_from - 1) & 1u);
+        if (!__all_sync(0xffffffffu, ok)) {
+            fail();
+        } else {
+            tc_fence_after_sync();
+            const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+            const unsigned long long item =
+                (((unsigned long long)b * p.query_rows + (exists ? my_row : 0u)) * p.query_heads + qhead) * kSpD;
+            bool finite = l == l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t o[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) o[c] = 0u;
+                if (any) {   // every lane takes part; only rows that exist store
+                    tmem_ld32(o_col + 32 * i, o);
+                    tmem_wait_ld();
+                }
+                float v[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    v[c] = range.first < range.end ? __uint_as_float(o[c]) * inverse : 0.0f;
+                    finite = finite && isfinite(v[c]);
+                }
+                if (!exists) continue;
+                if (p.output_dtype == YVEX_DTYPE_BF16) {
+                    uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<unsigned short *>(p.output) + item + 32 * i);
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4)
+                        dst[q4] = make_uint4(pack_bf16(v[8 * q4], v[8 * q4 + 1]), pack_bf16(v[8 * q4 + 2], v[8 * q4 + 3]),
+                                             pack_bf16(v[8 * q4 + 4], v[8 * q4 + 5]), pack_bf16(v[8 * q4 + 6], v[8 * q4 + 7]));
+                } else {
+                    float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.output) + item + 32 * i);
+#pragma unroll
+                    for (int q4 = 0; q4 < 8; ++q4)
+                        dst[q4] = make_float4(v[4 * q4], v[4 * q4 + 1], v[4 * q4 + 2], v[4 * q4 + 3]);
+                }
+            }
+            if (exists && !finite) {
+                if (p.row_first || p.row_end) finite = sp_row_again(p, b, qhead, range, my_row);
+                if (!finite) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 9) tmem_dealloc(tmem, kSpTmemColumns);
+}
+
+bool scored_encode_rows(CUtensorMap *map, const void *base, int element_bytes, unsigned long long token_stride,
+                        unsigned long long head_stride, unsigned long long outer_stride, unsigned long long tokens,
+                        unsigned long long heads, unsigned long long outer, bool head_inner, unsigned int box_tokens);
+
+// 2: launched and final (nothing to fold), 0: not this kernel's shape, negative: an error.
+int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
+{
+    const unsigned long long head_stride = p.query_head_stride ? p.query_head_stride : kSpD;
+    if (p.head_dim != (unsigned)kSpD || p.query_dtype != YVEX_DTYPE_BF16 || p.kv_code != YVX_KV_PLAIN ||
+        p.kv_dtype != YVEX_DTYPE_BF16 || (reinterpret_cast<uintptr_t>(p.output) & 15u) ||
+        (p.block_table && p.block_tokens % 64u) || head_stride > p.query_row_stride)
+        return 0;
+    const bool head_inner = p.key_head_stride < p.key_token_stride;
+    if ((p.value_head_stride < p.value_token_stride) != head_inner) return 0;
+    const unsigned long long tokens = p.block_table ? p.block_tokens : p.kv_tokens_max;
+    const unsigned long long outer = p.block_table ? p.pool_blocks : p.sessions;
+    SpMaps maps;
+    if (!scored_encode_rows(&maps.query, p.query, 2, p.query_row_stride, head_stride, p.query_session_stride, p.query_rows,
+                            p.query_heads, p.sessions, true, kSpM) ||
+        !scored_encode_rows(&maps.key, p.key, 2, p.key_token_stride, p.key_head_stride, p.key_outer_stride, tokens,
+                            p.kv_heads, outer, head_inner, 64u) ||
+        !scored_encode_rows(&maps.value, p.value, 2, p.value_token_stride, p.value_head_stride, p.value_outer_stride,
+                            tokens, p.kv_heads, outer, head_inner, 64u))
+        return 0;
+    // lanes whose K + V fit half of the 126 MB L2 together form a group
+    const unsigned long long lanes = (unsigned long long)p.query_heads * p.sessions, group = p.query_heads / p.kv_heads;
+    unsigned long long streams = (64ull << 20) / ((unsigned long long)p.kv_tokens_max * kSpD * 4ull);
+    if (streams < 1ull) streams = 1ull;
+    const unsigned long long lane_group = streams * group < lanes ? streams * group : lanes;
+    const unsigned long long pairs = (p.query_rows + 2ull * kSpM - 1ull) / (2ull * kSpM);
+    const unsigned long long ctas = (lanes + lane_group - 1ull) / lane_group * lane_group * pairs;
+    if (lanes > 0xffffffffull || ctas > 0x7fffffffull) return 0;
+    const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
+    void (*const kernels[4])(const yvx_scored_problem, const SpMaps, const int, const unsigned int) = {
+        scored_prompt_kernel<false, false>, scored_prompt_kernel<true, false>, scored_prompt_kernel<false, true>,
+        scored_prompt_kernel<true, true>};
+    const auto kernel = kernels[(cap ? 1 : 0) + (bias ? 2 : 0)];
+    YVX_CUDA_TRY(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpSmemBytes));
+    kernel<<<dim3((unsigned int)ctas, 1, 1), kSpThreads, kSpSmemBytes, stream>>>(p, maps, head_inner ? 1 : 0,
+                                                                              (unsigned int)lane_group);
+    const int rc = yvx_cuda_check(cudaGetLastError(), "scored_prompt_kernel");
+    return rc != 0 ? rc : 2;
+}
+
+}  // namespace yvx

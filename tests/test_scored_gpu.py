@@ -61,6 +61,61 @@ def test_decode_kernel(backend, lengths, rows, heads, kv_heads, fields, chunk):
     Case(12, lengths, rows, heads, kv_heads, 128, **fields).check(backend, path, chunk=chunk)
 
 
+DOCS = [[100, 1, 130, 300, 0, 69]]
+PROMPT = [
+    # lengths, rows, heads, kv_heads, fields
+    ([130], 130, 2, 1, {}),
+    ([300, 257], 200, 2, 2, dict(out_dtype=BF16)),
+    ([129, 70], 70, 4, 4, dict(cap=50.0, q_scale=3.0)),
+    ([400, 390], 300, 2, 1, dict(cap=2.0, q_scale=8.0)),              # scores far outside the polynomial
+    ([300], 300, 4, 2, dict(slopes=True)),
+    ([520, 500], 500, 2, 1, dict(slopes=True, cap=20.0, q_scale=4.0, causal=False)),
+    ([600], 600, 2, 1, dict(ranges="documents")),
+    ([600], 600, 2, 1, dict(ranges="documents", slopes=True, cap=20.0)),
+    ([600], 600, 2, 1, dict(ranges="prefix", slopes=True)),
+    ([700, 650], 270, 2, 1, dict(window=140)),
+    ([700, 300], 90, 4, 2, dict(window=300, page=64)),
+    ([700, 300], 90, 4, 2, dict(page=128, pad=8, slopes=True)),
+    ([300, 290], 280, 2, 1, dict(head_major=True, kv_max=513, cap=5.0)),
+    ([300, 200], 150, 2, 1, dict(query_start=[10, 300])),
+    ([390, 261], 200, 4, 2, dict(cache=E4M3, page=64)),
+    ([390, 261], 200, 4, 2, dict(cache=I8, page=16, window=90, cap=9.0, q_scale=4.0)),
+    ([200, 210], 130, 2, 1, dict(page=16)),
+    ([0, 300], 257, 2, 1, {}),
+]
+
+
+@pytest.mark.parametrize("lengths,rows,heads,kv_heads,fields", PROMPT)
+def test_prompt_kernel(backend, lengths, rows, heads, kv_heads, fields):
+    fields = dict(fields)
+    if fields.get("ranges") == "documents":
+        fields["ranges"] = documents(DOCS, rows)
+    elif fields.get("ranges") == "prefix":
+        fields["ranges"] = documents([[rows]], rows, [250])
+    Case(14, lengths, rows, heads, kv_heads, 128, **fields).check(backend, "prompt")
+
+
+def test_prompt_rows_with_gaps_and_padding(backend):
+    # packed documents with padding between them: keys and values of the padding are NaN
+    first, end = np.zeros((1, 400), int), np.zeros((1, 400), int)
+    for lo, hi in ((0, 90), (100, 101), (140, 330), (350, 390)):
+        first[0, lo:hi], end[0, lo:hi] = lo, np.arange(lo, hi) + 1
+    Case(15, [400], 400, 2, 1, 128, ranges=(first, end)).check(backend, "prompt")
+    Case(15, [400], 400, 2, 1, 128, ranges=(first, end), cache=E4M3, page=64, slopes=True).check(backend, "prompt")
+
+
+def test_pages_in_front_of_a_window_may_be_gone(backend):
+    for rows, fields in ((1, dict(cache=E4M3, page=16)), (1, dict(page=64)), (100, dict(cache=I8, page=16)), (100, dict(page=64)),
+                         (100, dict(page=16))):
+        for general in (False, True):
+            c = Case(16, [700, 650], rows, 4, 2, 128, window=50, **fields)
+            for b in range(2):
+                c.table[b, :int(c.first[b].min()) // c.page] = -1
+            got, status = c.launch(backend, c.plan(backend, c.problem(backend, general)))
+            want, spread, size = c.answer()
+            assert status == 0 and np.all(np.abs(got - want) <= c.allowed(want, spread, size, "prompt"))
+
+
 def test_one_loud_token_does_not_hide_many_quiet_ones(backend):
     # weights far below the largest carry half of the result: they have to survive their rounding
     for fields, path in ((dict(page=64), "decode_bf16"), (dict(cache=E4M3, page=64), "decode_codes")):
