@@ -34,6 +34,7 @@ template <int CODE>
 struct SdShape {
     static constexpr int operand_bytes = kSdTokens * kSdDim * (CODE ? 1 : 2);  // one K or V tile
     static constexpr int stages = kSdRingBytes / (2 * operand_bytes);
+    static constexpr int pair = CODE ? 2 : 1;
 };
 constexpr int kSdMaxStages = SdShape<1>::stages;
 constexpr int kSdSmemBytes = kSdRingBytes + 16 * kSdQRowBytes + kSdMaxStages * kSdWarps * 8 + kSdMaxStages * 16 + 64 + 64 + 1024;
@@ -242,104 +243,135 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
 
-    for (unsigned int i = 0; i < tiles; ++i) {
-        const unsigned int stage = i % kStages;
-        if (!mbar_wait(&full[stage], (i / kStages) & 1u)) {
+    // kPair tiles per pass: their scores and weights are independent, which hides the latency of the matrix
+    // and conversion chains (a warp's issue slots are 40 % busy with one tile of codes at a time)
+    constexpr int kPair = Shape::pair, kCols = 2 * kPair;
+    for (unsigned int i = 0; i < tiles; i += kPair) {
+        unsigned int stage[kPair];
+        bool there[kPair], ok = true;
+#pragma unroll
+        for (int u = 0; u < kPair; ++u) {
+            there[u] = i + u < tiles;
+            stage[u] = (i + u) % kStages;
+            if (there[u]) ok = ok && mbar_wait(&full[stage[u]], ((i + u) / kStages) & 1u);
+        }
+        if (!ok) {
             atomicCAS(p.status, 0, YVX_STATUS_TIMEOUT);
             break;
         }
-        const unsigned char *k_tile = ring + stage * 2 * kOperand;
-        const uint32_t k_base = smem_u32(k_tile), v_base = k_base + kOperand;
-        const int token0 = t0 + (int)(i * kSdTokens) + 16 * (int)warp;
-        float2 scales = make_float2(1.0f, 1.0f);
-        if (CODE) scales = scale_smem[stage * kSdWarps + warp];
-
-        // ---- S = Q K^T over 16 tokens: column 8 n + j of the tile is token 8 n + j ----------------
-        float sc[2][4];
+        const int token0 = t0 + (int)(i * kSdTokens) + 16 * (int)warp;   // tile u: + 64 u
+        float2 scales[kPair];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int u = 0; u < kPair; ++u) {
+            scales[u] = make_float2(0.0f, 0.0f);
+            if (CODE && there[u]) scales[u] = scale_smem[stage[u] * kSdWarps + warp];
+        }
+
+        // ---- S = Q K^T over 16 tokens of a tile: column 8 n + j of tile u is its token 8 n + j ------
+        float sc[kCols][4];
+#pragma unroll
+        for (int n = 0; n < kCols; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
-        if (CODE) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const unsigned int row = 16u * warp + 8u * n + g;
+        for (int u = 0; u < kPair; ++u) {
+            if (!there[u]) continue;
+            const unsigned char *k_tile = ring + stage[u] * 2 * kOperand;
+            if (CODE) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint4 kq = *reinterpret_cast<const uint4 *>(k_tile + row * 128u + (((2u * c + half) ^ (row & 7u)) << 4));
-                    const uint32_t words[4] = {kq.x, kq.y, kq.z, kq.w};
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t b0, b1;
-                        sd_codes<CODE>(words[w], b0, b1);
-                        mma_f16(sc[n], qa[4 * half + w], b0, b1);
+                    for (int n = 0; n < 2; ++n) {
+                        const unsigned int row = 16u * warp + 8u * n + g;
+                        const uint4 kq = *reinterpret_cast<const uint4 *>(k_tile + row * 128u + (((2u * c + half) ^ (row & 7u)) << 4));
+                        const uint32_t words[4] = {kq.x, kq.y, kq.z, kq.w};
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            uint32_t b0, b1;
+                            sd_codes<CODE>(words[w], b0, b1);
+                            mma_f16(sc[2 * u + n], qa[4 * half + w], b0, b1);
+                        }
                     }
                 }
-            }
-        } else {
-            const unsigned int j = lane >> 3, r = lane & 7u;
-            const unsigned int token = 16u * warp + 8u * (j >> 1) + r;
+            } else {
+                const uint32_t k_base = smem_u32(k_tile);
+                const unsigned int j = lane >> 3, r = lane & 7u;
+                const unsigned int token = 16u * warp + 8u * (j >> 1) + r;
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                const unsigned int chunk = 2u * (ks & 3) + (j & 1u);
-                uint32_t kb[4];
-                ldmatrix_x4(kb, k_base + (ks >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
-                mma_bf16(sc[0], qa[ks], kb[0], kb[1]);
-                mma_bf16(sc[1], qa[ks], kb[2], kb[3]);
+                for (int ks = 0; ks < 8; ++ks) {
+                    const unsigned int chunk = 2u * (ks & 3) + (j & 1u);
+                    uint32_t kb[4];
+                    ldmatrix_x4(kb, k_base + (ks >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
+                    mma_bf16(sc[2 * u], qa[ks], kb[0], kb[1]);
+                    mma_bf16(sc[2 * u + 1], qa[ks], kb[2], kb[3]);
+                }
             }
         }
         // ---- the score rule, in log2 units --------------------------------------------------------
-        const float unit0 = mul[0] * scales.x, unit1 = mul[1] * scales.x;
+        if (capped || biased) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float z = sc[n][e] * (e < 2 ? unit0 : unit1);
-                if (capped) {
-                    // tanh from one exponential: 1 - 2 / (e^2x + 1), absolute error a few 2^-24
-                    const float t = exp2_approx(z * inverse_cap * (2.0f * kScoredLog2e));
-                    z = p.cap - 2.0f * p.cap * __frcp_rn(t + 1.0f);
-                }
-                if (biased) {
-                    const int distance = position[e >> 1] - (token0 + 8 * n + 2 * (int)c + (e & 1));
-                    z = fmaf(-slope[e >> 1], fabsf((float)distance), z);
-                }
-                sc[n][e] = z * kScoredLog2e;
-            }
-        // ---- visibility: tokens that no row of the CTA sees may hold anything in V ----------------
-        uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;
-        if (token0 < inner_first || token0 + 16 > inner_end) {
-            uint32_t seen = 0u;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < kCols; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int token = token0 + 8 * n + 2 * (int)c + (e & 1);
-                    const bool visible = token >= first[e >> 1] && token < end[e >> 1];
+                    float z = sc[n][e] * (mul[e >> 1] * (CODE ? scales[n >> 1].x : 1.0f));
+                    if (capped) {
+                        // tanh from one exponential: 1 - 2 / (e^2x + 1), absolute error a few 2^-23
+                        const float t = exp2_approx(z * inverse_cap * (2.0f * kScoredLog2e));
+                        z = fmaf(-2.0f * p.cap, rcp_approx(t + 1.0f), p.cap);
+                    }
+                    if (biased) {
+                        const int distance = position[e >> 1] - (token0 + 64 * (n >> 1) + 8 * (n & 1) + 2 * (int)c + (e & 1));
+                        z = fmaf(-slope[e >> 1], fabsf((float)distance), z);
+                    }
+                    sc[n][e] = z * kScoredLog2e;
+                }
+        } else {
+#pragma unroll
+            for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[n][e] *= mul[e >> 1] * kScoredLog2e * (CODE ? scales[n >> 1].x : 1.0f);
+        }
+        // ---- visibility: tokens that no row of the CTA sees may hold anything in V ----------------
+        uint32_t keep_lo[kPair], keep_hi[kPair];
+#pragma unroll
+        for (int u = 0; u < kPair; ++u) keep_lo[u] = keep_hi[u] = 0xffffffffu;
+        if (token0 < inner_first || token0 + 64 * (kPair - 1) + 16 > inner_end || !there[kPair - 1]) {
+            uint32_t seen = 0u;
+#pragma unroll
+            for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int token = token0 + 64 * (n >> 1) + 8 * (n & 1) + 2 * (int)c + (e & 1);
+                    const bool visible = there[n >> 1] && token >= first[e >> 1] && token < end[e >> 1];
                     if (!visible) sc[n][e] = -INFINITY;
                     seen |= (visible ? 1u : 0u) << (2 * n + (e & 1));
                 }
 #pragma unroll
             for (int offset = 4; offset < 32; offset <<= 1) seen |= __shfl_xor_sync(0xffffffffu, seen, offset);
-            keep_lo = (seen & 1u ? 0x0000ffffu : 0u) | (seen & 2u ? 0xffff0000u : 0u);
-            keep_hi = (seen & 4u ? 0x0000ffffu : 0u) | (seen & 8u ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int u = 0; u < kPair; ++u) {
+                const uint32_t bits = seen >> (4 * u);
+                keep_lo[u] = (bits & 1u ? 0x0000ffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
+                keep_hi[u] = (bits & 4u ? 0x0000ffffu : 0u) | (bits & 8u ? 0xffff0000u : 0u);
+            }
         }
         // ---- online softmax with a lazy maximum ----------------------------------------------------
+        float top[2];
         bool grow = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float bound = m[h] + kSlack;  // -inf while the row has seen nothing
+            top[h] = fmaxf(sc[0][2 * h], sc[0][2 * h + 1]);
 #pragma unroll
-            for (int n = 0; n < 2; ++n) grow = grow || sc[n][2 * h] > bound || sc[n][2 * h + 1] > bound;
+            for (int n = 1; n < kCols; ++n) top[h] = max3(top[h], sc[n][2 * h], sc[n][2 * h + 1]);
+            grow = grow || top[h] > m[h] + kSlack;   // m is -inf while the row has seen nothing
         }
         if (__any_sync(0xffffffffu, grow)) {
             float keep[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float top = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float fresh = fmaxf(m[h], top);
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                const float fresh = fmaxf(m[h], top[h]);
                 keep[h] = fresh == -INFINITY ? 1.0f : exp2_approx(m[h] - fresh);
                 m[h] = fresh;
                 l[h] *= keep[h];
@@ -352,10 +384,12 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                 o[n][3] *= keep[1];
             }
         }
-        float ratio = 1.0f;
+        float ratio[kPair];
         if (CODE) {
-            const float size = fabsf(scales.y);
-            if (size > v_ref) {  // the warp's 16 tokens share a page: uniform
+            float size = fabsf(scales[0].y);
+#pragma unroll
+            for (int u = 1; u < kPair; ++u) size = fmaxf(size, fabsf(scales[u].y));
+            if (size > v_ref) {  // a warp's 16 tokens of a tile share a page: uniform
                 const float factor = v_ref / size;
 #pragma unroll
                 for (int n = 0; n < 16; ++n)
@@ -364,61 +398,69 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                 v_ref = size;
                 v_inverse = 1.0f / size;
             }
-            ratio = scales.y * v_inverse;
+#pragma unroll
+            for (int u = 0; u < kPair; ++u) ratio[u] = scales[u].y * v_inverse;
         }
         float offset[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) offset[h] = m[h] == -INFINITY ? 0.0f : kLift - m[h];
-        uint32_t p_head[4], p_tail[4];
+        uint32_t p_head[kPair][4], p_tail[kPair][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < kCols; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float p0 = exp2_approx(sc[n][2 * h] + offset[h]), p1 = exp2_approx(sc[n][2 * h + 1] + offset[h]);
                 l[h] += p0 + p1;
                 if (CODE) {
-                    p_head[2 * n + h] = pack_f16(p0 * ratio, p1 * ratio);
+                    p_head[n >> 1][2 * (n & 1) + h] = pack_f16(p0 * ratio[n >> 1], p1 * ratio[n >> 1]);
                 } else {
                     const uint32_t head = pack_bf16(p0, p1);
-                    p_head[2 * n + h] = head;
-                    p_tail[2 * n + h] = pack_bf16(p0 - __uint_as_float(head << 16), p1 - __uint_as_float(head & 0xffff0000u));
+                    p_head[n >> 1][2 * (n & 1) + h] = head;
+                    p_tail[n >> 1][2 * (n & 1) + h] = pack_bf16(p0 - __uint_as_float(head << 16), p1 - __uint_as_float(head & 0xffff0000u));
                 }
             }
         // ---- O += P V -------------------------------------------------------------------------------
         const unsigned int j = lane >> 3, r = lane & 7u;
         const unsigned int token = 16u * warp + 8u * (j & 1u) + r;
-        if (CODE) {
-            // A transposed 8x8 block of 16-bit pairs gives a thread two tokens of two adjacent dims; columns of
-            // the accumulator tile 2 ch + parity are the dims 16 ch + 2 g + parity.
 #pragma unroll
-            for (int np = 0; np < 4; ++np) {
-                uint32_t raw[4];
-                ldmatrix_x4_trans(raw, v_base + token * 128u + (((2u * np + (j >> 1)) ^ (token & 7u)) << 4));
+        for (int u = 0; u < kPair; ++u) {
+            if (!there[u]) continue;
+            const uint32_t v_base = smem_u32(ring + stage[u] * 2 * kOperand + kOperand);
+            if (CODE) {
+                // A transposed 8x8 block of 16-bit pairs gives a thread two tokens of two adjacent dims; columns
+                // of the accumulator tile 2 ch + parity are the dims 16 ch + 2 g + parity.
 #pragma unroll
-                for (int ch = 0; ch < 2; ++ch) {
-                    uint32_t lo, hi, lo_even, lo_odd, hi_even, hi_odd;
-                    asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(lo) : "r"(raw[2 * ch]));
-                    asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(hi) : "r"(raw[2 * ch + 1]));
-                    sd_codes<CODE>(lo, lo_even, lo_odd);
-                    sd_codes<CODE>(hi, hi_even, hi_odd);
-                    mma_f16(o[4 * np + 2 * ch], p_head, lo_even & keep_lo, hi_even & keep_hi);
-                    mma_f16(o[4 * np + 2 * ch + 1], p_head, lo_odd & keep_lo, hi_odd & keep_hi);
+                for (int np = 0; np < 4; ++np) {
+                    uint32_t raw[4];
+                    ldmatrix_x4_trans(raw, v_base + token * 128u + (((2u * np + (j >> 1)) ^ (token & 7u)) << 4));
+#pragma unroll
+                    for (int ch = 0; ch < 2; ++ch) {
+                        uint32_t lo, hi, lo_even, lo_odd, hi_even, hi_odd;
+                        asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(lo) : "r"(raw[2 * ch]));
+                        asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(hi) : "r"(raw[2 * ch + 1]));
+                        sd_codes<CODE>(lo, lo_even, lo_odd);
+                        sd_codes<CODE>(hi, hi_even, hi_odd);
+                        mma_f16(o[4 * np + 2 * ch], p_head[u], lo_even & keep_lo[u], hi_even & keep_hi[u]);
+                        mma_f16(o[4 * np + 2 * ch + 1], p_head[u], lo_odd & keep_lo[u], hi_odd & keep_hi[u]);
+                    }
                 }
-            }
-        } else {
+            } else {
 #pragma unroll
-            for (int np = 0; np < 8; ++np) {
-                const unsigned int chunk = 2u * (np & 3) + (j >> 1);
-                uint32_t vb[4];
-                ldmatrix_x4_trans(vb, v_base + (np >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
-                mma_bf16(o[2 * np], p_head, vb[0] & keep_lo, vb[1] & keep_hi);
-                mma_bf16(o[2 * np], p_tail, vb[0] & keep_lo, vb[1] & keep_hi);
-                mma_bf16(o[2 * np + 1], p_head, vb[2] & keep_lo, vb[3] & keep_hi);
-                mma_bf16(o[2 * np + 1], p_tail, vb[2] & keep_lo, vb[3] & keep_hi);
+                for (int np = 0; np < 8; ++np) {
+                    const unsigned int chunk = 2u * (np & 3) + (j >> 1);
+                    uint32_t vb[4];
+                    ldmatrix_x4_trans(vb, v_base + (np >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
+                    mma_bf16(o[2 * np], p_head[u], vb[0] & keep_lo[u], vb[1] & keep_hi[u]);
+                    mma_bf16(o[2 * np], p_tail[u], vb[0] & keep_lo[u], vb[1] & keep_hi[u]);
+                    mma_bf16(o[2 * np + 1], p_head[u], vb[2] & keep_lo[u], vb[3] & keep_hi[u]);
+                    mma_bf16(o[2 * np + 1], p_tail[u], vb[2] & keep_lo[u], vb[3] & keep_hi[u]);
+                }
             }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[stage]);
+#pragma unroll
+        for (int u = 0; u < kPair; ++u)
+            if (lane == 0 && there[u]) mbar_arrive(&empty[stage[u]]);
     }
 
     // ---- merge the four warps and publish ------------------------------------------------------------

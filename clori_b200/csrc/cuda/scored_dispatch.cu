@@ -29,8 +29,8 @@ static int scored_check(const yvx_scored_problem *p)
         return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: the block table does not cover kv_tokens_max");
     if (!p->chunk_tokens || (p->chunk_tokens & 63u) || !p->max_splits)
         return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: yvx_cuda_scored_plan has not been called");
-    if (p->kv_tokens_max > 0x7fffffffu - 1024u || p->sessions > 65535u || p->max_splits > 65535u)
-        return scored_refuse(YVEX_ERR_BOUNDS, "scored attention: lengths below 2^31 - 1024, at most 65535 sessions and splits");
+    if (p->kv_tokens_max > 0x7fffffffu - 1024u || p->sessions > 65535u || p->max_splits > 8192u)
+        return scored_refuse(YVEX_ERR_BOUNDS, "scored attention: lengths below 2^31 - 1024, at most 65535 sessions and 8192 splits");
     return 0;
 }
 
@@ -96,7 +96,7 @@ void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
         }
         if (fill >= 0.9) break;
     }
-    while ((span + best - 1ull) / best > 65535ull) best += 64u;
+    while ((span + best - 1ull) / best > 8192ull) best += 64u;
     if (lanes >= wave && vectors > 64ull) best = (unsigned int)span;  // many rows fill the machine by themselves
     p->chunk_tokens = best;
     p->max_splits = (unsigned int)((span + best - 1ull) / best);

@@ -224,42 +224,76 @@ __global__ void __launch_bounds__(kSgThreads) scored_general_kernel(const yvx_sc
     }
 }
 
-// One CTA per item. Every warp reads all (maximum, sum) pairs, so the weights need no exchange; the
-// warps share the splits and are added in warp order: the result depends on the inputs alone.
-constexpr int kScThreads = 128, kScWarps = kScThreads / 32, kScDims = 8;
+// One CTA per item. The splits' weights go to shared memory once; then eight warps share the splits, a lane
+// owns four adjacent dims at a time and the rows of four splits are in flight together. Warps are added in
+// order: the result depends on the inputs alone.
+constexpr int kScThreads = 256, kScWarps = kScThreads / 32, kScBatch = 4;
 
 __global__ void __launch_bounds__(kScThreads) scored_combine_kernel(const yvx_scored_problem p)
 {
-    __shared__ float total[kScWarps][256];
+    extern __shared__ float weight[];               // [max_splits]
+    __shared__ float total[kScWarps][256 + 4];
+    __shared__ float warp_top[kScWarps], warp_sum_of[kScWarps];
     const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, hd = p.head_dim;
     const unsigned long long item = blockIdx.x;
     pdl_wait();
     const float *parts = scored_partial(p, item, 0u);
     const unsigned long long pitch = hd + 4ull;
     float top = -INFINITY;
-    for (unsigned int j = lane; j < p.max_splits; j += 32u)
-        if (parts[j * pitch + hd + 1] != 0.0f) top = fmaxf(top, parts[j * pitch + hd]);
+    for (unsigned int j = threadIdx.x; j < p.max_splits; j += kScThreads) {
+        const float m = parts[j * pitch + hd], l = parts[j * pitch + hd + 1];
+        weight[j] = l == 0.0f ? -INFINITY : m;
+        if (l != 0.0f) top = fmaxf(top, m);
+    }
     top = warp_max(top);
-    float sum = 0.0f, acc[kScDims];
+    if (lane == 0) warp_top[warp] = top;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kScDims; ++i) acc[i] = 0.0f;
-    for (unsigned int j = lane; j < p.max_splits; j += 32u) {
-        const float l = parts[j * pitch + hd + 1];
-        if (l != 0.0f) sum += l * exp2f(parts[j * pitch + hd] - top);
+    for (int w = 0; w < kScWarps; ++w) top = fmaxf(top, warp_top[w]);
+    float sum = 0.0f;
+    for (unsigned int j = threadIdx.x; j < p.max_splits; j += kScThreads) {
+        const float m = weight[j], w = m == -INFINITY ? 0.0f : exp2f(m - top);
+        weight[j] = w;
+        if (w != 0.0f) sum += parts[j * pitch + hd + 1] * w;
     }
     sum = warp_sum(sum);
-    for (unsigned int j = warp; j < p.max_splits; j += kScWarps) {
-        const float *part = parts + j * pitch;
-        if (part[hd + 1] == 0.0f) continue;
-        const float weight = exp2f(part[hd] - top);
+    if (lane == 0) warp_sum_of[warp] = sum;
+    __syncthreads();
+    sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kScDims; ++i) {
-            const unsigned int d = lane + 32u * i;
-            if (d < hd) acc[i] = fmaf(part[d], weight, acc[i]);
+    for (int w = 0; w < kScWarps; ++w) sum += warp_sum_of[w];
+    for (unsigned int d0 = 0; d0 < hd; d0 += 128u) {
+        const unsigned int d = d0 + 4u * lane;
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (hd % 4u == 0u ? d < hd : false) {
+            for (unsigned int j0 = warp; j0 < p.max_splits; j0 += kScWarps * kScBatch) {
+                float4 o[kScBatch];
+                float w[kScBatch];
+#pragma unroll
+                for (int u = 0; u < kScBatch; ++u) {
+                    const unsigned int j = j0 + u * kScWarps;
+                    w[u] = j < p.max_splits ? weight[j] : 0.0f;
+                    if (w[u] != 0.0f) o[u] = *reinterpret_cast<const float4 *>(parts + j * pitch + d);  // rows of weight 0 hold anything
+                }
+#pragma unroll
+                for (int u = 0; u < kScBatch; ++u)
+                    if (w[u] != 0.0f) {
+                        acc[0] = fmaf(o[u].x, w[u], acc[0]);
+                        acc[1] = fmaf(o[u].y, w[u], acc[1]);
+                        acc[2] = fmaf(o[u].z, w[u], acc[2]);
+                        acc[3] = fmaf(o[u].w, w[u], acc[3]);
+                    }
+            }
+        } else {
+            for (unsigned int j = warp; j < p.max_splits; j += kScWarps)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (d + i < hd && weight[j] != 0.0f) acc[i] = fmaf(parts[j * pitch + d + i], weight[j], acc[i]);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < kScDims; ++i) total[warp][lane + 32 * i] = acc[i];
+        for (int i = 0; i < 4; ++i)
+            if (d + i < hd) total[warp][d + i] = acc[i];
+    }
     __syncthreads();
     for (unsigned int d = threadIdx.x; d < hd; d += kScThreads) {
         float x = 0.0f;
@@ -278,6 +312,7 @@ int scored_combine_launch(const yvx_scored_problem &p, cudaStream_t stream)
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned int)items, 1, 1);
     config.blockDim = dim3(kScThreads, 1, 1);
+    config.dynamicSmemBytes = p.max_splits * sizeof(float);  // the plan keeps them within 8192
     config.stream = stream;
     cudaLaunchAttribute attribute = {};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
