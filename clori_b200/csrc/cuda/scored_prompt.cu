@@ -6,14 +6,15 @@
 // 128-byte swizzle, two stages each), warp 9 issues S = Q K^T (both operands in shared memory) and
 // O += P V (P in tensor memory, where it overwrites its scores), warps 0-3 and 4-7 run the softmax
 // of A and B, a thread per row; warps 10 and 11 only complete the warpgroup that gives its registers
-// to the softmax (224 and 56 a thread of the 168 at launch). A tile walks only the token tiles that some row of it sees.
+// to the softmax (224 and 56 a thread of the 168 at launch). A tile walks only the token tiles that some row of it sees,
+// the last one first: with a bias against distance, and often without, the largest weights come early.
 //
-// The score rule is applied to the 128 scores that a thread holds in registers, two at a time
-// (f32x2 instructions):
-//   cap    tanh(x) = x p(x^2) with p of degree 5 while all 128 scores of all 32 rows of the warp stay
-//          inside |x| <= 1, absolute error below 3e-7 (p was fitted for this kernel); otherwise
-//          1 - 2 / (e^2x + 1) from the exponential unit. With the latter alone the exponential unit would
-//          do three operations per score instead of one, and it is as loaded as the tensor cores.
+// A thread takes its row's 128 products out of tensor memory twice: once for the maximum, then 64 at a time
+// for the weights, which go back over products that have been read; P V of the first half starts while the
+// second is exponentiated. The score rule runs two lanes at a time (f32x2 instructions):
+//   cap    tanh(x) = x p(x^2), p of degree 4, while every |x| of the warp's tile is at most 3/4: absolute error
+//          below 2e-7 (p was fitted for this kernel); otherwise 1 - 2 / (e^2x + 1) from the exponential unit,
+//          which is as loaded as the tensor cores (one exponential per score against two more operations).
 //   bias   slope * (s - position) is linear in the token inside a tile: one multiply-add per score and one
 //          constant per row and tile; tokens behind the row's position (prefixes) take |.| in full.
 // Weights are rounded to bf16, sums and the accumulator are F32.
@@ -27,7 +28,8 @@ constexpr int kSpHalfBytes = kSpM * 64 * 2;        // [128][64] bf16, swizzled
 constexpr int kSpTileBytes = 2 * kSpHalfBytes;     // 32 KB
 constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 1024 + 512;
 constexpr float kSpRescale = 8.0f;                 // log2 units the maximum may lag behind
-constexpr uint32_t kSpTmemColumns = 512;
+constexpr uint32_t kSpTmemColumns = 512;           // S 128 | P_A 64 | P_B 64 | O_A 128 | O_B 128
+constexpr uint32_t kSpPColumn = 128, kSpOColumn = 256;
 
 struct SpMaps {
     CUtensorMap query, key, value;
@@ -36,7 +38,7 @@ struct SpMaps {
 struct SpShared {
     uint64_t q_full;
     uint64_t k_full[kSpStages], k_empty[kSpStages], v_full[kSpStages], v_empty[kSpStages];
-    uint64_t s_full[2], p_half[2][2], pv_done[2];
+    uint64_t s_full[2], s_free, p_half[2][2], pv_done[2];
     uint32_t tmem_base;
     int first[8], end[8];      // visible run of each softmax warp's rows
 };
@@ -70,6 +72,18 @@ __device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsig
     unsigned long long r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+
+__device__ __forceinline__ unsigned long long f2_load(const uint32_t (&s)[32], int c)
+{
+    return f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+}
+__device__ __forceinline__ void f2_store(unsigned long long v, uint32_t (&s)[32], int c)
+{
+    float lo, hi;
+    f2_unpack(v, lo, hi);
+    s[c] = __float_as_uint(lo);
+    s[c + 1] = __float_as_uint(hi);
 }
 
 // A row of a finite call that came out non-finite: weights of zero met a NaN or infinity in rows of V that
@@ -156,6 +170,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
     }
     if (threadIdx.x == 0) {
         mbar_init(&sh->q_full, 1);
+        mbar_init(&sh->s_free, kSpM);
         for (int i = 0; i < kSpStages; ++i) {
             mbar_init(&sh->k_full[i], 1);
             mbar_init(&sh->k_empty[i], 1);
@@ -196,6 +211,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
     const int start = hull_end > 0 ? hull_first / kSpN : 0, stop = (hull_end + kSpN - 1) / kSpN;
     auto active = [&](int x, int j) { return j >= from[x] && j < until[x]; };
     auto fail = [&]() { atomicCAS(p.status, 0, YVX_STATUS_TIMEOUT); };
+    auto waited = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -207,8 +223,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     for (int h = 0; h < 2; ++h)
                         tma_load_4d(q_smem + x * kSpTileBytes + h * kSpHalfBytes, &maps.query, &sh->q_full, 64 * h, (int)qhead,
                                     (int)(q0 + x * kSpM), (int)b);
-                for (int j = start; j < stop; ++j) {
-                    const unsigned int n = (unsigned int)(j - start), stage = n % kSpStages;
+                for (int j = stop - 1; j >= start; --j) {
+                    const unsigned int n = (unsigned int)(stop - 1 - j), stage = n % kSpStages;
                     const uint32_t parity = ((n / kSpStages) - 1u) & 1u;
                     // two runs of 64 tokens (a page may end between them); one behind the hull is not loaded
                     int outer[2], inner[2], runs = 0;
@@ -230,7 +246,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         const CUtensorMap *map = operand ? &maps.value : &maps.key;
                         if (n >= (unsigned int)kSpStages && !mbar_wait(empty, parity)) {
                             fail();
-                            j = stop;
+                            j = start;
                             break;
                         }
                         mbar_expect_tx(full, (uint32_t)runs * (kSpTileBytes / 2));
@@ -243,109 +259,107 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 }
             }
         } else if (warp == 9) {
-            // ------------------------------ matrix products -------------------------------------------
+            // ------------------------------ S = Q K^T, A and B in turn ------------------------------
             // all 32 lanes run converged, one elected lane issues
-            if (stop > start) {
-                constexpr uint32_t idesc_qk = idesc_bf16_f32(kSpM, kSpN, false), idesc_pv = idesc_bf16_f32(kSpM, kSpD, true);
-                const uint32_t q_addr = smem_u32(q_smem), k_addr = smem_u32(k_smem), v_addr = smem_u32(v_smem);
-                auto waited = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
-                auto issue_qk = [&](int x, unsigned int stage) {
-                    const uint32_t ka = k_addr + stage * kSpTileBytes, qa = q_addr + x * kSpTileBytes;
-    #pragma unroll
+            constexpr uint32_t idesc = idesc_bf16_f32(kSpM, kSpN, false);
+            const uint32_t q_addr = smem_u32(q_smem), k_addr = smem_u32(k_smem);
+            bool ok = stop > start && waited(&sh->q_full, 0);
+            unsigned int issued = 0u;
+            for (int j = stop - 1; ok && j >= start; --j) {
+                const unsigned int n = (unsigned int)(stop - 1 - j), stage = n % kSpStages;
+                ok = waited(&sh->k_full[stage], (n / kSpStages) & 1u);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (!ok || !active(x, j)) continue;
+                    if (issued) ok = waited(&sh->s_free, (issued - 1u) & 1u);   // the previous products have been read
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    ++issued;
+#pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
                         const uint32_t off = (ks >> 2) * kSpHalfBytes + (ks & 3) * 32;
-                        tc_mma_ss_elect(tmem + x * kSpN, smem_desc_sw128(qa + off, 16, 1024), smem_desc_sw128(ka + off, 16, 1024),
-                                        idesc_qk, ks ? 1u : 0u);
+                        tc_mma_ss_elect(tmem, smem_desc_sw128(q_addr + x * kSpTileBytes + off, 16, 1024),
+                                        smem_desc_sw128(k_addr + stage * kSpTileBytes + off, 16, 1024), idesc, ks ? 1u : 0u);
                     }
                     tc_commit_elect(&sh->s_full[x]);
-                };
-                auto issue_pv = [&](int x, unsigned int stage, unsigned int count) -> bool {
-                    const uint32_t va = v_addr + stage * kSpTileBytes;
-    #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (!waited(&sh->p_half[x][h], count & 1u)) return false;
-                        tc_fence_after_sync();
-    #pragma unroll
-                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-                            tc_mma_ts_elect(tmem + (2 + x) * kSpN, tmem + x * kSpN + kk * 8,
-                                            smem_desc_sw128(va + kk * 2048, kSpHalfBytes, 1024), idesc_pv, (count || kk) ? 1u : 0u);
-                    }
-                    tc_commit_elect(&sh->pv_done[x]);
-                    return true;
-                };
-                bool ok = waited(&sh->q_full, 0) && waited(&sh->k_full[0], 0);
-                if (ok) {
-                    tc_fence_after_sync();
-    #pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        if (active(x, start)) issue_qk(x, 0u);
-                    tc_commit_elect(&sh->k_empty[0]);
                 }
-                for (int j = start; ok && j < stop; ++j) {
-                    const unsigned int n = (unsigned int)(j - start), stage = n % kSpStages, next = (n + 1u) % kSpStages;
-                    const bool more = j + 1 < stop;
-                    ok = waited(&sh->v_full[stage], (n / kSpStages) & 1u);
-                    if (ok && more) ok = waited(&sh->k_full[next], ((n + 1u) / kSpStages) & 1u);
-                    if (ok) tc_fence_after_sync();
-    #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        if (ok && active(x, j)) ok = issue_pv(x, stage, (unsigned int)(j - from[x]));
-                        if (ok && active(x, j + 1)) issue_qk(x, next);
-                    }
-                    if (!ok) break;
-                    tc_commit_elect(&sh->v_empty[stage]);
-                    if (more) tc_commit_elect(&sh->k_empty[next]);
-                }
-                if (!ok && lane == 0) fail();
+                if (ok) tc_commit_elect(&sh->k_empty[stage]);
             }
+            if (!ok && stop > start && lane == 0) fail();
+        } else if (warp == 10) {
+            // ------------------------------ O += P V ------------------------------------------------
+            constexpr uint32_t idesc = idesc_bf16_f32(kSpM, kSpD, true);
+            const uint32_t v_addr = smem_u32(v_smem);
+            bool ok = true;
+            for (int j = stop - 1; ok && j >= start; --j) {
+                const unsigned int n = (unsigned int)(stop - 1 - j), stage = n % kSpStages;
+                ok = waited(&sh->v_full[stage], (n / kSpStages) & 1u);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (!ok || !active(x, j)) continue;
+                    const unsigned int count = (unsigned int)(until[x] - 1 - j);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        ok = ok && waited(&sh->p_half[x][h], count & 1u);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+#pragma unroll
+                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                            tc_mma_ts_elect(tmem + kSpOColumn + x * kSpD, tmem + kSpPColumn + x * 64 + kk * 8,
+                                            smem_desc_sw128(v_addr + stage * kSpTileBytes + kk * 2048, kSpHalfBytes, 1024), idesc,
+                                            (count || kk) ? 1u : 0u);
+                    }
+                    if (ok) tc_commit_elect(&sh->pv_done[x]);
+                }
+                if (ok) tc_commit_elect(&sh->v_empty[stage]);
+            }
+            if (!ok && lane == 0) fail();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ------------------------------ softmax ----------------------------------------------------
         const int x = (int)(warp >> 2);
         const uint32_t lane_base = tmem + (((warp & 3u) * 32u) << 16);
-        const uint32_t s_col = lane_base + x * kSpN, o_col = lane_base + (2u + x) * kSpN;
+        const uint32_t p_col = lane_base + kSpPColumn + x * 64u, o_col = lane_base + kSpOColumn + x * kSpD;
         const unsigned int tile_row = threadIdx.x & 127u;
         const int my_from = from[x], my_until = until[x];
-        const float mul = (CAP ? p.cap : p.scale) * kScoredLog2e;   // what a held score is multiplied with
+        // Raw products become exponents (log2 units): s * mul, or mul * tanh(s * to_unit) with
+        // tanh(x) = x (a0 + a1 x^2 + .. + a4 x^8) for |x| <= 3/4, all constants folded into the coefficients.
+        const float mul = (CAP ? p.cap : p.scale) * kScoredLog2e;
         const float slope2 = BIAS && exists ? p.slopes[qhead] * kScoredLog2e : 0.0f;
-        const float slope_held = BIAS ? slope2 / mul : 0.0f;
-        unsigned long long poly[6];
-        float inside = 0.0f, to_unit = 0.0f;
+        const float to_unit = CAP ? p.scale / p.cap : 0.0f, inside = CAP ? 0.75f / to_unit : 0.0f;
+        const float to_exp = to_unit * (2.0f * kScoredLog2e);
+        float poly[5];
+        unsigned long long poly2[5];
         if (CAP) {
-            // tanh(x) = x (a0 + a1 x^2 + ...), the powers of scale / cap folded into the coefficients
-            constexpr float a[6] = {0.9999968538734331f,  -0.33324003815111036f, 0.13253525482390585f,
-                                    -0.05097287022853855f, 0.016114189461285185f, -0.0028394691373163504f};
-            to_unit = p.scale / p.cap;
-            inside = p.cap / p.scale;
-            float power = to_unit;
+            constexpr float a[5] = {0.999997228434978f, -0.33323076828402465f, 0.13226094281675813f, -0.049280520544446996f,
+                                    0.012318897799912349f};
+            float power = to_unit * mul;
 #pragma unroll
-            for (int i = 0; i < 6; ++i) {
-                poly[i] = f2_pack(a[i] * power, a[i] * power);
+            for (int i = 0; i < 5; ++i) {
+                poly[i] = a[i] * power;
+                poly2[i] = f2_pack(poly[i], poly[i]);
                 power *= to_unit * to_unit;
             }
         }
-        float m_used = -INFINITY, l = 0.0f;
-        bool ok = true;
-        for (int j = my_from; j < my_until; ++j) {
-            const uint32_t parity = (unsigned int)(j - my_from) & 1u;
-            if (!mbar_wait(&sh->s_full[x], parity)) {
-                ok = false;
-                break;
-            }
+        const float slope_held = BIAS ? slope2 / mul : 0.0f;
+        float m = -INFINITY, l = 0.0f;
+        bool small = true, ok = true;
+        for (int j = my_until - 1; j >= my_from; --j) {
+            const uint32_t parity = (unsigned int)(my_until - 1 - j) & 1u;
+            const int k0 = j * kSpN;
+            if (!waited(&sh->s_full[x], parity)) ok = false;
             tc_fence_after_sync();
             uint32_t s[4][32];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld32(s_col + 32 * i, s[i]);
+            for (int q = 0; q < 4; ++q) tmem_ld32(lane_base + 32 * q, s[q]);
             tmem_wait_ld();
-            const int k0 = j * kSpN;
+            tc_fence_before_sync();
+            mbar_arrive(&sh->s_free);   // the other tile's products may come
             if (k0 < hull_first || k0 + kSpN > hull_end) {
                 // tokens that no row of the CTA sees: their rows of V may hold anything and become zero
-                const unsigned int n = (unsigned int)(j - start), stage = n % kSpStages;
-                if (!mbar_wait(&sh->v_full[stage], (n / kSpStages) & 1u)) {
-                    ok = false;
-                    break;
-                }
+                const unsigned int n = (unsigned int)(stop - 1 - j), stage = n % kSpStages;
+                if (!waited(&sh->v_full[stage], (n / kSpStages) & 1u)) ok = false;
                 const int token = k0 + (int)tile_row;
                 if (token < hull_first || token >= hull_end) {
                     unsigned char *v_row = v_smem + stage * kSpTileBytes + tile_row * 128u;
@@ -357,136 +371,139 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 }
                 fence_proxy_async();
             }
-            float row_top = -INFINITY;
-            if (CAP) {
-                // largest and smallest score; tanh keeps their order
-                float hi[2] = {-INFINITY, -INFINITY}, lo[2] = {INFINITY, INFINITY};
+            const int lo = range.first - k0, hi = range.end - k0;
+            const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kSpN);
+            // the bias of column c: slope * (ahead + c), or -slope * |ahead + c| where a row sees tokens behind itself
+            const int ahead = BIAS ? (int)max(min((long long)k0 - range.position, 0x3fffffffll), -0x3fffffffll) : 0;
+            const bool linear = !BIAS || __all_sync(0xffffffffu, (long long)min(range.end, k0 + kSpN) <= range.position + 1);
+            const float ahead_f = BIAS && linear ? (float)ahead : 0.0f;
+            // The reference m follows the maximum when it lags by more than 2^8. P of the previous tile is overwritten
+            // afterwards, and O may be touched: its P V has to have landed.
+            auto agree = [&](float found) {
+                if (j < my_until - 1 && !waited(&sh->pv_done[x], parity ^ 1u)) ok = false;
+                const bool grow = found > m + kSpRescale || (m == -INFINITY && found > -INFINITY);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float fresh = grow ? found : m, factor = m == -INFINITY ? 1.0f : exp2_approx(m - fresh);
+                    m = fresh;
+                    l *= factor;
+                    if (j < my_until - 1) {
+                        tc_fence_after_sync();
+#pragma unroll 1
+                        for (int i = 0; i < 8; ++i) {
+                            uint32_t o[16];
+                            tmem_ld16(o_col + 16 * i, o);
+                            tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float s0 = __uint_as_float(s[i][c]), s1 = __uint_as_float(s[i][c + 1]);
-                        hi[(c >> 1) & 1] = max3(hi[(c >> 1) & 1], s0, s1);
-                        lo[(c >> 1) & 1] = min3(lo[(c >> 1) & 1], s0, s1);
-                    }
-                row_top = fmaxf(hi[0], hi[1]);
-                row_top = fmaf(-2.0f, __frcp_rn(exp2_approx(row_top * to_unit * (2.0f * kScoredLog2e)) + 1.0f), 1.0f);
-                if (__all_sync(0xffffffffu, fmaxf(fmaxf(hi[0], hi[1]), -fminf(lo[0], lo[1])) <= inside)) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            const unsigned long long v = f2_pack(__uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1]));
-                            const unsigned long long w = f2_mul(v, v);
-                            unsigned long long y = f2_fma(poly[5], w, poly[4]);
-                            y = f2_fma(y, w, poly[3]);
-                            y = f2_fma(y, w, poly[2]);
-                            y = f2_fma(y, w, poly[1]);
-                            y = f2_fma(y, w, poly[0]);
-                            y = f2_mul(y, v);
-                            float lo, hi;
-                            f2_unpack(y, lo, hi);
-                            s[i][c] = __float_as_uint(lo);
-                            s[i][c + 1] = __float_as_uint(hi);
+                            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * factor);
+                            tmem_st16(o_col + 16 * i, o);
                         }
-                } else {
-                    const float unit = to_unit * (2.0f * kScoredLog2e);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const float t = exp2_approx(__uint_as_float(s[i][c]) * unit);
-                            s[i][c] = __float_as_uint(fmaf(-2.0f, __frcp_rn(t + 1.0f), 1.0f));
-                        }
-                }
-            }
-            float ahead_f = 0.0f;
-            if (BIAS) {
-                const int ahead = (int)max(min((long long)k0 - range.position, 0x3fffffffll), -0x3fffffffll);
-                if (__all_sync(0xffffffffu, (long long)min(range.end, k0 + kSpN) <= range.position + 1)) {
-                    ahead_f = (float)ahead;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            s[i][c] = __float_as_uint(fmaf((float)(32 * i + c), slope_held, __uint_as_float(s[i][c])));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            s[i][c] = __float_as_uint(fmaf(-slope_held, fabsf((float)(ahead + 32 * i + c)), __uint_as_float(s[i][c])));
-                }
-            }
-            const bool masked = k0 < range.first || k0 + kSpN > range.end;
-            if (masked) {
-                const int lo = range.first - k0, hi = range.end - k0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (32 * i + c < lo || 32 * i + c >= hi) s[i][c] = 0xff800000u;
-            }
-            if (!CAP || BIAS || __any_sync(0xffffffffu, masked)) {
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2)
-                        mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1]));
-                row_top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
-            }
-            const float m_tile = fmaf(row_top, mul, slope2 * ahead_f);
-            const bool grow = m_tile > m_used + kSpRescale || (m_used == -INFINITY && m_tile > -INFINITY);
-            if (__any_sync(0xffffffffu, grow)) {
-                const float m_new = fmaxf(m_used, m_tile);
-                const float factor = m_new == -INFINITY ? 1.0f : exp2_approx(m_used - m_new);
-                l *= factor;
-                m_used = m_new;
-                if (j > my_from) {
-                    // O may be touched once the previous tile's P V has landed
-                    if (!mbar_wait(&sh->pv_done[x], parity ^ 1u)) {
-                        ok = false;
-                        break;
+                        tmem_wait_st();
                     }
-                    tc_fence_after_sync();
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        uint32_t o[16];
-                        tmem_ld16(o_col + 16 * i, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * factor);
-                        tmem_st16(o_col + 16 * i, o);
-                    }
-                    tmem_wait_st();
                 }
-            }
-            const float offset = m_used == -INFINITY ? 0.0f : fmaf(slope2, ahead_f, -m_used);
-            const unsigned long long mul2 = f2_pack(mul, mul), offset2 = f2_pack(offset, offset);
-            unsigned long long sum2 = 0ull;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t packed[32];
-#pragma unroll
-                for (int i = 2 * h; i < 2 * h + 2; ++i)
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        float e0, e1;
-                        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[i][c]), __uint_as_float(s[i][c + 1])), mul2, offset2), e0, e1);
-                        e0 = exp2_approx(e0);
-                        e1 = exp2_approx(e1);
-                        sum2 = f2_add(sum2, f2_pack(e0, e1));
-                        packed[(i & 1) * 16 + (c >> 1)] = pack_bf16(e0, e1);
-                    }
-                tmem_st32(s_col + 32 * h, packed);
+                return m == -INFINITY ? 0.0f : fmaf(slope2, ahead_f, -m);
+            };
+            auto hand_over = [&](const uint32_t (&packed)[32], int h) {
+                tmem_st32(p_col + 32 * h, packed);
                 tmem_wait_st();
                 tc_fence_before_sync();
-                mbar_arrive(&sh->p_half[x][h]);   // weights of tokens 64 h .. 64 h + 63
+                mbar_arrive(&sh->p_half[x][h]);      // weights of tokens 64 h .. 64 h + 63
+            };
+            // ---- the common tile: nothing masked, bias linear, products inside the polynomial. Straight code, the
+            // other kinds of tile stand apart: a thread's registers stay where tensor memory put them.
+            bool done = false;
+            if (!masked && (!BIAS || (linear && !CAP)) && (!CAP || small)) {
+                float top[2] = {-INFINITY, -INFINITY}, low[2] = {INFINITY, INFINITY};
+#pragma unroll
+                for (int i = 0; i < 128; i += 2) {
+                    uint32_t &u0 = s[i >> 5][i & 31], &u1 = s[i >> 5][(i & 31) + 1];
+                    if (BIAS) {
+                        u0 = __float_as_uint(fmaf((float)i, slope_held, __uint_as_float(u0)));
+                        u1 = __float_as_uint(fmaf((float)(i + 1), slope_held, __uint_as_float(u1)));
+                    }
+                    top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(u0), __uint_as_float(u1));
+                    if (CAP) low[(i >> 1) & 1] = min3(low[(i >> 1) & 1], __uint_as_float(u0), __uint_as_float(u1));
+                }
+                float found = fmaxf(top[0], top[1]);
+                if (CAP) small = __all_sync(0xffffffffu, fmaxf(found, -fminf(low[0], low[1])) <= inside);
+                if (!CAP || small) {
+                    found = CAP ? fmaf(-2.0f * mul, rcp_approx(exp2_approx(found * to_exp) + 1.0f), mul)   // tanh keeps the order
+                                : fmaf(found, mul, slope2 * ahead_f);
+                    const float offset = agree(found);
+                    const unsigned long long offset2 = f2_pack(offset, offset), mul2 = f2_pack(mul, mul);
+                    unsigned long long sum2[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t packed[32];
+#pragma unroll
+                        for (int i = 0; i < 64; i += 2) {
+                            const unsigned long long v = f2_load(s[2 * h + (i >> 5)], i & 31);
+                            float e0, e1;
+                            if (CAP) {
+                                const unsigned long long w = f2_mul(v, v);
+                                unsigned long long y = f2_fma(w, poly2[4], poly2[3]);
+                                y = f2_fma(y, w, poly2[2]);
+                                y = f2_fma(y, w, poly2[1]);
+                                y = f2_fma(y, w, poly2[0]);
+                                f2_unpack(f2_fma(v, y, offset2), e0, e1);
+                            } else {
+                                f2_unpack(f2_fma(v, mul2, offset2), e0, e1);
+                            }
+                            e0 = exp2_approx(e0);
+                            e1 = exp2_approx(e1);
+                            sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(e0, e1));
+                            packed[i >> 1] = pack_bf16(e0, e1);
+                        }
+                        hand_over(packed, h);
+                    }
+                    float sum_lo, sum_hi;
+                    f2_unpack(f2_add(sum2[0], sum2[1]), sum_lo, sum_hi);
+                    l += sum_lo + sum_hi;
+                    done = true;
+                }
             }
-            float sum_lo, sum_hi;
-            f2_unpack(sum2, sum_lo, sum_hi);
-            l += sum_lo + sum_hi;
+            if (!done) {
+                // ---- any other tile: logits in log2 units in place, their maximum, weights --------------------------
+                if (CAP && small) {
+                    float size = 0.0f;   // of what the row sees: the other columns may hold anything
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c >= lo && c < hi) size = fmaxf(size, fabsf(__uint_as_float(s[c >> 5][c & 31])));
+                    small = __all_sync(0xffffffffu, size <= inside);   // once false: for the rest of this warp's tiles
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 128; ++c) {
+                    const float v = __uint_as_float(s[c >> 5][c & 31]);
+                    float z;
+                    if (!CAP) {
+                        z = v * mul;
+                    } else if (small) {
+                        const float w = v * v;
+                        z = v * fmaf(w, fmaf(w, fmaf(w, fmaf(w, poly[4], poly[3]), poly[2]), poly[1]), poly[0]);
+                    } else {
+                        z = fmaf(-2.0f * mul, rcp_approx(exp2_approx(v * to_exp) + 1.0f), mul);
+                    }
+                    if (BIAS) z = fmaf(linear ? slope2 : -slope2, linear ? (float)c : fabsf((float)(ahead + c)), z);
+                    if (c < lo || c >= hi) z = -INFINITY;
+                    top = fmaxf(top, z);
+                    s[c >> 5][c & 31] = __float_as_uint(z);
+                }
+                const float offset = agree(fmaf(slope2, ahead_f, top));
+                float sum = 0.0f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t packed[32];
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const float e0 = exp2_approx(__uint_as_float(s[2 * h + (i >> 5)][i & 31]) + offset);
+                        const float e1 = exp2_approx(__uint_as_float(s[2 * h + (i >> 5)][(i & 31) + 1]) + offset);
+                        sum += e0 + e1;
+                        packed[i >> 1] = pack_bf16(e0, e1);
+                    }
+                    hand_over(packed, h);
+                }
+                l += sum;
+            }
         }
         // ------------------------------ epilogue ----------------------------------------------------
         const bool any = my_until > my_from;
