@@ -6,7 +6,7 @@
 // 128-byte swizzle, two stages each), warp 9 issues S = Q K^T (both operands in shared memory) and
 // O += P V (P in tensor memory, where it overwrites its scores), warps 0-3 and 4-7 run the softmax
 // of A and B, a thread per row; warps 10 and 11 only complete the warpgroup that gives its registers
-// to the softmax (224 and 56 a thread of the 168 at launch). A tile walks only the token tiles that some row of it sees,
+// to the softmax (232 and 40 a thread of the 168 at launch). A tile walks only the token tiles that some row of it sees,
 // the last one first: with a bias against distance, and often without, the largest weights come early.
 //
 // A thread takes its row's 128 products out of tensor memory twice: once for the maximum, then 64 at a time
@@ -84,6 +84,12 @@ __device__ __forceinline__ void f2_store(unsigned long long v, uint32_t (&s)[32]
     f2_unpack(v, lo, hi);
     s[c] = __float_as_uint(lo);
     s[c + 1] = __float_as_uint(hi);
+}
+
+// The polynomial of degree 4 in w.
+__device__ __forceinline__ unsigned long long f2_poly(const unsigned long long (&a)[5], unsigned long long w)
+{
+    return f2_fma(f2_fma(f2_fma(f2_fma(w, a[4], a[3]), w, a[2]), w, a[1]), w, a[0]);
 }
 
 // A row of a finite call that came out non-finite: weights of zero met a NaN or infinity in rows of V that
@@ -214,7 +220,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
     auto waited = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 8) {
             // ------------------------------ tiled copies ----------------------------------------------
             if (lane == 0 && stop > start) {
@@ -316,7 +322,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             if (!ok && lane == 0) fail();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         // ------------------------------ softmax ----------------------------------------------------
         const int x = (int)(warp >> 2);
         const uint32_t lane_base = tmem + (((warp & 3u) * 32u) << 16);
@@ -329,20 +335,18 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         const float slope2 = BIAS && exists ? p.slopes[qhead] * kScoredLog2e : 0.0f;
         const float to_unit = CAP ? p.scale / p.cap : 0.0f, inside = CAP ? 0.75f / to_unit : 0.0f;
         const float to_exp = to_unit * (2.0f * kScoredLog2e);
-        float poly[5];
-        unsigned long long poly2[5];
+        unsigned long long poly2[5];   // each coefficient twice
         if (CAP) {
             constexpr float a[5] = {0.999997228434978f, -0.33323076828402465f, 0.13226094281675813f, -0.049280520544446996f,
                                     0.012318897799912349f};
             float power = to_unit * mul;
 #pragma unroll
             for (int i = 0; i < 5; ++i) {
-                poly[i] = a[i] * power;
-                poly2[i] = f2_pack(poly[i], poly[i]);
+                poly2[i] = f2_pack(a[i] * power, a[i] * power);
                 power *= to_unit * to_unit;
             }
         }
-        const float slope_held = BIAS ? slope2 / mul : 0.0f;
+        const float slope_held = BIAS ? (CAP ? slope2 : slope2 / mul) : 0.0f;
         float m = -INFINITY, l = 0.0f;
         bool small = true, ok = true;
         for (int j = my_until - 1; j >= my_from; --j) {
@@ -408,29 +412,29 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 tc_fence_before_sync();
                 mbar_arrive(&sh->p_half[x][h]);      // weights of tokens 64 h .. 64 h + 63
             };
-            // ---- the common tile: nothing masked, bias linear, products inside the polynomial. Straight code, the
-            // other kinds of tile stand apart: a thread's registers stay where tensor memory put them.
+            unsigned long long sum2[2] = {0ull, 0ull};
+            // ---- a cap's common tile: nothing masked, no bias, products inside the polynomial ------------------------
             bool done = false;
-            if (!masked && (!BIAS || (linear && !CAP)) && (!CAP || small)) {
+            if (CAP) {
+                if (masked) {   // columns that a row does not see may hold anything
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c < lo || c >= hi) s[c >> 5][c & 31] = 0u;
+                }
                 float top[2] = {-INFINITY, -INFINITY}, low[2] = {INFINITY, INFINITY};
 #pragma unroll
                 for (int i = 0; i < 128; i += 2) {
-                    uint32_t &u0 = s[i >> 5][i & 31], &u1 = s[i >> 5][(i & 31) + 1];
-                    if (BIAS) {
-                        u0 = __float_as_uint(fmaf((float)i, slope_held, __uint_as_float(u0)));
-                        u1 = __float_as_uint(fmaf((float)(i + 1), slope_held, __uint_as_float(u1)));
-                    }
-                    top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(u0), __uint_as_float(u1));
-                    if (CAP) low[(i >> 1) & 1] = min3(low[(i >> 1) & 1], __uint_as_float(u0), __uint_as_float(u1));
+                    const float s0 = __uint_as_float(s[i >> 5][i & 31]), s1 = __uint_as_float(s[i >> 5][(i & 31) + 1]);
+                    top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], s0, s1);
+                    low[(i >> 1) & 1] = min3(low[(i >> 1) & 1], s0, s1);
                 }
                 float found = fmaxf(top[0], top[1]);
-                if (CAP) small = __all_sync(0xffffffffu, fmaxf(found, -fminf(low[0], low[1])) <= inside);
-                if (!CAP || small) {
-                    found = CAP ? fmaf(-2.0f * mul, rcp_approx(exp2_approx(found * to_exp) + 1.0f), mul)   // tanh keeps the order
-                                : fmaf(found, mul, slope2 * ahead_f);
+                // once false: for the rest of this warp's tiles
+                small = small && __all_sync(0xffffffffu, fmaxf(found, -fminf(low[0], low[1])) <= inside);
+                if (!BIAS && !masked && small) {
+                    found = fmaf(-2.0f * mul, rcp_approx(exp2_approx(found * to_exp) + 1.0f), mul);   // tanh keeps the order
                     const float offset = agree(found);
-                    const unsigned long long offset2 = f2_pack(offset, offset), mul2 = f2_pack(mul, mul);
-                    unsigned long long sum2[2] = {0ull, 0ull};
+                    const unsigned long long offset2 = f2_pack(offset, offset);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t packed[32];
@@ -438,16 +442,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         for (int i = 0; i < 64; i += 2) {
                             const unsigned long long v = f2_load(s[2 * h + (i >> 5)], i & 31);
                             float e0, e1;
-                            if (CAP) {
-                                const unsigned long long w = f2_mul(v, v);
-                                unsigned long long y = f2_fma(w, poly2[4], poly2[3]);
-                                y = f2_fma(y, w, poly2[2]);
-                                y = f2_fma(y, w, poly2[1]);
-                                y = f2_fma(y, w, poly2[0]);
-                                f2_unpack(f2_fma(v, y, offset2), e0, e1);
-                            } else {
-                                f2_unpack(f2_fma(v, mul2, offset2), e0, e1);
-                            }
+                            f2_unpack(f2_fma(v, f2_poly(poly2, f2_mul(v, v)), offset2), e0, e1);
                             e0 = exp2_approx(e0);
                             e1 = exp2_approx(e1);
                             sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(e0, e1));
@@ -455,55 +450,74 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         }
                         hand_over(packed, h);
                     }
-                    float sum_lo, sum_hi;
-                    f2_unpack(f2_add(sum2[0], sum2[1]), sum_lo, sum_hi);
-                    l += sum_lo + sum_hi;
                     done = true;
                 }
             }
             if (!done) {
-                // ---- any other tile: logits in log2 units in place, their maximum, weights --------------------------
-                if (CAP && small) {
-                    float size = 0.0f;   // of what the row sees: the other columns may hold anything
+                // ---- without a cap: raw products, the bias in their units; with one: logits in log2 units. Then the mask,
+                // the maximum and the weights are the same for all.
+                if (CAP) {
+                    if (small) {
+#pragma unroll
+                        for (int i = 0; i < 128; i += 2) {
+                            const unsigned long long v = f2_load(s[i >> 5], i & 31);
+                            f2_store(f2_mul(v, f2_poly(poly2, f2_mul(v, v))), s[i >> 5], i & 31);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 128; ++c)
+                            s[c >> 5][c & 31] = __float_as_uint(fmaf(
+                                -2.0f * mul, rcp_approx(exp2_approx(__uint_as_float(s[c >> 5][c & 31]) * to_exp) + 1.0f), mul));
+                    }
+                }
+                if (BIAS) {
+                    if (linear) {
+#pragma unroll
+                        for (int c = 0; c < 128; ++c)
+                            s[c >> 5][c & 31] = __float_as_uint(fmaf((float)c, slope_held, __uint_as_float(s[c >> 5][c & 31])));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 128; ++c)
+                            s[c >> 5][c & 31] =
+                                __float_as_uint(fmaf(-slope_held, fabsf((float)(ahead + c)), __uint_as_float(s[c >> 5][c & 31])));
+                    }
+                }
+                if (masked) {
+                    // the smaller of the value and two ramps: at least kHuge / 2 inside the run, at most -kHuge / 2
+                    // outside, whatever stands there (min passes over a NaN)
+                    constexpr float kHuge = 1e30f;
+                    const float up = kHuge * (0.5f - (float)max(lo, -kSpN)), down = kHuge * ((float)min(max(hi, -1), 2 * kSpN) - 0.5f);
 #pragma unroll
                     for (int c = 0; c < 128; ++c)
-                        if (c >= lo && c < hi) size = fmaxf(size, fabsf(__uint_as_float(s[c >> 5][c & 31])));
-                    small = __all_sync(0xffffffffu, size <= inside);   // once false: for the rest of this warp's tiles
+                        s[c >> 5][c & 31] = __float_as_uint(min3(__uint_as_float(s[c >> 5][c & 31]), fmaf((float)c, kHuge, up),
+                                                                 fmaf((float)c, -kHuge, down)));
                 }
-                float top = -INFINITY;
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 128; ++c) {
-                    const float v = __uint_as_float(s[c >> 5][c & 31]);
-                    float z;
-                    if (!CAP) {
-                        z = v * mul;
-                    } else if (small) {
-                        const float w = v * v;
-                        z = v * fmaf(w, fmaf(w, fmaf(w, fmaf(w, poly[4], poly[3]), poly[2]), poly[1]), poly[0]);
-                    } else {
-                        z = fmaf(-2.0f * mul, rcp_approx(exp2_approx(v * to_exp) + 1.0f), mul);
-                    }
-                    if (BIAS) z = fmaf(linear ? slope2 : -slope2, linear ? (float)c : fabsf((float)(ahead + c)), z);
-                    if (c < lo || c >= hi) z = -INFINITY;
-                    top = fmaxf(top, z);
-                    s[c >> 5][c & 31] = __float_as_uint(z);
-                }
-                const float offset = agree(fmaf(slope2, ahead_f, top));
-                float sum = 0.0f;
+                for (int i = 0; i < 128; i += 2)
+                    top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
+                const float held = CAP ? 1.0f : mul, found = fmaxf(top[0], top[1]);
+                float offset = agree(found < -1e29f ? -INFINITY : fmaf(found, held, slope2 * ahead_f));
+                if (found > 1e29f) offset = __int_as_float(0x7fffffff);   // a NaN (or infinity) inside the run: not lost in the mask
+                const unsigned long long offset2 = f2_pack(offset, offset), held2 = f2_pack(held, held);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t packed[32];
 #pragma unroll
                     for (int i = 0; i < 64; i += 2) {
-                        const float e0 = exp2_approx(__uint_as_float(s[2 * h + (i >> 5)][i & 31]) + offset);
-                        const float e1 = exp2_approx(__uint_as_float(s[2 * h + (i >> 5)][(i & 31) + 1]) + offset);
-                        sum += e0 + e1;
+                        float e0, e1;
+                        f2_unpack(f2_fma(f2_load(s[2 * h + (i >> 5)], i & 31), held2, offset2), e0, e1);
+                        e0 = exp2_approx(e0);
+                        e1 = exp2_approx(e1);
+                        sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(e0, e1));
                         packed[i >> 1] = pack_bf16(e0, e1);
                     }
                     hand_over(packed, h);
                 }
-                l += sum;
             }
+            float sum_lo, sum_hi;
+            f2_unpack(f2_add(sum2[0], sum2[1]), sum_lo, sum_hi);
+            l += sum_lo + sum_hi;
         }
         // ------------------------------ epilogue ----------------------------------------------------
         const bool any = my_until > my_from;

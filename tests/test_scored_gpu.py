@@ -162,6 +162,19 @@ def test_a_nan_that_is_seen_is_reported(backend):
             assert c.launch(backend, c.plan(backend, c.problem(backend)))[1] == 1
 
 
+@pytest.mark.parametrize("fields", [dict(), dict(cap=10.0), dict(slopes=True), dict(cap=10.0, slopes=True)])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_a_nan_that_a_prompt_row_sees_is_reported(backend, fields, value):
+    # in a tile that every row sees whole, in one that the causal mask cuts, and for the last row alone
+    for token in (50, 250, 299):
+        for x in ("k", "v"):
+            c = Case(7, [300], 300, 2, 1, 128, garbage=False, **fields)
+            c.arrays[x][0, token] = value
+            if x == "k" and value == np.inf and fields.get("cap"):
+                continue                        # a cap makes an infinite product finite
+            assert c.launch(backend, c.plan(backend, c.problem(backend)))[1] == 1, (token, x)
+
+
 def test_bad_lengths_and_table_entries_are_reported(backend):
     c = Case(8, [100, 90], 1, 4, 2, 128, page=64, cache=E4M3)
     c.table[1, 0] = 9999
