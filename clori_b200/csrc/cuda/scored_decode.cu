@@ -273,39 +273,54 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
         for (int n = 0; n < kCols; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
+        // (consecutive matrix instructions go to different accumulators: each of them has a long latency)
+        if (CODE) {
 #pragma unroll
-        for (int u = 0; u < kPair; ++u) {
-            if (!there[u]) continue;
-            const unsigned char *k_tile = ring + stage[u] * 2 * kOperand;
-            if (CODE) {
+            for (int half = 0; half < 2; ++half) {
+                uint4 kq[kCols];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                for (int n = 0; n < kCols; ++n) {
+                    // a tile behind the split's end stands in for itself with the first one; it is masked below
+                    const unsigned char *k_tile = ring + stage[there[n >> 1] ? n >> 1 : 0] * 2 * kOperand;
+                    const unsigned int row = 16u * warp + 8u * (n & 1) + g;
+                    kq[n] = *reinterpret_cast<const uint4 *>(k_tile + row * 128u + (((2u * c + half) ^ (row & 7u)) << 4));
+                }
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const unsigned int row = 16u * warp + 8u * n + g;
-                        const uint4 kq = *reinterpret_cast<const uint4 *>(k_tile + row * 128u + (((2u * c + half) ^ (row & 7u)) << 4));
-                        const uint32_t words[4] = {kq.x, kq.y, kq.z, kq.w};
+                for (int w = 0; w < 4; ++w)
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            uint32_t b0, b1;
-                            sd_codes<CODE>(words[w], b0, b1);
-                            mma_f16(sc[2 * u + n], qa[4 * half + w], b0, b1);
-                        }
+                    for (int n = 0; n < kCols; ++n) {
+                        const uint32_t words[4] = {kq[n].x, kq[n].y, kq[n].z, kq[n].w};
+                        uint32_t b0, b1;
+                        sd_codes<CODE>(words[w], b0, b1);
+                        mma_f16(sc[n], qa[4 * half + w], b0, b1);
                     }
-                }
-            } else {
-                const uint32_t k_base = smem_u32(k_tile);
-                const unsigned int j = lane >> 3, r = lane & 7u;
-                const unsigned int token = 16u * warp + 8u * (j >> 1) + r;
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const unsigned int chunk = 2u * (ks & 3) + (j & 1u);
-                    uint32_t kb[4];
-                    ldmatrix_x4(kb, k_base + (ks >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
-                    mma_bf16(sc[2 * u], qa[ks], kb[0], kb[1]);
-                    mma_bf16(sc[2 * u + 1], qa[ks], kb[2], kb[3]);
-                }
             }
+        } else {
+            const uint32_t k_base = smem_u32(ring + stage[0] * 2 * kOperand);
+            const unsigned int j = lane >> 3, r = lane & 7u;
+            const unsigned int token = 16u * warp + 8u * (j >> 1) + r;
+            float odd[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd[n][e] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < 8; ks += 2) {
+                uint32_t kb[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const unsigned int chunk = 2u * ((ks + i) & 3) + (j & 1u);
+                    ldmatrix_x4(kb[i], k_base + (ks >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
+                }
+                mma_bf16(sc[0], qa[ks], kb[0][0], kb[0][1]);
+                mma_bf16(sc[1], qa[ks], kb[0][2], kb[0][3]);
+                mma_bf16(odd[0], qa[ks + 1], kb[1][0], kb[1][1]);
+                mma_bf16(odd[1], qa[ks + 1], kb[1][2], kb[1][3]);
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[n][e] += odd[n][e];
         }
         // ---- the score rule, in log2 units --------------------------------------------------------
         if (capped || biased) {
@@ -335,7 +350,8 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
         uint32_t keep_lo[kPair], keep_hi[kPair];
 #pragma unroll
         for (int u = 0; u < kPair; ++u) keep_lo[u] = keep_hi[u] = 0xffffffffu;
-        if (token0 < inner_first || token0 + 64 * (kPair - 1) + 16 > inner_end || !there[kPair - 1]) {
+        const bool cut = token0 < inner_first || token0 + 64 * (kPair - 1) + 16 > inner_end || !there[kPair - 1];
+        if (cut) {
             uint32_t seen = 0u;
 #pragma unroll
             for (int n = 0; n < kCols; ++n)
@@ -433,6 +449,10 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                 for (int np = 0; np < 4; ++np) {
                     uint32_t raw[4];
                     ldmatrix_x4_trans(raw, v_base + token * 128u + (((2u * np + (j >> 1)) ^ (token & 7u)) << 4));
+                    if (cut) {   // both dims' codes of a token are 16 bits of the register
+#pragma unroll
+                        for (int ch = 0; ch < 2; ++ch) raw[2 * ch] &= keep_lo[u], raw[2 * ch + 1] &= keep_hi[u];
+                    }
 #pragma unroll
                     for (int ch = 0; ch < 2; ++ch) {
                         uint32_t lo, hi, lo_even, lo_odd, hi_even, hi_odd;
@@ -440,8 +460,8 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                         asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(hi) : "r"(raw[2 * ch + 1]));
                         sd_codes<CODE>(lo, lo_even, lo_odd);
                         sd_codes<CODE>(hi, hi_even, hi_odd);
-                        mma_f16(o[4 * np + 2 * ch], p_head[u], lo_even & keep_lo[u], hi_even & keep_hi[u]);
-                        mma_f16(o[4 * np + 2 * ch + 1], p_head[u], lo_odd & keep_lo[u], hi_odd & keep_hi[u]);
+                        mma_f16(o[4 * np + 2 * ch], p_head[u], lo_even, hi_even);
+                        mma_f16(o[4 * np + 2 * ch + 1], p_head[u], lo_odd, hi_odd);
                     }
                 }
             } else {
@@ -450,10 +470,14 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                     const unsigned int chunk = 2u * (np & 3) + (j >> 1);
                     uint32_t vb[4];
                     ldmatrix_x4_trans(vb, v_base + (np >> 2) * (kOperand / 2) + token * 128u + ((chunk ^ (token & 7u)) << 4));
-                    mma_bf16(o[2 * np], p_head[u], vb[0] & keep_lo[u], vb[1] & keep_hi[u]);
-                    mma_bf16(o[2 * np], p_tail[u], vb[0] & keep_lo[u], vb[1] & keep_hi[u]);
-                    mma_bf16(o[2 * np + 1], p_head[u], vb[2] & keep_lo[u], vb[3] & keep_hi[u]);
-                    mma_bf16(o[2 * np + 1], p_tail[u], vb[2] & keep_lo[u], vb[3] & keep_hi[u]);
+                    if (cut) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) vb[i] &= i & 1 ? keep_hi[u] : keep_lo[u];
+                    }
+                    mma_bf16(o[2 * np], p_head[u], vb[0], vb[1]);
+                    mma_bf16(o[2 * np + 1], p_head[u], vb[2], vb[3]);
+                    mma_bf16(o[2 * np], p_tail[u], vb[0], vb[1]);
+                    mma_bf16(o[2 * np + 1], p_tail[u], vb[2], vb[3]);
                 }
             }
         }
