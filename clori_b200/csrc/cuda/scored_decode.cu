@@ -142,18 +142,7 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
             const unsigned int mine = slot * per_tile + min(lane, per_tile - 1u);
             const int unit_page = __shfl_sync(0xffffffffu, page, mine), unit_inner = __shfl_sync(0xffffffffu, inner, mine);
             const unsigned int loaded = __ballot_sync(0xffffffffu, lane < per_tile && unit_page >= 0);
-            if (CODE) {
-                // the scales of the 16 tokens of consumer warp `lane`; a unit behind the split's end: 0
-                const unsigned int of_warp = slot * per_tile + (16u * min(lane, 3u)) / (unsigned int)unit;
-                const float ks = __shfl_sync(0xffffffffu, key_scale, of_warp), vs = __shfl_sync(0xffffffffu, value_scale, of_warp);
-                const int there = __shfl_sync(0xffffffffu, page, of_warp);
-                if (lane < (unsigned int)kSdWarps)
-                    scale_smem[stage * kSdWarps + lane] = there >= 0 ? make_float2(ks, vs) : make_float2(0.0f, 0.0f);
-                __syncwarp();
-            }
             unsigned char *k_dst = ring + stage * 2 * kOperand, *v_dst = k_dst + kOperand;
-            if (lane == 0) mbar_expect_tx(&full[stage], (uint32_t)__popc(loaded) * (uint32_t)unit * kSdDim * 2u * (CODE ? 1u : 2u));
-            __syncwarp();
             if (lane < per_tile && unit_page >= 0) {
                 const int c1 = head_inner ? (int)kv_head : unit_inner, c2 = head_inner ? unit_inner : (int)kv_head;
                 const uint32_t at = lane * (uint32_t)unit * 128u;
@@ -162,6 +151,17 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                 tma_load_4d(v_dst + at, &maps.value, &full[stage], 0, c1, c2, unit_page);
                 if (!CODE) tma_load_4d(v_dst + kOperand / 2 + at, &maps.value, &full[stage], 64, c1, c2, unit_page);
             }
+            if (CODE) {
+                // meanwhile the scales of the 16 tokens of consumer warp `lane`; a unit that is not loaded: 0
+                const unsigned int of_warp = slot * per_tile + (16u * min(lane, 3u)) / (unsigned int)unit;
+                const float ks = __shfl_sync(0xffffffffu, key_scale, of_warp), vs = __shfl_sync(0xffffffffu, value_scale, of_warp);
+                const int there = __shfl_sync(0xffffffffu, page, of_warp);
+                if (lane < (unsigned int)kSdWarps)
+                    scale_smem[stage * kSdWarps + lane] = there >= 0 ? make_float2(ks, vs) : make_float2(0.0f, 0.0f);
+            }
+            // the phase ends with this arrival, the bytes may have landed before
+            __syncwarp();
+            if (lane == 0) mbar_expect_tx(&full[stage], (uint32_t)__popc(loaded) * (uint32_t)unit * kSdDim * 2u * (CODE ? 1u : 2u));
         }
         return;
     }

@@ -69,36 +69,32 @@ static bool scored_needs_stage(const yvx_scored_problem *p)
 
 extern "C" {
 
-// Splits fill the machine: two CTAs of the split kernels run on an SM, so a wave is 2 * sm_count
-// items. The chunk is the largest multiple of 64 tokens, at most 4096, whose items fill their
-// last wave to 90 %; else the best-filled one with at least a wave; else 64.
+// Splits fill the machine: two CTAs of the split kernels run on an SM, so a wave is 2 * sm_count items. Every
+// wave costs its chunk's tiles of 64 tokens and about four tiles more (start, first data, merge of the warps,
+// partial rows); the chunk with the smallest sum is taken, at most 8192 tokens. One session of 4096 tokens:
+// 128 tokens 10.3 us, 64 tokens 15.4, 512 tokens 13.0; 64 sessions behind a window of 4096: one chunk 177 us,
+// two 193, four 190; one session of 131072 tokens: 3584 (one wave) 95 us, 1792 107, 4096 105.
 void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
 {
     if (!p || !p->kv_heads || !p->query_rows || !p->kv_tokens_max) return;
     const unsigned long long wave = 2ull * (unsigned long long)(sm_count > 0 ? sm_count : 148);
     const unsigned long long vectors = (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads);
     const unsigned long long span = yvx::scored_span(p);
-    if (yvx::scored_prompt_shape(p)) {
-        p->chunk_tokens = (unsigned int)span;
-        p->max_splits = 1u;
-        return;
-    }
     const unsigned long long lanes = (unsigned long long)p->sessions * p->kv_heads * ((vectors + 15ull) / 16ull);
-    unsigned int best = 64u;
-    double best_fill = -1.0;
-    for (unsigned int chunk = 4096u; chunk >= 64u; chunk -= 64u) {
-        const unsigned long long items = lanes * ((span + chunk - 1ull) / chunk);
-        if (items < wave) continue;
-        const double fill = (double)items / (double)((items + wave - 1ull) / wave * wave);
-        if (fill > best_fill) {
-            best_fill = fill;
-            best = chunk;
+    unsigned long long best = span, best_cost = ~0ull;
+    if (!yvx::scored_prompt_shape(p) && (vectors <= 64ull || lanes < wave)) {
+        for (unsigned long long chunk = 64ull; chunk <= 8192ull; chunk += 64ull) {
+            const unsigned long long splits = (span + chunk - 1ull) / chunk;
+            const unsigned long long cost = (lanes * splits + wave - 1ull) / wave * (4ull + chunk / 64ull);
+            if (splits <= 8192ull && cost < best_cost) {
+                best_cost = cost;
+                best = chunk;
+            }
+            if (splits == 1ull) break;
         }
-        if (fill >= 0.9) break;
+        while ((span + best - 1ull) / best > 8192ull) best += 64ull;
     }
-    while ((span + best - 1ull) / best > 8192ull) best += 64u;
-    if (lanes >= wave && vectors > 64ull) best = (unsigned int)span;  // many rows fill the machine by themselves
-    p->chunk_tokens = best;
+    p->chunk_tokens = (unsigned int)best;
     p->max_splits = (unsigned int)((span + best - 1ull) / best);
 }
 
