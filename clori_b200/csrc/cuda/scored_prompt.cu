@@ -6,7 +6,7 @@
 // 128-byte swizzle, two stages each), warp 9 issues S = Q K^T (both operands in shared memory) and
 // O += P V (P in tensor memory, where it overwrites its scores), warps 0-3 and 4-7 run the softmax
 // of A and B, a thread per row; warps 10 and 11 only complete the warpgroup that gives its registers
-// to the softmax (232 and 40 a thread of the 168 at launch). A tile walks only the token tiles that some row of it sees,
+// to the softmax (224 and 56 a thread of the 168 at launch). A tile walks only the token tiles that some row of it sees,
 // the last one first: with a bias against distance, and often without, the largest weights come early.
 //
 // A thread takes its row's 128 products out of tensor memory twice: once for the maximum, then 64 at a time
@@ -26,23 +26,58 @@ namespace yvx {
 constexpr int kSpM = 128, kSpN = 128, kSpD = 128, kSpStages = 2, kSpThreads = 384;
 constexpr int kSpHalfBytes = kSpM * 64 * 2;        // [128][64] bf16, swizzled
 constexpr int kSpTileBytes = 2 * kSpHalfBytes;     // 32 KB
-constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 1024 + 512;
+constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 1024 + 5 * 1024;
 constexpr float kSpRescale = 8.0f;                 // log2 units the maximum may lag behind
 constexpr uint32_t kSpTmemColumns = 512;           // S 128 | P_A 64 | P_B 64 | O_A 128 | O_B 128
+constexpr int kSpReaders = 11;                     // warps that read a piece of work
 constexpr uint32_t kSpPColumn = 128, kSpOColumn = 256;
 
 struct SpMaps {
     CUtensorMap query, key, value;
 };
 
+// One piece of work: two row tiles of one head and what they see. Warp 11 fills it.
+struct SpWork {
+    int first[2 * kSpM], end[2 * kSpM];   // visible run of each row; rows that do not exist see nothing
+    int hull_first, hull_end;             // of all of them
+    int from[2], until[2];                // token tiles [from[x], until[x]) of the two row tiles
+    unsigned int q0, qhead, b;
+    int valid;                            // 0: nothing is left
+    long long query_start;
+};
+
 struct SpShared {
-    uint64_t q_full;
+    uint4 next_block;                     // the answer to a request for another block's work
+    uint64_t next_full, work_full[2], work_empty[2], ask;
+    uint64_t q_full, q_empty;
     uint64_t k_full[kSpStages], k_empty[kSpStages], v_full[kSpStages], v_empty[kSpStages];
     uint64_t s_full[2], s_free, p_half[2][2], pv_done[2];
     uint32_t tmem_base;
-    int first[8], end[8];      // visible run of each softmax warp's rows
+    SpWork work[2];
 };
-static_assert(sizeof(SpShared) <= 512, "the barrier block outgrew its slot");
+static_assert(sizeof(SpShared) <= 5 * 1024, "the barrier block outgrew its slot");
+
+// Asks the hardware for a block of the grid that has not started: its index, or "none is left", arrives in *slot.
+__device__ __forceinline__ void sp_ask_block(uint4 *slot, uint64_t *bar)
+{
+    mbar_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 :: "r"(smem_u32(slot)), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool sp_block_given(const uint4 *slot, unsigned int &block)
+{
+    uint32_t given;
+    asm volatile(
+        "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+        "ld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, r;\n\t}"
+        : "=r"(given), "=r"(block) : "r"(smem_u32(slot)) : "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the slot may be written again
+    return given != 0u;
+}
 
 // ---- two floats at a time -----------------------------------------------------------------------------
 __device__ __forceinline__ unsigned long long f2_pack(float lo, float hi)
@@ -153,30 +188,16 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
     SpShared *sh = reinterpret_cast<SpShared *>(v_smem + kSpStages * kSpTileBytes);
 
     const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const unsigned int pairs = (p.query_rows + 2 * kSpM - 1) / (2 * kSpM);
-    const unsigned long long per_group = (unsigned long long)pairs * lane_group;
-    const unsigned int within = (unsigned int)(blockIdx.x % per_group);
-    const unsigned int work_lane = (unsigned int)(blockIdx.x / per_group) * lane_group + within % lane_group;
-    if (work_lane >= p.query_heads * p.sessions) return;  // the last group may be short; uniform over the CTA
-    const unsigned int q0 = (pairs - 1u - within / lane_group) * 2u * kSpM;
-    const unsigned int qhead = work_lane % p.query_heads, b = work_lane / p.query_heads;
-    const unsigned int kv_head = qhead / (p.query_heads / p.kv_heads);
-    const unsigned int kv_tokens = admitted_kv_tokens(p.kv_tokens, b, p.kv_tokens_uniform, p.kv_tokens_max, p.status);
-    const long long query_start = scored_query_start(p, b, kv_tokens);
-
-    ScoredRange range = {0, 0, 0};
-    const unsigned int my_row = q0 + threadIdx.x;      // softmax threads: A's rows, then B's
-    const bool exists = threadIdx.x < 2 * kSpM && my_row < p.query_rows;
-    if (exists) range = scored_range(p, b, my_row, kv_tokens, query_start);
-    if (warp < 8) {
-        const bool sees = range.first < range.end;
-        const int lo = __reduce_min_sync(0xffffffffu, sees ? range.first : 0x7fffffff);
-        const int hi = __reduce_max_sync(0xffffffffu, sees ? range.end : 0);
-        if (lane == 0) sh->first[warp] = lo, sh->end[warp] = hi;
-    }
     if (threadIdx.x == 0) {
+        mbar_init(&sh->next_full, 1);
+        mbar_init(&sh->ask, 1);
         mbar_init(&sh->q_full, 1);
+        mbar_init(&sh->q_empty, 1);
         mbar_init(&sh->s_free, kSpM);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->work_full[i], 1);
+            mbar_init(&sh->work_empty[i], kSpReaders);
+        }
         for (int i = 0; i < kSpStages; ++i) {
             mbar_init(&sh->k_full[i], 1);
             mbar_init(&sh->k_empty[i], 1);
@@ -199,140 +220,241 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = sh->tmem_base;
-    // token tiles [from[x], until[x]) of the two row tiles; the CTA walks their hull
-    int hull_first = 0x7fffffff, hull_end = 0, from[2], until[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        int lo = 0x7fffffff, hi = 0;
-#pragma unroll
-        for (int w = 4 * x; w < 4 * x + 4; ++w) {
-            lo = min(lo, sh->first[w]);
-            hi = max(hi, sh->end[w]);
-        }
-        from[x] = hi > 0 ? lo / kSpN : 0;
-        until[x] = (hi + kSpN - 1) / kSpN;
-        hull_first = min(hull_first, lo);
-        hull_end = max(hull_end, hi);
-    }
-    const int start = hull_end > 0 ? hull_first / kSpN : 0, stop = (hull_end + kSpN - 1) / kSpN;
-    auto active = [&](int x, int j) { return j >= from[x] && j < until[x]; };
     auto fail = [&]() { atomicCAS(p.status, 0, YVX_STATUS_TIMEOUT); };
     auto waited = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
+    // The turn-th piece of work, or null when none is left (or a wait gave up).
+    auto take = [&](unsigned int turn) -> const SpWork * {
+        const SpWork *w = &sh->work[turn & 1u];
+        if (!waited(&sh->work_full[turn & 1u], (turn >> 1) & 1u)) {
+            if (lane == 0) fail();
+            return nullptr;
+        }
+        return w->valid ? w : nullptr;
+    };
+    auto give_back = [&](unsigned int turn) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->work_empty[turn & 1u]);
+    };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 8) {
             // ------------------------------ tiled copies ----------------------------------------------
-            if (lane == 0 && stop > start) {
-                mbar_expect_tx(&sh->q_full, 2u * kSpTileBytes);
-                for (int x = 0; x < 2; ++x)
-                    for (int h = 0; h < 2; ++h)
-                        tma_load_4d(q_smem + x * kSpTileBytes + h * kSpHalfBytes, &maps.query, &sh->q_full, 64 * h, (int)qhead,
-                                    (int)(q0 + x * kSpM), (int)b);
-                for (int j = stop - 1; j >= start; --j) {
-                    const unsigned int n = (unsigned int)(stop - 1 - j), stage = n % kSpStages;
-                    const uint32_t parity = ((n / kSpStages) - 1u) & 1u;
-                    // two runs of 64 tokens (a page may end between them); one behind the hull is not loaded
-                    int outer[2], inner[2], runs = 0;
-                    for (int r = 0; r < 2; ++r) {
-                        const int token = j * kSpN + 64 * r;
-                        if (token >= hull_end) break;
-                        outer[r] = (int)b, inner[r] = token;
-                        if (p.block_table) {
-                            const int page = token + 64 > hull_first ? scored_page(p, b, (unsigned int)token / p.block_tokens) : 0;
-                            outer[r] = page < 0 ? 0 : page;
-                            inner[r] = (int)((unsigned int)token % p.block_tokens);
-                        }
-                        ++runs;
-                    }
-                    for (int operand = 0; operand < 2; ++operand) {
-                        uint64_t *full = operand ? &sh->v_full[stage] : &sh->k_full[stage];
-                        uint64_t *empty = operand ? &sh->v_empty[stage] : &sh->k_empty[stage];
-                        unsigned char *dst = (operand ? v_smem : k_smem) + stage * kSpTileBytes;
-                        const CUtensorMap *map = operand ? &maps.value : &maps.key;
-                        if (n >= (unsigned int)kSpStages && !mbar_wait(empty, parity)) {
-                            fail();
-                            j = start;
-                            break;
-                        }
-                        mbar_expect_tx(full, (uint32_t)runs * (kSpTileBytes / 2));
-                        for (int r = 0; r < runs; ++r) {
-                            const int c1 = head_inner ? (int)kv_head : inner[r], c2 = head_inner ? inner[r] : (int)kv_head;
-                            tma_load_4d(dst + r * 64 * 128, map, full, 0, c1, c2, outer[r]);
-                            tma_load_4d(dst + kSpHalfBytes + r * 64 * 128, map, full, 64, c1, c2, outer[r]);
+            unsigned int tiles = 0u, pieces = 0u;   // so far: token tiles, pieces of work with any
+            bool ok = true;
+            for (unsigned int turn = 0; ok; ++turn) {
+                const SpWork *const w = take(turn);
+                if (w == nullptr) break;
+                const int hull_first = w->hull_first, hull_end = w->hull_end, start = hull_first / kSpN;
+                const int stop = (hull_end + kSpN - 1) / kSpN;
+                const unsigned int b = w->b, kv_head = w->qhead / (p.query_heads / p.kv_heads);
+                if (lane == 0) {
+                    if (stop > start) {
+                        if (pieces) ok = mbar_wait(&sh->q_empty, (pieces - 1u) & 1u);
+                        if (ok) {
+                            mbar_expect_tx(&sh->q_full, 2u * kSpTileBytes);
+                            for (int x = 0; x < 2; ++x)
+                                for (int h = 0; h < 2; ++h)
+                                    tma_load_4d(q_smem + x * kSpTileBytes + h * kSpHalfBytes, &maps.query, &sh->q_full, 64 * h,
+                                                (int)w->qhead, (int)(w->q0 + x * kSpM), (int)b);
                         }
                     }
+                    for (int j = stop - 1; ok && j >= start; --j) {
+                        const unsigned int n = tiles + (unsigned int)(stop - 1 - j), stage = n % kSpStages;
+                        const uint32_t parity = ((n / kSpStages) - 1u) & 1u;
+                        // two runs of 64 tokens (a page may end between them); one behind the hull is not loaded
+                        int outer[2], inner[2], runs = 0;
+                        for (int r = 0; r < 2; ++r) {
+                            const int token = j * kSpN + 64 * r;
+                            if (token >= hull_end) break;
+                            outer[r] = (int)b, inner[r] = token;
+                            if (p.block_table) {
+                                const int page = token + 64 > hull_first ? scored_page(p, b, (unsigned int)token / p.block_tokens) : 0;
+                                outer[r] = page < 0 ? 0 : page;
+                                inner[r] = (int)((unsigned int)token % p.block_tokens);
+                            }
+                            ++runs;
+                        }
+                        for (int operand = 0; ok && operand < 2; ++operand) {
+                            uint64_t *full = operand ? &sh->v_full[stage] : &sh->k_full[stage];
+                            uint64_t *empty = operand ? &sh->v_empty[stage] : &sh->k_empty[stage];
+                            unsigned char *dst = (operand ? v_smem : k_smem) + stage * kSpTileBytes;
+                            const CUtensorMap *map = operand ? &maps.value : &maps.key;
+                            if (n >= (unsigned int)kSpStages) ok = mbar_wait(empty, parity);
+                            if (!ok) break;
+                            mbar_expect_tx(full, (uint32_t)runs * (kSpTileBytes / 2));
+                            for (int r = 0; r < runs; ++r) {
+                                const int c1 = head_inner ? (int)kv_head : inner[r], c2 = head_inner ? inner[r] : (int)kv_head;
+                                tma_load_4d(dst + r * 64 * 128, map, full, 0, c1, c2, outer[r]);
+                                tma_load_4d(dst + kSpHalfBytes + r * 64 * 128, map, full, 64, c1, c2, outer[r]);
+                            }
+                        }
+                    }
+                    if (!ok) fail();
+                    mbar_arrive(&sh->ask);   // all loads are under way: time to look for the next piece
                 }
+                ok = __all_sync(0xffffffffu, ok);
+                tiles += (unsigned int)(stop - start);
+                pieces += stop > start ? 1u : 0u;
+                give_back(turn);
             }
         } else if (warp == 9) {
             // ------------------------------ S = Q K^T, A and B in turn ------------------------------
             // all 32 lanes run converged, one elected lane issues
             constexpr uint32_t idesc = idesc_bf16_f32(kSpM, kSpN, false);
             const uint32_t q_addr = smem_u32(q_smem), k_addr = smem_u32(k_smem);
-            bool ok = stop > start && waited(&sh->q_full, 0);
-            unsigned int issued = 0u;
-            for (int j = stop - 1; ok && j >= start; --j) {
-                const unsigned int n = (unsigned int)(stop - 1 - j), stage = n % kSpStages;
-                ok = waited(&sh->k_full[stage], (n / kSpStages) & 1u);
+            unsigned int issued = 0u, tiles = 0u, pieces = 0u;
+            bool ok = true;
+            for (unsigned int turn = 0; ok; ++turn) {
+                const SpWork *const w = take(turn);
+                if (w == nullptr) break;
+                const int start = w->hull_first / kSpN, stop = (w->hull_end + kSpN - 1) / kSpN;
+                const int from[2] = {w->from[0], w->from[1]}, until[2] = {w->until[0], w->until[1]};
+                give_back(turn);
+                if (stop <= start) continue;
+                ok = waited(&sh->q_full, pieces & 1u);
+                for (int j = stop - 1; ok && j >= start; --j) {
+                    const unsigned int n = tiles + (unsigned int)(stop - 1 - j), stage = n % kSpStages;
+                    ok = waited(&sh->k_full[stage], (n / kSpStages) & 1u);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (!ok || !active(x, j)) continue;
-                    if (issued) ok = waited(&sh->s_free, (issued - 1u) & 1u);   // the previous products have been read
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    ++issued;
+                    for (int x = 0; x < 2; ++x) {
+                        if (!ok || j < from[x] || j >= until[x]) continue;
+                        if (issued) ok = waited(&sh->s_free, (issued - 1u) & 1u);   // the previous products have been read
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        ++issued;
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const uint32_t off = (ks >> 2) * kSpHalfBytes + (ks & 3) * 32;
-                        tc_mma_ss_elect(tmem, smem_desc_sw128(q_addr + x * kSpTileBytes + off, 16, 1024),
-                                        smem_desc_sw128(k_addr + stage * kSpTileBytes + off, 16, 1024), idesc, ks ? 1u : 0u);
+                        for (int ks = 0; ks < 8; ++ks) {
+                            const uint32_t off = (ks >> 2) * kSpHalfBytes + (ks & 3) * 32;
+                            tc_mma_ss_elect(tmem, smem_desc_sw128(q_addr + x * kSpTileBytes + off, 16, 1024),
+                                            smem_desc_sw128(k_addr + stage * kSpTileBytes + off, 16, 1024), idesc, ks ? 1u : 0u);
+                        }
+                        tc_commit_elect(&sh->s_full[x]);
                     }
-                    tc_commit_elect(&sh->s_full[x]);
+                    if (ok) tc_commit_elect(&sh->k_empty[stage]);
                 }
-                if (ok) tc_commit_elect(&sh->k_empty[stage]);
+                if (ok) tc_commit_elect(&sh->q_empty);
+                if (!ok && lane == 0) fail();
+                tiles += (unsigned int)(stop - start);
+                ++pieces;
             }
-            if (!ok && stop > start && lane == 0) fail();
         } else if (warp == 10) {
             // ------------------------------ O += P V ------------------------------------------------
             constexpr uint32_t idesc = idesc_bf16_f32(kSpM, kSpD, true);
             const uint32_t v_addr = smem_u32(v_smem);
+            unsigned int tiles = 0u, counts[2] = {0u, 0u};
             bool ok = true;
-            for (int j = stop - 1; ok && j >= start; --j) {
-                const unsigned int n = (unsigned int)(stop - 1 - j), stage = n % kSpStages;
-                ok = waited(&sh->v_full[stage], (n / kSpStages) & 1u);
+            for (unsigned int turn = 0; ok; ++turn) {
+                const SpWork *const w = take(turn);
+                if (w == nullptr) break;
+                const int start = w->hull_first / kSpN, stop = (w->hull_end + kSpN - 1) / kSpN;
+                const int from[2] = {w->from[0], w->from[1]}, until[2] = {w->until[0], w->until[1]};
+                give_back(turn);
+                for (int j = stop - 1; ok && j >= start; --j) {
+                    const unsigned int n = tiles + (unsigned int)(stop - 1 - j), stage = n % kSpStages;
+                    ok = waited(&sh->v_full[stage], (n / kSpStages) & 1u);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (!ok || !active(x, j)) continue;
-                    const unsigned int count = (unsigned int)(until[x] - 1 - j);
+                    for (int x = 0; x < 2; ++x) {
+                        if (!ok || j < from[x] || j >= until[x]) continue;
+                        const uint32_t later = j < until[x] - 1 ? 1u : 0u;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        ok = ok && waited(&sh->p_half[x][h], count & 1u);
-                        if (!ok) break;
-                        tc_fence_after_sync();
+                        for (int h = 0; h < 2; ++h) {
+                            ok = ok && waited(&sh->p_half[x][h], counts[x] & 1u);
+                            if (!ok) break;
+                            tc_fence_after_sync();
 #pragma unroll
-                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-                            tc_mma_ts_elect(tmem + kSpOColumn + x * kSpD, tmem + kSpPColumn + x * 64 + kk * 8,
-                                            smem_desc_sw128(v_addr + stage * kSpTileBytes + kk * 2048, kSpHalfBytes, 1024), idesc,
-                                            (count || kk) ? 1u : 0u);
+                            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                                tc_mma_ts_elect(tmem + kSpOColumn + x * kSpD, tmem + kSpPColumn + x * 64 + kk * 8,
+                                                smem_desc_sw128(v_addr + stage * kSpTileBytes + kk * 2048, kSpHalfBytes, 1024), idesc,
+                                                kk ? 1u : later);
+                        }
+                        if (ok) tc_commit_elect(&sh->pv_done[x]);
+                        ++counts[x];
                     }
-                    if (ok) tc_commit_elect(&sh->pv_done[x]);
+                    if (ok) tc_commit_elect(&sh->v_empty[stage]);
                 }
-                if (ok) tc_commit_elect(&sh->v_empty[stage]);
+                if (!ok && lane == 0) fail();
+                tiles += (unsigned int)(stop - start);
             }
-            if (!ok && lane == 0) fail();
+        } else {
+            // ------------------------------ pieces of work ------------------------------------------
+            // The block's own first, then those of blocks that have not started, as long as there are any.
+            const unsigned int pairs = (p.query_rows + 2 * kSpM - 1) / (2 * kSpM);
+            const unsigned long long per_group = (unsigned long long)pairs * lane_group;
+            unsigned int block = blockIdx.x, asked = 0u;
+            bool ok = true, more = true;
+            for (unsigned int turn = 0; ok && more; ++turn) {
+                SpWork *const w = &sh->work[turn & 1u];
+                if (turn >= 2u) ok = waited(&sh->work_empty[turn & 1u], ((turn >> 1) - 1u) & 1u);
+                unsigned int work_lane = 0u, within = 0u;
+                auto given = [&]() {
+                    within = (unsigned int)(block % per_group);
+                    work_lane = (unsigned int)(block / per_group) * lane_group + within % lane_group;
+                    return work_lane < p.query_heads * p.sessions;   // the last group may be short
+                };
+                bool look = turn > 0u || !given();
+                while (ok && look) {
+                    if (lane == 0) sp_ask_block(&sh->next_block, &sh->next_full);
+                    ok = waited(&sh->next_full, asked & 1u);
+                    ++asked;
+                    more = ok && sp_block_given(&sh->next_block, block);
+                    __syncwarp();
+                    look = more && !given();
+                }
+                if (!ok) {
+                    if (lane == 0) fail();
+                    break;   // who waits for the piece gives up as well
+                }
+                int tiles = 0;
+                if (more) {
+                    const unsigned int q0 = (pairs - 1u - within / lane_group) * 2u * kSpM;
+                    const unsigned int qhead = work_lane % p.query_heads, b = work_lane / p.query_heads;
+                    const unsigned int kv_tokens = admitted_kv_tokens(p.kv_tokens, b, p.kv_tokens_uniform, p.kv_tokens_max, p.status);
+                    const long long query_start = scored_query_start(p, b, kv_tokens);
+                    int hull_first = 0x7fffffff, hull_end = 0;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        int lo = 0x7fffffff, hi = 0;
+#pragma unroll
+                        for (int i = 0; i < kSpM / 32; ++i) {
+                            const unsigned int at = x * kSpM + 32u * i + lane;
+                            ScoredRange range = {0, 0, 0};
+                            if (q0 + at < p.query_rows) range = scored_range(p, b, q0 + at, kv_tokens, query_start);
+                            w->first[at] = range.first, w->end[at] = range.end;
+                            if (range.first < range.end) lo = min(lo, range.first), hi = max(hi, range.end);
+                        }
+                        lo = __reduce_min_sync(0xffffffffu, lo);
+                        hi = __reduce_max_sync(0xffffffffu, hi);
+                        if (lane == 0) w->from[x] = hi > 0 ? lo / kSpN : 0, w->until[x] = (hi + kSpN - 1) / kSpN;
+                        hull_first = min(hull_first, lo);
+                        hull_end = max(hull_end, hi);
+                    }
+                    if (hull_end == 0) hull_first = 0;
+                    if (lane == 0)
+                        w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->qhead = qhead, w->b = b,
+                        w->query_start = query_start;
+                    tiles = (hull_end + kSpN - 1) / kSpN - hull_first / kSpN;
+                }
+                if (lane == 0) w->valid = more;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->work_full[turn & 1u]);
+                // the next one when this one's loads are all under way: a piece taken earlier might start later here
+                // than elsewhere. A wait's limit is meant for one tile.
+                ok = !more;
+                for (int i = 0; !ok && i <= tiles; ++i) ok = waited(&sh->ask, turn & 1u);
+                if (!ok && lane == 0) fail();
+            }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // ------------------------------ softmax ----------------------------------------------------
         const int x = (int)(warp >> 2);
         const uint32_t lane_base = tmem + (((warp & 3u) * 32u) << 16);
         const uint32_t p_col = lane_base + kSpPColumn + x * 64u, o_col = lane_base + kSpOColumn + x * kSpD;
         const unsigned int tile_row = threadIdx.x & 127u;
-        const int my_from = from[x], my_until = until[x];
         // Raw products become exponents (log2 units): s * mul, or mul * tanh(s * to_unit) with
         // tanh(x) = x (a0 + a1 x^2 + .. + a4 x^8) for |x| <= 3/4, all constants folded into the coefficients.
         const float mul = (CAP ? p.cap : p.scale) * kScoredLog2e;
-        const float slope2 = BIAS && exists ? p.slopes[qhead] * kScoredLog2e : 0.0f;
         const float to_unit = CAP ? p.scale / p.cap : 0.0f, inside = CAP ? 0.75f / to_unit : 0.0f;
         const float to_exp = to_unit * (2.0f * kScoredLog2e);
         unsigned long long poly2[5];   // each coefficient twice
@@ -346,11 +468,24 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 power *= to_unit * to_unit;
             }
         }
+        unsigned int tiles = 0u, count = 0u;   // so far: token tiles of the block, of this row tile
+        bool ok = true;
+        for (unsigned int turn = 0; ok; ++turn) {
+        const SpWork *const w = take(turn);
+        if (w == nullptr) break;
+        const unsigned int my_row = w->q0 + threadIdx.x, qhead = w->qhead, b = w->b;
+        const bool exists = my_row < p.query_rows;
+        const ScoredRange range = {w->first[threadIdx.x], w->end[threadIdx.x], w->query_start + (long long)my_row};
+        const int hull_first = w->hull_first, hull_end = w->hull_end, my_from = w->from[x], my_until = w->until[x];
+        const int stop = (hull_end + kSpN - 1) / kSpN, start = hull_first / kSpN;
+        give_back(turn);
+        const float slope2 = BIAS ? p.slopes[qhead] * kScoredLog2e : 0.0f;
         const float slope_held = BIAS ? (CAP ? slope2 : slope2 / mul) : 0.0f;
         float m = -INFINITY, l = 0.0f;
-        bool small = true, ok = true;
+        bool small = true;
         for (int j = my_until - 1; j >= my_from; --j) {
-            const uint32_t parity = (unsigned int)(my_until - 1 - j) & 1u;
+            const uint32_t parity = count & 1u;
+            ++count;
             const int k0 = j * kSpN;
             if (!waited(&sh->s_full[x], parity)) ok = false;
             tc_fence_after_sync();
@@ -362,7 +497,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             mbar_arrive(&sh->s_free);   // the other tile's products may come
             if (k0 < hull_first || k0 + kSpN > hull_end) {
                 // tokens that no row of the CTA sees: their rows of V may hold anything and become zero
-                const unsigned int n = (unsigned int)(stop - 1 - j), stage = n % kSpStages;
+                const unsigned int n = tiles + (unsigned int)(stop - 1 - j), stage = n % kSpStages;
                 if (!waited(&sh->v_full[stage], (n / kSpStages) & 1u)) ok = false;
                 const int token = k0 + (int)tile_row;
                 if (token < hull_first || token >= hull_end) {
@@ -521,8 +656,9 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         }
         // ------------------------------ epilogue ----------------------------------------------------
         const bool any = my_until > my_from;
-        if (ok && any) ok = mbar_wait(&sh->pv_done[x], (unsigned int)(my_until - my_from - 1) & 1u);
-        if (!__all_sync(0xffffffffu, ok)) {
+        tiles += (unsigned int)(stop - start);
+        if (any && !waited(&sh->pv_done[x], (count - 1u) & 1u)) ok = false;
+        if (!ok) {
             fail();
         } else {
             tc_fence_after_sync();
@@ -563,6 +699,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 if (p.row_first || p.row_end) finite = sp_row_again(p, b, qhead, range, my_row);
                 if (!finite) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
             }
+        }
         }
     }
     tc_fence_before_sync();
