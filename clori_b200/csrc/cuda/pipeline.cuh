@@ -173,6 +173,13 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
+__device__ __forceinline__ float max3_abs(float a, float b, float c)
+{
+    float r;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 __device__ __forceinline__ float min3(float a, float b, float c)
 {
     float r;

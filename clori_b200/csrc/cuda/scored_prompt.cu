@@ -12,8 +12,9 @@
 // A thread takes its row's 128 products out of tensor memory twice: once for the maximum, then 64 at a time
 // for the weights, which go back over products that have been read; P V of the first half starts while the
 // second is exponentiated. The score rule runs two lanes at a time (f32x2 instructions):
-//   cap    tanh(x) = x p(x^2), p of degree 4, while every |x| of the warp's tile is at most 3/4: absolute error
-//          below 2e-7 (p was fitted for this kernel); otherwise 1 - 2 / (e^2x + 1) from the exponential unit,
+//   cap    tanh(x) = x p(x^2) with p of degree 3 while every |x| of the warp's tile is at most 5/8 (such logits are
+//          so near each other that no maximum is looked for either), of degree 4 up to 7/8; both were fitted for
+//          this kernel, their absolute error is below 8.5e-7; otherwise 1 - 2 / (e^2x + 1) from the exponential unit,
 //          which is as loaded as the tensor cores (one exponential per score against two more operations).
 //   bias   slope * (s - position) is linear in the token inside a tile: one multiply-add per score and one
 //          constant per row and tile; tokens behind the row's position (prefixes) take |.| in full.
@@ -453,18 +454,24 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         const uint32_t p_col = lane_base + kSpPColumn + x * 64u, o_col = lane_base + kSpOColumn + x * kSpD;
         const unsigned int tile_row = threadIdx.x & 127u;
         // Raw products become exponents (log2 units): s * mul, or mul * tanh(s * to_unit) with
-        // tanh(x) = x (a0 + a1 x^2 + .. + a4 x^8) for |x| <= 3/4, all constants folded into the coefficients.
+        // tanh(x) = x (a0 + a1 x^2 + .. + a4 x^8) for |x| <= 7/8, all constants folded into the coefficients.
         const float mul = (CAP ? p.cap : p.scale) * kScoredLog2e;
-        const float to_unit = CAP ? p.scale / p.cap : 0.0f, inside = CAP ? 0.75f / to_unit : 0.0f;
+        const float to_unit = CAP ? p.scale / p.cap : 0.0f, inside = CAP ? 0.875f / to_unit : 0.0f;
         const float to_exp = to_unit * (2.0f * kScoredLog2e);
-        unsigned long long poly2[5];   // each coefficient twice
+        // With a cap of at most 100 log2 units (69) a row's reference starts at a quarter of it below zero: a weight is
+        // then at least 2^-75, and at most 2^80 while |x| <= 5/8, in range of F32 and bf16 whatever the maximum is.
+        const float lowest = CAP && !BIAS && mul <= 100.0f ? -0.25f * mul : -INFINITY;
+        const float inside_tiny = lowest > -INFINITY ? 0.625f / to_unit : -1.0f;
+        unsigned long long poly2[5], tiny2[4];   // each coefficient twice
         if (CAP) {
-            constexpr float a[5] = {0.999997228434978f, -0.33323076828402465f, 0.13226094281675813f, -0.049280520544446996f,
-                                    0.012318897799912349f};
+            constexpr float a[5] = {0.9999895364888953f, -0.3330450229921434f, 0.13108151117714426f, -0.046552073169092247f,
+                                    0.010236377790690908f};
+            constexpr float a_tiny[4] = {0.999987904734053f, -0.33290581616016607f, 0.1292045463446343f, -0.03864439123986797f};
             float power = to_unit * mul;
 #pragma unroll
             for (int i = 0; i < 5; ++i) {
                 poly2[i] = f2_pack(a[i] * power, a[i] * power);
+                if (i < 4) tiny2[i] = f2_pack(a_tiny[i] * power, a_tiny[i] * power);
                 power *= to_unit * to_unit;
             }
         }
@@ -556,19 +563,18 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     for (int c = 0; c < 128; ++c)
                         if (c < lo || c >= hi) s[c >> 5][c & 31] = 0u;
                 }
-                float top[2] = {-INFINITY, -INFINITY}, low[2] = {INFINITY, INFINITY};
+                float top[2] = {0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < 128; i += 2) {
-                    const float s0 = __uint_as_float(s[i >> 5][i & 31]), s1 = __uint_as_float(s[i >> 5][(i & 31) + 1]);
-                    top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], s0, s1);
-                    low[(i >> 1) & 1] = min3(low[(i >> 1) & 1], s0, s1);
-                }
-                float found = fmaxf(top[0], top[1]);
-                // once false: for the rest of this warp's tiles
-                small = small && __all_sync(0xffffffffu, fmaxf(found, -fminf(low[0], low[1])) <= inside);
-                if (!BIAS && !masked && small) {
-                    found = fmaf(-2.0f * mul, rcp_approx(exp2_approx(found * to_exp) + 1.0f), mul);   // tanh keeps the order
-                    const float offset = agree(found);
+                for (int i = 0; i < 128; i += 2)
+                    top[(i >> 1) & 1] = max3_abs(top[(i >> 1) & 1], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
+                const float largest = fmaxf(top[0], top[1]);
+                const bool tiny = __all_sync(0xffffffffu, largest <= inside_tiny);
+                small = tiny || __all_sync(0xffffffffu, largest <= inside);
+                if (!BIAS && !masked && tiny) {
+                    // no maximum is needed
+                    if (j < my_until - 1 && !waited(&sh->pv_done[x], parity ^ 1u)) ok = false;
+                    if (m == -INFINITY) m = lowest;
+                    const float offset = -m;
                     const unsigned long long offset2 = f2_pack(offset, offset);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -577,7 +583,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         for (int i = 0; i < 64; i += 2) {
                             const unsigned long long v = f2_load(s[2 * h + (i >> 5)], i & 31);
                             float e0, e1;
-                            f2_unpack(f2_fma(v, f2_poly(poly2, f2_mul(v, v)), offset2), e0, e1);
+                            const unsigned long long w2 = f2_mul(v, v);
+                            f2_unpack(f2_fma(v, f2_fma(f2_fma(f2_fma(w2, tiny2[3], tiny2[2]), w2, tiny2[1]), w2, tiny2[0]), offset2), e0, e1);
                             e0 = exp2_approx(e0);
                             e1 = exp2_approx(e1);
                             sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(e0, e1));
@@ -632,7 +639,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 for (int i = 0; i < 128; i += 2)
                     top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
                 const float held = CAP ? 1.0f : mul, found = fmaxf(top[0], top[1]);
-                float offset = agree(found < -1e29f ? -INFINITY : fmaf(found, held, slope2 * ahead_f));
+                float offset = agree(found < -1e29f ? -INFINITY : fmaxf(fmaf(found, held, slope2 * ahead_f), lowest));
                 if (found > 1e29f) offset = __int_as_float(0x7fffffff);   // a NaN (or infinity) inside the run: not lost in the mask
                 const unsigned long long offset2 = f2_pack(offset, offset), held2 = f2_pack(held, held);
 #pragma unroll
