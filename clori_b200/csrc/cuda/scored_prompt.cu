@@ -27,7 +27,8 @@ namespace yvx {
 constexpr int kSpM = 128, kSpN = 128, kSpD = 128, kSpStages = 2, kSpThreads = 384;
 constexpr int kSpHalfBytes = kSpM * 64 * 2;        // [128][64] bf16, swizzled
 constexpr int kSpTileBytes = 2 * kSpHalfBytes;     // 32 KB
-constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 1024 + 5 * 1024;
+constexpr int kSpOutBytes = 32 * 64;               // a warp's rows on their way out, 64 bytes of each at a time
+constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 8 * kSpOutBytes + 1024 + 5 * 1024;
 constexpr float kSpRescale = 8.0f;                 // log2 units the maximum may lag behind
 constexpr uint32_t kSpTmemColumns = 512;           // S 128 | P_A 64 | P_B 64 | O_A 128 | O_B 128
 constexpr int kSpReaders = 11;                     // warps that read a piece of work
@@ -186,7 +187,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
     unsigned char *q_smem = smem;                                  // tile A, then tile B
     unsigned char *k_smem = smem + 2 * kSpTileBytes;
     unsigned char *v_smem = k_smem + kSpStages * kSpTileBytes;
-    SpShared *sh = reinterpret_cast<SpShared *>(v_smem + kSpStages * kSpTileBytes);
+    unsigned char *out_smem = v_smem + kSpStages * kSpTileBytes;
+    SpShared *sh = reinterpret_cast<SpShared *>(out_smem + 8 * kSpOutBytes);
 
     const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     if (threadIdx.x == 0) {
@@ -480,7 +482,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         for (unsigned int turn = 0; ok; ++turn) {
         const SpWork *const w = take(turn);
         if (w == nullptr) break;
-        const unsigned int my_row = w->q0 + threadIdx.x, qhead = w->qhead, b = w->b;
+        const unsigned int w_q0 = w->q0, my_row = w_q0 + threadIdx.x, qhead = w->qhead, b = w->b;
         const bool exists = my_row < p.query_rows;
         const ScoredRange range = {w->first[threadIdx.x], w->end[threadIdx.x], w->query_start + (long long)my_row};
         const int hull_first = w->hull_first, hull_end = w->hull_end, my_from = w->from[x], my_until = w->until[x];
@@ -511,8 +513,10 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     unsigned char *v_row = v_smem + stage * kSpTileBytes + tile_row * 128u;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        *reinterpret_cast<uint4 *>(v_row + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
-                        *reinterpret_cast<uint4 *>(v_row + kSpHalfBytes + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+                        // eight rows write to eight different groups of banks
+                        const unsigned int at = 16u * (i ^ (tile_row & 7u));
+                        *reinterpret_cast<uint4 *>(v_row + at) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4 *>(v_row + kSpHalfBytes + at) = make_uint4(0u, 0u, 0u, 0u);
                     }
                 }
                 fence_proxy_async();
@@ -670,38 +674,59 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         } else {
             tc_fence_after_sync();
             const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-            const unsigned long long item =
-                (((unsigned long long)b * p.query_rows + (exists ? my_row : 0u)) * p.query_heads + qhead) * kSpD;
-            bool finite = l == l;
+            // A thread holds a row, a store wants lanes side by side: 64 bytes of each row (32 bf16 or 16 F32 lanes) at a
+            // time go through shared memory, their four 16-byte pieces in an order that spreads them over the banks.
+            unsigned char *const out = out_smem + warp * kSpOutBytes;
+            const bool narrow = p.output_dtype == YVEX_DTYPE_BF16, sees = range.first < range.end;
+            const unsigned int out_lane = lane >> 2, width = narrow ? 2u : 4u;
+            const unsigned int out_row = w_q0 + x * kSpM + (warp & 3u) * 32u + out_lane;
+            unsigned char *const dst = reinterpret_cast<unsigned char *>(p.output) +
+                (((unsigned long long)b * p.query_rows + out_row) * p.query_heads + qhead) * kSpD * width + 16u * (lane & 3u);
+            const unsigned long long eight_rows = 8ull * p.query_heads * kSpD * width;
+            float check = l * 0.0f;   // NaN once a lane is not finite
+            uint4 staged[4];
+            auto send = [&](int chunk) {
 #pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(out + lane * 64u + 16u * (i ^ ((lane >> 1) & 3u))) = staged[i];
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned int r = 8u * i + out_lane;
+                    const uint4 piece = *reinterpret_cast<const uint4 *>(out + r * 64u + 16u * ((lane & 3u) ^ ((r >> 1) & 3u)));
+                    if (out_row + 8u * i < p.query_rows) *reinterpret_cast<uint4 *>(dst + i * eight_rows + 64 * chunk) = piece;
+                }
+                __syncwarp();
+            };
+#pragma unroll 1
             for (int i = 0; i < 4; ++i) {
                 uint32_t o[32];
 #pragma unroll
                 for (int c = 0; c < 32; ++c) o[c] = 0u;
-                if (any) {   // every lane takes part; only rows that exist store
+                if (any) {
                     tmem_ld32(o_col + 32 * i, o);
                     tmem_wait_ld();
                 }
-                float v[32];
 #pragma unroll
                 for (int c = 0; c < 32; ++c) {
-                    v[c] = range.first < range.end ? __uint_as_float(o[c]) * inverse : 0.0f;
-                    finite = finite && isfinite(v[c]);
+                    const float v = sees ? __uint_as_float(o[c]) * inverse : 0.0f;
+                    check = fmaf(v, 0.0f, check);
+                    o[c] = __float_as_uint(v);
                 }
-                if (!exists) continue;
-                if (p.output_dtype == YVEX_DTYPE_BF16) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<unsigned short *>(p.output) + item + 32 * i);
+                if (narrow) {
 #pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4)
-                        dst[q4] = make_uint4(pack_bf16(v[8 * q4], v[8 * q4 + 1]), pack_bf16(v[8 * q4 + 2], v[8 * q4 + 3]),
-                                             pack_bf16(v[8 * q4 + 4], v[8 * q4 + 5]), pack_bf16(v[8 * q4 + 6], v[8 * q4 + 7]));
+                    for (int c = 0; c < 16; ++c)
+                        (&staged[c >> 2].x)[c & 3] = pack_bf16(__uint_as_float(o[2 * c]), __uint_as_float(o[2 * c + 1]));
+                    send(i);
                 } else {
-                    float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.output) + item + 32 * i);
 #pragma unroll
-                    for (int q4 = 0; q4 < 8; ++q4)
-                        dst[q4] = make_float4(v[4 * q4], v[4 * q4 + 1], v[4 * q4 + 2], v[4 * q4 + 3]);
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) (&staged[c >> 2].x)[c & 3] = o[16 * h + c];
+                        send(2 * i + h);
+                    }
                 }
             }
+            bool finite = check == 0.0f;
             if (exists && !finite) {
                 if (p.row_first || p.row_end) finite = sp_row_again(p, b, qhead, range, my_row);
                 if (!finite) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
