@@ -12,13 +12,14 @@
 // A thread takes its row's 128 products out of tensor memory twice: once for the maximum, then 64 at a time
 // for the weights, which go back over products that have been read; P V of the first half starts while the
 // second is exponentiated. The score rule runs two lanes at a time (f32x2 instructions):
-//   cap    tanh(x) = x p(x^2) with p of degree 3 while every |x| of the warp's tile is at most 5/8 (such logits are
-//          so near each other that no maximum is looked for either), of degree 4 up to 7/8; both were fitted for
-//          this kernel, their absolute error is below 8.5e-7; otherwise 1 - 2 / (e^2x + 1) from the exponential unit,
-//          which is as loaded as the tensor cores (one exponential per score against two more operations).
+//   cap    tanh(x) = x p(x^2) with p of degree 3 while every |x| of the warp's tile is at most 5/8, of degree 6 up to
+//          11/8, beyond 1 - 2 / (e^2x + 1) from the exponential unit, which is as loaded as the tensor cores. A cap bounds the
+//          logits: up to 55 the weights stay in range against the reference 0 and no maximum is looked for.
 //   bias   slope * (s - position) is linear in the token inside a tile: one multiply-add per score and one
 //          constant per row and tile; tokens behind the row's position (prefixes) take |.| in full.
 // Weights are rounded to bf16, sums and the accumulator are F32.
+#include <type_traits>
+
 #include "scored.cuh"
 #include "tcgen05.cuh"
 
@@ -123,11 +124,11 @@ __device__ __forceinline__ void f2_store(unsigned long long v, uint32_t (&s)[32]
     s[c + 1] = __float_as_uint(hi);
 }
 
-// The polynomial of degree 4 in w.
-__device__ __forceinline__ unsigned long long f2_poly(const unsigned long long (&a)[5], unsigned long long w)
-{
-    return f2_fma(f2_fma(f2_fma(f2_fma(w, a[4], a[3]), w, a[2]), w, a[1]), w, a[0]);
-}
+// tanh(x) = x (a0 + a1 x^2 + ..) for |x| <= 5/8 and |x| <= 11/8, fitted for this kernel: the largest absolute errors
+// are 8.3e-7 and 8.2e-7.
+__device__ constexpr float kSpTanhTiny[4] = {0.999987904734053f, -0.33290581616016607f, 0.1292045463446343f, -0.03864439123986797f};
+__device__ constexpr float kSpTanhSmall[7] = {0.9999906071821962f,  -0.3331309371709024f,   0.13205654305843492f, -0.050316830005499996f,
+                                              0.016203115118873665f, -0.0035891439879808845f, 0.00038086217121292696f};
 
 // A row of a finite call that came out non-finite: weights of zero met a NaN or infinity in rows of V that
 // this row does not see (between packed documents, say). It is computed again token by token over what it
@@ -456,27 +457,13 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         const uint32_t p_col = lane_base + kSpPColumn + x * 64u, o_col = lane_base + kSpOColumn + x * kSpD;
         const unsigned int tile_row = threadIdx.x & 127u;
         // Raw products become exponents (log2 units): s * mul, or mul * tanh(s * to_unit) with
-        // tanh(x) = x (a0 + a1 x^2 + .. + a4 x^8) for |x| <= 7/8, all constants folded into the coefficients.
+        // tanh(x) = x (a0 + a1 x^2 + ..), the constants folded into the coefficients.
         const float mul = (CAP ? p.cap : p.scale) * kScoredLog2e;
-        const float to_unit = CAP ? p.scale / p.cap : 0.0f, inside = CAP ? 0.875f / to_unit : 0.0f;
-        const float to_exp = to_unit * (2.0f * kScoredLog2e);
-        // With a cap of at most 100 log2 units (69) a row's reference starts at a quarter of it below zero: a weight is
-        // then at least 2^-75, and at most 2^80 while |x| <= 5/8, in range of F32 and bf16 whatever the maximum is.
-        const float lowest = CAP && !BIAS && mul <= 100.0f ? -0.25f * mul : -INFINITY;
-        const float inside_tiny = lowest > -INFINITY ? 0.625f / to_unit : -1.0f;
-        unsigned long long poly2[5], tiny2[4];   // each coefficient twice
-        if (CAP) {
-            constexpr float a[5] = {0.9999895364888953f, -0.3330450229921434f, 0.13108151117714426f, -0.046552073169092247f,
-                                    0.010236377790690908f};
-            constexpr float a_tiny[4] = {0.999987904734053f, -0.33290581616016607f, 0.1292045463446343f, -0.03864439123986797f};
-            float power = to_unit * mul;
-#pragma unroll
-            for (int i = 0; i < 5; ++i) {
-                poly2[i] = f2_pack(a[i] * power, a[i] * power);
-                if (i < 4) tiny2[i] = f2_pack(a_tiny[i] * power, a_tiny[i] * power);
-                power *= to_unit * to_unit;
-            }
-        }
+        const float to_unit = CAP ? p.scale / p.cap : 0.0f;
+        // Under a cap of at most 80 log2 units (55) every row's reference is 0: weights lie in 2^-80 .. 2^80, in range of
+        // F32 and bf16, and no maximum is looked for.
+        const bool fixed = CAP && !BIAS && mul <= 80.0f;
+        const float inside_tiny = CAP ? 0.625f / to_unit : 0.0f, inside_small = CAP ? 1.375f / to_unit : 0.0f;
         unsigned int tiles = 0u, count = 0u;   // so far: token tiles of the block, of this row tile
         bool ok = true;
         for (unsigned int turn = 0; ok; ++turn) {
@@ -491,7 +478,6 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         const float slope2 = BIAS ? p.slopes[qhead] * kScoredLog2e : 0.0f;
         const float slope_held = BIAS ? (CAP ? slope2 : slope2 / mul) : 0.0f;
         float m = -INFINITY, l = 0.0f;
-        bool small = true;
         for (int j = my_until - 1; j >= my_from; --j) {
             const uint32_t parity = count & 1u;
             ++count;
@@ -521,16 +507,27 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 }
                 fence_proxy_async();
             }
-            const int lo = range.first - k0, hi = range.end - k0;
-            const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kSpN);
+            // rows that do not exist (their Q is zero, nothing is stored) ask for no mask
+            const int lo = exists ? range.first - k0 : 0, hi = exists ? range.end - k0 : kSpN;
+            bool cut[2];   // tokens 64 h .. 64 h + 63: some row of the warp does not see all of them
+#pragma unroll
+            for (int h = 0; h < 2; ++h) cut[h] = __any_sync(0xffffffffu, lo > 64 * h || hi < 64 * h + 64);
+            // a value inside the run [lo, hi) against two ramps: at least kHuge / 2 inside, at most -kHuge / 2 outside,
+            // and the smallest of the three hides what stands there (min passes over a NaN)
+            constexpr float kHuge = 1e30f;
+            const float up = kHuge * (0.5f - (float)max(lo, -kSpN)), down = kHuge * ((float)min(max(hi, -1), 2 * kSpN) - 0.5f);
+            auto hide = [&](float value, int c) { return min3(value, fmaf((float)c, kHuge, up), fmaf((float)c, -kHuge, down)); };
             // the bias of column c: slope * (ahead + c), or -slope * |ahead + c| where a row sees tokens behind itself
             const int ahead = BIAS ? (int)max(min((long long)k0 - range.position, 0x3fffffffll), -0x3fffffffll) : 0;
-            const bool linear = !BIAS || __all_sync(0xffffffffu, (long long)min(range.end, k0 + kSpN) <= range.position + 1);
+            const bool linear = !BIAS || __all_sync(0xffffffffu, !exists || (long long)min(range.end, k0 + kSpN) <= range.position + 1);
             const float ahead_f = BIAS && linear ? (float)ahead : 0.0f;
             // The reference m follows the maximum when it lags by more than 2^8. P of the previous tile is overwritten
             // afterwards, and O may be touched: its P V has to have landed.
-            auto agree = [&](float found) {
+            auto landed = [&]() {
                 if (j < my_until - 1 && !waited(&sh->pv_done[x], parity ^ 1u)) ok = false;
+            };
+            auto agree = [&](float found) {
+                landed();
                 const bool grow = found > m + kSpRescale || (m == -INFINITY && found > -INFINITY);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float fresh = grow ? found : m, factor = m == -INFINITY ? 1.0f : exp2_approx(m - fresh);
@@ -559,43 +556,59 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 mbar_arrive(&sh->p_half[x][h]);      // weights of tokens 64 h .. 64 h + 63
             };
             unsigned long long sum2[2] = {0ull, 0ull};
-            // ---- a cap's common tile: nothing masked, no bias, products inside the polynomial ------------------------
-            bool done = false;
+            // ---- a cap: how large the products are decides on the form of tanh ---------------------------------------
+            bool done = false, small = false;
             if (CAP) {
-                if (masked) {   // columns that a row does not see may hold anything
 #pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c < lo || c >= hi) s[c >> 5][c & 31] = 0u;
-                }
+                for (int h = 0; h < 2; ++h)
+                    if (cut[h]) {   // columns that a row does not see may hold anything
+#pragma unroll
+                        for (int c = 64 * h; c < 64 * h + 64; ++c)
+                            if (c < lo || c >= hi) s[c >> 5][c & 31] = 0u;
+                    }
                 float top[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < 128; i += 2)
                     top[(i >> 1) & 1] = max3_abs(top[(i >> 1) & 1], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
                 const float largest = fmaxf(top[0], top[1]);
-                const bool tiny = __all_sync(0xffffffffu, largest <= inside_tiny);
-                small = tiny || __all_sync(0xffffffffu, largest <= inside);
-                if (!BIAS && !masked && tiny) {
-                    // no maximum is needed
-                    if (j < my_until - 1 && !waited(&sh->pv_done[x], parity ^ 1u)) ok = false;
-                    if (m == -INFINITY) m = lowest;
-                    const float offset = -m;
-                    const unsigned long long offset2 = f2_pack(offset, offset);
+                small = __all_sync(0xffffffffu, largest <= inside_small);
+                // x p(x^2), the exponential, sum and rounding of both halves as one straight run of instructions (a branch
+                // between the halves costs the common tile 13 %)
+                auto weights = [&](const auto &a, auto masks) {
+                    constexpr int kTerms = sizeof(a) / sizeof(a[0]);
+                    constexpr bool kMasks = decltype(masks)::value;
+                    unsigned long long poly2[kTerms];   // each coefficient twice
+                    float power = to_unit * mul;
+#pragma unroll
+                    for (int i = 0; i < kTerms; ++i) {
+                        poly2[i] = f2_pack(a[i] * power, a[i] * power);
+                        power *= to_unit * to_unit;
+                    }
+                    landed();
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t packed[32];
 #pragma unroll
                         for (int i = 0; i < 64; i += 2) {
-                            const unsigned long long v = f2_load(s[2 * h + (i >> 5)], i & 31);
-                            float e0, e1;
+                            unsigned long long v = f2_load(s[2 * h + (i >> 5)], i & 31);
+                            if (kMasks || kTerms > 4) asm volatile("" : "+l"(v));   // or what several branches share is drawn in front of them
                             const unsigned long long w2 = f2_mul(v, v);
-                            f2_unpack(f2_fma(v, f2_fma(f2_fma(f2_fma(w2, tiny2[3], tiny2[2]), w2, tiny2[1]), w2, tiny2[0]), offset2), e0, e1);
-                            e0 = exp2_approx(e0);
-                            e1 = exp2_approx(e1);
+                            unsigned long long r = poly2[kTerms - 1];
+#pragma unroll
+                            for (int k = kTerms - 2; k >= 0; --k) r = f2_fma(r, w2, poly2[k]);
+                            float e0, e1;
+                            f2_unpack(f2_mul(v, r), e0, e1);
+                            e0 = exp2_approx(kMasks ? hide(e0, 64 * h + i) : e0);
+                            e1 = exp2_approx(kMasks ? hide(e1, 64 * h + i + 1) : e1);
                             sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(e0, e1));
                             packed[i >> 1] = pack_bf16(e0, e1);
                         }
                         hand_over(packed, h);
                     }
+                };
+                if (fixed && small && !cut[0] && !cut[1]) {
+                    if (__all_sync(0xffffffffu, largest <= inside_tiny)) weights(kSpTanhTiny, std::false_type{});
+                    else weights(kSpTanhSmall, std::false_type{});
                     done = true;
                 }
             }
@@ -603,11 +616,21 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 // ---- without a cap: raw products, the bias in their units; with one: logits in log2 units. Then the mask,
                 // the maximum and the weights are the same for all.
                 if (CAP) {
+                    const float to_exp = to_unit * (2.0f * kScoredLog2e);
                     if (small) {
+                        float power = to_unit * mul, a[7];
+#pragma unroll
+                        for (int i = 0; i < 7; ++i) {
+                            a[i] = kSpTanhSmall[i] * power;
+                            power *= to_unit * to_unit;
+                        }
 #pragma unroll
                         for (int i = 0; i < 128; i += 2) {
-                            const unsigned long long v = f2_load(s[i >> 5], i & 31);
-                            f2_store(f2_mul(v, f2_poly(poly2, f2_mul(v, v))), s[i >> 5], i & 31);
+                            const unsigned long long v = f2_load(s[i >> 5], i & 31), w2 = f2_mul(v, v);
+                            unsigned long long r = f2_pack(a[6], a[6]);
+#pragma unroll
+                            for (int k = 5; k >= 0; --k) r = f2_fma(r, w2, f2_pack(a[k], a[k]));
+                            f2_store(f2_mul(v, r), s[i >> 5], i & 31);
                         }
                     } else {
 #pragma unroll
@@ -628,23 +651,25 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                                 __float_as_uint(fmaf(-slope_held, fabsf((float)(ahead + c)), __uint_as_float(s[c >> 5][c & 31])));
                     }
                 }
-                if (masked) {
-                    // the smaller of the value and two ramps: at least kHuge / 2 inside the run, at most -kHuge / 2
-                    // outside, whatever stands there (min passes over a NaN)
-                    constexpr float kHuge = 1e30f;
-                    const float up = kHuge * (0.5f - (float)max(lo, -kSpN)), down = kHuge * ((float)min(max(hi, -1), 2 * kSpN) - 0.5f);
+                if (cut[0] || cut[1]) {
 #pragma unroll
                     for (int c = 0; c < 128; ++c)
-                        s[c >> 5][c & 31] = __float_as_uint(min3(__uint_as_float(s[c >> 5][c & 31]), fmaf((float)c, kHuge, up),
-                                                                 fmaf((float)c, -kHuge, down)));
+                        s[c >> 5][c & 31] = __float_as_uint(hide(__uint_as_float(s[c >> 5][c & 31]), c));
                 }
-                float top[2] = {-INFINITY, -INFINITY};
+                const float held = CAP ? 1.0f : mul;
+                float offset = 0.0f;
+                if (fixed) {
+                    landed();
+                } else {
+                    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 128; i += 2)
-                    top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
-                const float held = CAP ? 1.0f : mul, found = fmaxf(top[0], top[1]);
-                float offset = agree(found < -1e29f ? -INFINITY : fmaxf(fmaf(found, held, slope2 * ahead_f), lowest));
-                if (found > 1e29f) offset = __int_as_float(0x7fffffff);   // a NaN (or infinity) inside the run: not lost in the mask
+                    for (int i = 0; i < 128; i += 2)
+                        top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
+                    const float found = fmaxf(top[0], top[1]);
+                    offset = agree(found < -1e29f ? -INFINITY : fmaf(found, held, slope2 * ahead_f));
+                    // a NaN (or infinity) inside the run: not lost in the mask (under a fixed reference its weight is infinite)
+                    if (found > 1e29f) offset = __int_as_float(0x7fffffff);
+                }
                 const unsigned long long offset2 = f2_pack(offset, offset), held2 = f2_pack(held, held);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
