@@ -101,7 +101,7 @@ __device__ __forceinline__ void scored_store_empty(const yvx_scored_problem &p, 
 int scored_general_launch(const yvx_scored_problem &p, cudaStream_t stream);
 int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream);
 unsigned long long scored_stage_bytes(const yvx_scored_problem &p);
-int scored_stage_launch(const yvx_scored_problem &p, yvx_scored_problem *staged, cudaStream_t stream);
+int scored_stage_launch(const yvx_scored_problem &p, void *rows, yvx_scored_problem *staged, cudaStream_t stream);
 int scored_decode_launch(const yvx_scored_problem &p, cudaStream_t stream);
 int scored_combine_launch(const yvx_scored_problem &p, cudaStream_t stream);
 

@@ -43,9 +43,8 @@ static unsigned long long scored_span(const yvx_scored_problem *p)
     return seen < all ? (seen + 63ull) / 64ull * 64ull : all;
 }
 
-// Calls of more than 64 vectors (query rows x heads of a KV head) on the shapes of the tensor cores: the
-// rows fill 128-row tiles by themselves and the KV sequence is not split. Decided by the shape, types and
-// alignment alone, before the plan.
+// Calls of more than 64 vectors (query rows x heads of a KV head) on the shapes of the tensor cores. Decided by the
+// shape, types and alignment alone, before the plan.
 static bool scored_prompt_shape(const yvx_scored_problem *p)
 {
     const unsigned long long bytes = p->kv_code == YVX_KV_PLAIN ? 2ull : 1ull;
@@ -57,6 +56,14 @@ static bool scored_prompt_shape(const yvx_scored_problem *p)
            (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) > 64ull &&
            !((reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value) |
               reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->output) | strides * bytes | q_strides * 2ull) & 15ull);
+}
+
+// Partial rows of all splits, a multiple of 256 bytes; staged rows lie behind them.
+static unsigned long long scored_partial_bytes(const yvx_scored_problem *p)
+{
+    if (p->max_splits <= 1u) return 0ull;
+    const unsigned long long items = (unsigned long long)p->sessions * p->query_rows * p->query_heads;
+    return (items * p->max_splits * (p->head_dim + 4ull) * 4ull + 255ull) / 256ull * 256ull;
 }
 
 // Caches that the tensor-core kernel does not read in place: codes, and pages that are no multiple of 64 tokens.
@@ -74,6 +81,10 @@ extern "C" {
 // partial rows); the chunk with the smallest sum is taken, at most 8192 tokens. One session of 4096 tokens:
 // 128 tokens 10.3 us, 64 tokens 15.4, 512 tokens 13.0; 64 sessions behind a window of 4096: one chunk 177 us,
 // two 193, four 190; one session of 131072 tokens: 3584 (one wave) 95 us, 1792 107, 4096 105.
+// Prompt-sized calls are split only to fill the machine: one CTA on an SM, a piece of work is 256 rows of a head, a
+// split costs its tiles of 128 tokens and about five more, the fold two tiles and its traffic. 32 heads over 131072
+// tokens, 20 rows: one split 1330 us, four 346, five 538, nine (taken) 313; 256 rows: 1655, 493, 813, 476;
+// 300 rows over 32768: one 422, two (taken) 260, three 305; 2048 rows over 16384: one (taken) 437, two 690.
 void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
 {
     if (!p || !p->kv_heads || !p->query_rows || !p->kv_tokens_max) return;
@@ -82,7 +93,20 @@ void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
     const unsigned long long span = yvx::scored_span(p);
     const unsigned long long lanes = (unsigned long long)p->sessions * p->kv_heads * ((vectors + 15ull) / 16ull);
     unsigned long long best = span, best_cost = ~0ull;
-    if (!yvx::scored_prompt_shape(p) && (vectors <= 64ull || lanes < wave)) {
+    if (yvx::scored_prompt_shape(p)) {
+        const unsigned long long pieces = (unsigned long long)p->sessions * p->query_heads * ((p->query_rows + 255ull) / 256ull);
+        const unsigned long long moved = (unsigned long long)p->sessions * p->query_rows * p->query_heads * 1056ull;
+        for (unsigned long long splits = 1ull; splits <= (span + 127ull) / 128ull && splits <= 8192ull; ++splits) {
+            const unsigned long long tiles = ((span + 127ull) / 128ull + splits - 1ull) / splits;
+            const unsigned long long cost = (pieces * splits + wave / 2ull - 1ull) / (wave / 2ull) * (tiles + 5ull) +
+                                            (splits > 1ull ? 2ull + splits * moved / (8ull << 20) : 0ull);
+            if (cost < best_cost) {
+                best_cost = cost;
+                best = splits > 1ull ? tiles * 128ull : span;
+            }
+            if (pieces * splits >= 2ull * wave) break;
+        }
+    } else if (vectors <= 64ull || lanes < wave) {
         for (unsigned long long chunk = 64ull; chunk <= 8192ull; chunk += 64ull) {
             const unsigned long long splits = (span + chunk - 1ull) / chunk;
             const unsigned long long cost = (lanes * splits + wave - 1ull) / wave * (4ull + chunk / 64ull);
@@ -101,9 +125,8 @@ void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
 unsigned long long yvx_cuda_scored_workspace_bytes(const yvx_scored_problem *p)
 {
     if (!p || !p->kv_heads || !p->query_rows) return 0ull;
-    if (p->max_splits <= 1u)
-        return yvx::scored_prompt_shape(p) && yvx::scored_needs_stage(p) ? yvx::scored_stage_bytes(*p) : 0ull;
-    return (unsigned long long)p->sessions * p->query_rows * p->query_heads * p->max_splits * (p->head_dim + 4ull) * 4ull;
+    return yvx::scored_partial_bytes(p) +
+           (yvx::scored_prompt_shape(p) && yvx::scored_needs_stage(p) ? yvx::scored_stage_bytes(*p) : 0ull);
 }
 
 int yvx_cuda_scored_attention(const yvx_scored_problem *p, void *stream, unsigned int *launches)
@@ -116,11 +139,11 @@ int yvx_cuda_scored_attention(const yvx_scored_problem *p, void *stream, unsigne
         return yvx::scored_refuse(YVEX_ERR_BOUNDS, "scored attention: the workspace is missing, misaligned or too small");
     cudaStream_t s = (cudaStream_t)stream;
     unsigned int count = 0u;
-    rc = 0;  // specialised kernels answer 1 or 2 (no fold needed) when they took the call, 0 when its shape is not theirs
-    if (yvx::scored_prompt_shape(p) && p->max_splits == 1u) {
+    rc = 0;  // specialised kernels answer 1 when they took the call, 0 when its shape is not theirs
+    if (yvx::scored_prompt_shape(p)) {
         yvx_scored_problem staged = *p;
         if (yvx::scored_needs_stage(p)) {
-            rc = yvx::scored_stage_launch(*p, &staged, s);
+            rc = yvx::scored_stage_launch(*p, static_cast<unsigned char *>(p->workspace) + yvx::scored_partial_bytes(p), &staged, s);
             if (rc != 0) return rc;
             ++count;
         }

@@ -44,7 +44,7 @@ struct SpWork {
     int first[2 * kSpM], end[2 * kSpM];   // visible run of each row; rows that do not exist see nothing
     int hull_first, hull_end;             // of all of them
     int from[2], until[2];                // token tiles [from[x], until[x]) of the two row tiles
-    unsigned int q0, qhead, b;
+    unsigned int q0, qhead, b, split;
     int valid;                            // 0: nothing is left
     long long query_start;
 };
@@ -132,9 +132,9 @@ __device__ constexpr float kSpTanhSmall[7] = {0.9999906071821962f,  -0.333130937
 
 // A row of a finite call that came out non-finite: weights of zero met a NaN or infinity in rows of V that
 // this row does not see (between packed documents, say). It is computed again token by token over what it
-// does see. Rare and slow (a thread per row).
+// does see, into `part` or as the final row. Rare and slow (a thread per row).
 __device__ __noinline__ bool sp_row_again(const yvx_scored_problem &p, unsigned int b, unsigned int qhead,
-                                          const ScoredRange &range, unsigned int row)
+                                          const ScoredRange &range, unsigned int row, float *part)
 {
     const unsigned int kv_head = qhead / (p.query_heads / p.kv_heads);
     const __nv_bfloat16 *q = reinterpret_cast<const __nv_bfloat16 *>(p.query) + (unsigned long long)b * p.query_session_stride +
@@ -169,16 +169,18 @@ __device__ __noinline__ bool sp_row_again(const yvx_scored_problem &p, unsigned 
     }
     bool finite = true;
     for (int d = 0; d < kSpD; ++d) {
-        const float x = l == 0.0f ? 0.0f : o[d] / l;
+        const float x = part ? o[d] : l == 0.0f ? 0.0f : o[d] / l;
         finite = finite && isfinite(x);
-        store_output(p.output, p.output_dtype, item + d, x);
+        if (part) part[d] = x;
+        else store_output(p.output, p.output_dtype, item + d, x);
     }
+    if (part) part[kSpD] = m, part[kSpD + 1] = l;
     return finite;
 }
 
-// grid: one dimension. (session, head) lanes in groups whose K and V fit the L2 together; inside a group the
+// grid: one dimension, the split of the KV sequence slowest. (session, head) lanes in groups whose K and V fit the L2 together; inside a group the
 // pair of row tiles varies slowest, last rows first, and the lane fastest.
-template <bool CAP, bool BIAS>
+template <bool CAP, bool BIAS, bool SPLIT>
 __global__ void __launch_bounds__(kSpThreads, 1)
 scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps maps, const int head_inner,
                      const unsigned int lane_group)
@@ -384,16 +386,19 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             // ------------------------------ pieces of work ------------------------------------------
             // The block's own first, then those of blocks that have not started, as long as there are any.
             const unsigned int pairs = (p.query_rows + 2 * kSpM - 1) / (2 * kSpM);
-            const unsigned long long per_group = (unsigned long long)pairs * lane_group;
+            const unsigned int per_group = pairs * lane_group;   // the grid holds it: below 2^31
+            const unsigned int per_split = (p.query_heads * p.sessions + lane_group - 1u) / lane_group * per_group;
             unsigned int block = blockIdx.x, asked = 0u;
             bool ok = true, more = true;
             for (unsigned int turn = 0; ok && more; ++turn) {
                 SpWork *const w = &sh->work[turn & 1u];
                 if (turn >= 2u) ok = waited(&sh->work_empty[turn & 1u], ((turn >> 1) - 1u) & 1u);
-                unsigned int work_lane = 0u, within = 0u;
+                unsigned int work_lane = 0u, within = 0u, split = 0u;
                 auto given = [&]() {
-                    within = (unsigned int)(block % per_group);
-                    work_lane = (unsigned int)(block / per_group) * lane_group + within % lane_group;
+                    split = SPLIT ? block / per_split : 0u;
+                    const unsigned int rest = SPLIT ? block % per_split : block;
+                    within = rest % per_group;
+                    work_lane = rest / per_group * lane_group + within % lane_group;
                     return work_lane < p.query_heads * p.sessions;   // the last group may be short
                 };
                 bool look = turn > 0u || !given();
@@ -415,27 +420,42 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     const unsigned int qhead = work_lane % p.query_heads, b = work_lane / p.query_heads;
                     const unsigned int kv_tokens = admitted_kv_tokens(p.kv_tokens, b, p.kv_tokens_uniform, p.kv_tokens_max, p.status);
                     const long long query_start = scored_query_start(p, b, kv_tokens);
-                    int hull_first = 0x7fffffff, hull_end = 0;
+                    int hull_first, hull_end;
+                    auto look_at_rows = [&](int t0, int t1) {   // as far as they see tokens [t0, t1)
+                        hull_first = 0x7fffffff, hull_end = 0;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        int lo = 0x7fffffff, hi = 0;
+                        for (int x = 0; x < 2; ++x) {
+                            int lo = 0x7fffffff, hi = 0;
 #pragma unroll
-                        for (int i = 0; i < kSpM / 32; ++i) {
-                            const unsigned int at = x * kSpM + 32u * i + lane;
-                            ScoredRange range = {0, 0, 0};
-                            if (q0 + at < p.query_rows) range = scored_range(p, b, q0 + at, kv_tokens, query_start);
-                            w->first[at] = range.first, w->end[at] = range.end;
-                            if (range.first < range.end) lo = min(lo, range.first), hi = max(hi, range.end);
+                            for (int i = 0; i < kSpM / 32; ++i) {
+                                const unsigned int at = x * kSpM + 32u * i + lane;
+                                ScoredRange range = {0, 0, 0};
+                                if (q0 + at < p.query_rows) range = scored_range(p, b, q0 + at, kv_tokens, query_start);
+                                if (SPLIT) {
+                                    range.first = max(range.first, t0), range.end = min(range.end, t1);
+                                    if (range.first >= range.end) range.first = range.end = 0;
+                                }
+                                w->first[at] = range.first, w->end[at] = range.end;
+                                if (range.first < range.end) lo = min(lo, range.first), hi = max(hi, range.end);
+                            }
+                            lo = __reduce_min_sync(0xffffffffu, lo);
+                            hi = __reduce_max_sync(0xffffffffu, hi);
+                            if (lane == 0) w->from[x] = hi > 0 ? lo / kSpN : 0, w->until[x] = (hi + kSpN - 1) / kSpN;
+                            hull_first = min(hull_first, lo);
+                            hull_end = max(hull_end, hi);
                         }
-                        lo = __reduce_min_sync(0xffffffffu, lo);
-                        hi = __reduce_max_sync(0xffffffffu, hi);
-                        if (lane == 0) w->from[x] = hi > 0 ? lo / kSpN : 0, w->until[x] = (hi + kSpN - 1) / kSpN;
-                        hull_first = min(hull_first, lo);
-                        hull_end = max(hull_end, hi);
+                    };
+                    look_at_rows(0, 0x7fffffff);
+                    if (SPLIT && hull_end > 0) {
+                        // a split takes its part of the pair's own hull, from the hull's first boundary of 128 tokens; the
+                        // last one takes what is left
+                        const long long t0 = (hull_first & ~(kSpN - 1)) + (long long)split * p.chunk_tokens;
+                        look_at_rows((int)min(t0, (long long)hull_end),
+                                     split + 1u < p.max_splits ? (int)min(t0 + p.chunk_tokens, (long long)hull_end) : hull_end);
                     }
                     if (hull_end == 0) hull_first = 0;
                     if (lane == 0)
-                        w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->qhead = qhead, w->b = b,
+                        w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->qhead = qhead, w->b = b, w->split = split,
                         w->query_start = query_start;
                     tiles = (hull_end + kSpN - 1) / kSpN - hull_first / kSpN;
                 }
@@ -469,7 +489,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         for (unsigned int turn = 0; ok; ++turn) {
         const SpWork *const w = take(turn);
         if (w == nullptr) break;
-        const unsigned int w_q0 = w->q0, my_row = w_q0 + threadIdx.x, qhead = w->qhead, b = w->b;
+        const unsigned int w_q0 = w->q0, my_row = w_q0 + threadIdx.x, qhead = w->qhead, b = w->b, split = w->split;
         const bool exists = my_row < p.query_rows;
         const ScoredRange range = {w->first[threadIdx.x], w->end[threadIdx.x], w->query_start + (long long)my_row};
         const int hull_first = w->hull_first, hull_end = w->hull_end, my_from = w->from[x], my_until = w->until[x];
@@ -698,16 +718,19 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             fail();
         } else {
             tc_fence_after_sync();
-            const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inverse = SPLIT ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             // A thread holds a row, a store wants lanes side by side: 64 bytes of each row (32 bf16 or 16 F32 lanes) at a
             // time go through shared memory, their four 16-byte pieces in an order that spreads them over the banks.
             unsigned char *const out = out_smem + warp * kSpOutBytes;
-            const bool narrow = p.output_dtype == YVEX_DTYPE_BF16, sees = range.first < range.end;
+            const bool narrow = !SPLIT && p.output_dtype == YVEX_DTYPE_BF16, sees = range.first < range.end;
             const unsigned int out_lane = lane >> 2, width = narrow ? 2u : 4u;
             const unsigned int out_row = w_q0 + x * kSpM + (warp & 3u) * 32u + out_lane;
-            unsigned char *const dst = reinterpret_cast<unsigned char *>(p.output) +
-                (((unsigned long long)b * p.query_rows + out_row) * p.query_heads + qhead) * kSpD * width + 16u * (lane & 3u);
-            const unsigned long long eight_rows = 8ull * p.query_heads * kSpD * width;
+            const unsigned long long out_item = ((unsigned long long)b * p.query_rows + out_row) * p.query_heads + qhead;
+            unsigned char *const dst = 16u * (lane & 3u) +
+                (SPLIT ? reinterpret_cast<unsigned char *>(scored_partial(p, out_item, split))
+                         : reinterpret_cast<unsigned char *>(p.output) + out_item * kSpD * width);
+            const unsigned long long eight_rows =
+                8ull * p.query_heads * (SPLIT ? p.max_splits * (kSpD + 4ull) * sizeof(float) : (unsigned long long)kSpD * width);
             float check = l * 0.0f;   // NaN once a lane is not finite
             uint4 staged[4];
             auto send = [&](int chunk) {
@@ -752,9 +775,14 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 }
             }
             bool finite = check == 0.0f;
-            if (exists && !finite) {
-                if (p.row_first || p.row_end) finite = sp_row_again(p, b, qhead, range, my_row);
-                if (!finite) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
+            if (exists) {
+                float *part = SPLIT ? scored_partial(p, ((unsigned long long)b * p.query_rows + my_row) * p.query_heads + qhead, split)
+                                      : nullptr;
+                if (SPLIT) part[kSpD] = fixed ? 0.0f : m, part[kSpD + 1] = l;
+                if (!finite) {
+                    if (p.row_first || p.row_end) finite = sp_row_again(p, b, qhead, range, my_row, part);
+                    if (!finite) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
+                }
             }
         }
         }
@@ -768,7 +796,7 @@ bool scored_encode_rows(CUtensorMap *map, const void *base, int element_bytes, u
                         unsigned long long head_stride, unsigned long long outer_stride, unsigned long long tokens,
                         unsigned long long heads, unsigned long long outer, bool head_inner, unsigned int box_tokens);
 
-// 2: launched and final (nothing to fold), 0: not this kernel's shape, negative: an error.
+// 1: launched, 0: not this kernel's shape, negative: an error.
 int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
 {
     const unsigned long long head_stride = p.query_head_stride ? p.query_head_stride : kSpD;
@@ -794,18 +822,20 @@ int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
     if (streams < 1ull) streams = 1ull;
     const unsigned long long lane_group = streams * group < lanes ? streams * group : lanes;
     const unsigned long long pairs = (p.query_rows + 2ull * kSpM - 1ull) / (2ull * kSpM);
-    const unsigned long long ctas = (lanes + lane_group - 1ull) / lane_group * lane_group * pairs;
+    const unsigned long long ctas = (lanes + lane_group - 1ull) / lane_group * lane_group * pairs * p.max_splits;
     if (lanes > 0xffffffffull || ctas > 0x7fffffffull) return 0;
     const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
-    void (*const kernels[4])(const yvx_scored_problem, const SpMaps, const int, const unsigned int) = {
-        scored_prompt_kernel<false, false>, scored_prompt_kernel<true, false>, scored_prompt_kernel<false, true>,
-        scored_prompt_kernel<true, true>};
-    const auto kernel = kernels[(cap ? 1 : 0) + (bias ? 2 : 0)];
+    void (*const kernels[8])(const yvx_scored_problem, const SpMaps, const int, const unsigned int) = {
+        scored_prompt_kernel<false, false, false>, scored_prompt_kernel<true, false, false>,
+        scored_prompt_kernel<false, true, false>,  scored_prompt_kernel<true, true, false>,
+        scored_prompt_kernel<false, false, true>,  scored_prompt_kernel<true, false, true>,
+        scored_prompt_kernel<false, true, true>,   scored_prompt_kernel<true, true, true>};
+    const auto kernel = kernels[(cap ? 1 : 0) + (bias ? 2 : 0) + (p.max_splits > 1u ? 4 : 0)];
     YVX_CUDA_TRY(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpSmemBytes));
     kernel<<<dim3((unsigned int)ctas, 1, 1), kSpThreads, kSpSmemBytes, stream>>>(p, maps, head_inner ? 1 : 0,
                                                                               (unsigned int)lane_group);
     const int rc = yvx_cuda_check(cudaGetLastError(), "scored_prompt_kernel");
-    return rc != 0 ? rc : 2;
+    return rc != 0 ? rc : 1;
 }
 
 }  // namespace yvx

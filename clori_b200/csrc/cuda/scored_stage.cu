@@ -85,15 +85,15 @@ unsigned long long scored_stage_bytes(const yvx_scored_problem &p)
     return 2ull * p.sessions * p.kv_heads * stage_tokens(p) * 128ull * 2ull;
 }
 
-// Enqueues the staging and describes the staged rows.
-int scored_stage_launch(const yvx_scored_problem &p, yvx_scored_problem *staged, cudaStream_t stream)
+// Enqueues the staging into `rows` and describes the staged rows.
+int scored_stage_launch(const yvx_scored_problem &p, void *rows, yvx_scored_problem *staged, cudaStream_t stream)
 {
     if (p.kv_heads > 65535u) {
         yvx_cuda_set_error_text("scored attention: more than 65535 KV heads");
         return YVEX_ERR_BOUNDS;
     }
     const unsigned long long tokens = stage_tokens(p);
-    unsigned short *key = reinterpret_cast<unsigned short *>(p.workspace);
+    unsigned short *key = reinterpret_cast<unsigned short *>(rows);
     unsigned short *value = key + (unsigned long long)p.sessions * p.kv_heads * tokens * 128ull;
     const dim3 grid((unsigned int)(tokens / 32ull), p.kv_heads, p.sessions);
     if (p.kv_code == YVX_KV_E4M3)
