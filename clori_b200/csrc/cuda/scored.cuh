@@ -38,6 +38,14 @@ __device__ __forceinline__ ScoredRange scored_range(const yvx_scored_problem &p,
     return r;
 }
 
+// Query heads that share a 128-row tile of the prompt kernel: a KV head's group, so that few query rows fill a
+// tile too. One where a tile does not hold a group.
+__host__ __device__ __forceinline__ unsigned int scored_packed_heads(const yvx_scored_problem &p)
+{
+    const unsigned int group = p.query_heads / p.kv_heads;
+    return group <= 128u ? group : 1u;
+}
+
 // The run of tokens that some row of [row0, row1) sees (first == end: none does); all 32 lanes.
 __device__ __forceinline__ void scored_hull(const yvx_scored_problem &p, unsigned int b, unsigned int row0,
                                             unsigned int row1, unsigned int kv_tokens, long long query_start,

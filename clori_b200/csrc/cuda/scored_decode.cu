@@ -571,7 +571,8 @@ static ScoredEncodeFn scored_encode_entry()
 // Returns false when tiled copies cannot describe the layout.
 bool scored_encode_rows(CUtensorMap *map, const void *base, int element_bytes, unsigned long long token_stride,
                         unsigned long long head_stride, unsigned long long outer_stride, unsigned long long tokens,
-                        unsigned long long heads, unsigned long long outer, bool head_inner, unsigned int box_tokens)
+                        unsigned long long heads, unsigned long long outer, bool head_inner, unsigned int box_tokens,
+                        unsigned int box_heads)
 {
     ScoredEncodeFn encode = scored_encode_entry();
     const unsigned long long tb = token_stride * element_bytes, hb = head_stride * element_bytes;
@@ -582,7 +583,8 @@ bool scored_encode_rows(CUtensorMap *map, const void *base, int element_bytes, u
         return false;
     const cuuint64_t dims[4] = {kSdDim, head_inner ? heads : tokens, head_inner ? tokens : heads, outer};
     const cuuint64_t strides[3] = {head_inner ? hb : tb, head_inner ? tb : hb, ob};
-    const cuuint32_t box[4] = {128u / (unsigned int)element_bytes, head_inner ? 1u : box_tokens, head_inner ? box_tokens : 1u, 1u};
+    const cuuint32_t box[4] = {128u / (unsigned int)element_bytes, head_inner ? box_heads : box_tokens,
+                               head_inner ? box_tokens : box_heads, 1u};
     const cuuint32_t steps[4] = {1, 1, 1, 1};
     return encode(map, element_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                   const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -612,9 +614,9 @@ int scored_decode_launch(const yvx_scored_problem &p, cudaStream_t stream)
     const unsigned long long outer = p.block_table ? p.pool_blocks : p.sessions;
     SdMaps maps;
     if (!scored_encode_rows(&maps.key, p.key, element_bytes, p.key_token_stride, p.key_head_stride, p.key_outer_stride, tokens,
-                            p.kv_heads, outer, head_inner, unit) ||
+                            p.kv_heads, outer, head_inner, unit, 1u) ||
         !scored_encode_rows(&maps.value, p.value, element_bytes, p.value_token_stride, p.value_head_stride,
-                            p.value_outer_stride, tokens, p.kv_heads, outer, head_inner, unit))
+                            p.value_outer_stride, tokens, p.kv_heads, outer, head_inner, unit, 1u))
         return 0;
     void (*const kernels[3])(const yvx_scored_problem, const SdMaps, const int, const int) = {
         scored_decode_kernel<YVX_KV_PLAIN>, scored_decode_kernel<YVX_KV_E4M3>, scored_decode_kernel<YVX_KV_I8>};

@@ -94,7 +94,8 @@ void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
     const unsigned long long lanes = (unsigned long long)p->sessions * p->kv_heads * ((vectors + 15ull) / 16ull);
     unsigned long long best = span, best_cost = ~0ull;
     if (yvx::scored_prompt_shape(p)) {
-        const unsigned long long pieces = (unsigned long long)p->sessions * p->query_heads * ((p->query_rows + 255ull) / 256ull);
+        const unsigned long long heads = yvx::scored_packed_heads(*p), rows = 2ull * (128ull / heads);   // of a piece of work
+        const unsigned long long pieces = p->sessions * (p->query_heads / heads) * ((p->query_rows + rows - 1ull) / rows);
         const unsigned long long moved = (unsigned long long)p->sessions * p->query_rows * p->query_heads * 1056ull;
         for (unsigned long long splits = 1ull; splits <= (span + 127ull) / 128ull && splits <= 8192ull; ++splits) {
             const unsigned long long tiles = ((span + 127ull) / 128ull + splits - 1ull) / splits;

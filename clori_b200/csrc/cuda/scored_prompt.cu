@@ -1,7 +1,8 @@
 // Scored attention for prompt-sized calls on the 5th-generation tensor cores: bf16 Q / K / V,
 // head_dim 128, contiguous rows or pages of 64 n tokens, any rule and any visible runs.
 //
-// A CTA owns two tiles (A, B) of 128 query rows of one head: while one tile is in its softmax the
+// A CTA owns two tiles (A, B) of 128 rows, a row being a (query row, head of the KV head's group) pair: a tile of
+// a group of 4 is 32 query rows, which see fewer tokens in vain than 128 do, and few rows fill it. While one tile is in its softmax the
 // other is in its matrix products. Warp 8 brings K and V in tiles of 128 tokens (tiled copies,
 // 128-byte swizzle, two stages each), warp 9 issues S = Q K^T (both operands in shared memory) and
 // O += P V (P in tensor memory, where it overwrites its scores), warps 0-3 and 4-7 run the softmax
@@ -29,7 +30,7 @@ constexpr int kSpM = 128, kSpN = 128, kSpD = 128, kSpStages = 2, kSpThreads = 38
 constexpr int kSpHalfBytes = kSpM * 64 * 2;        // [128][64] bf16, swizzled
 constexpr int kSpTileBytes = 2 * kSpHalfBytes;     // 32 KB
 constexpr int kSpOutBytes = 32 * 64;               // a warp's rows on their way out, 64 bytes of each at a time
-constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 8 * kSpOutBytes + 1024 + 5 * 1024;
+constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 8 * kSpOutBytes + 1024 + 6 * 1024;
 constexpr float kSpRescale = 8.0f;                 // log2 units the maximum may lag behind
 constexpr uint32_t kSpTmemColumns = 512;           // S 128 | P_A 64 | P_B 64 | O_A 128 | O_B 128
 constexpr int kSpReaders = 11;                     // warps that read a piece of work
@@ -39,12 +40,12 @@ struct SpMaps {
     CUtensorMap query, key, value;
 };
 
-// One piece of work: two row tiles of one head and what they see. Warp 11 fills it.
+// One piece of work: two row tiles and what they see. Warp 11 fills it.
 struct SpWork {
-    int first[2 * kSpM], end[2 * kSpM];   // visible run of each row; rows that do not exist see nothing
+    int first[2 * kSpM], end[2 * kSpM];   // visible run of each query row; rows that do not exist see nothing
     int hull_first, hull_end;             // of all of them
     int from[2], until[2];                // token tiles [from[x], until[x]) of the two row tiles
-    unsigned int q0, qhead, b, split;
+    unsigned int q0, head, b, split;      // first query row, first query head
     int valid;                            // 0: nothing is left
     long long query_start;
 };
@@ -56,9 +57,10 @@ struct SpShared {
     uint64_t k_full[kSpStages], k_empty[kSpStages], v_full[kSpStages], v_empty[kSpStages];
     uint64_t s_full[2], s_free, p_half[2][2], pv_done[2];
     uint32_t tmem_base;
+    unsigned int where[kSpM];             // a tile's row: its query row | its head << 16, or ~0 when it is not used
     SpWork work[2];
 };
-static_assert(sizeof(SpShared) <= 5 * 1024, "the barrier block outgrew its slot");
+static_assert(sizeof(SpShared) <= 6 * 1024, "the barrier block outgrew its slot");
 
 // Asks the hardware for a block of the grid that has not started: its index, or "none is left", arrives in *slot.
 __device__ __forceinline__ void sp_ask_block(uint4 *slot, uint64_t *bar)
@@ -194,6 +196,15 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
     SpShared *sh = reinterpret_cast<SpShared *>(out_smem + 8 * kSpOutBytes);
 
     const unsigned int warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    // A tile holds `pack` query heads of `tile_rows` query rows each, the heads of a row side by side.
+    const unsigned int pack = scored_packed_heads(p), tile_rows = kSpM / pack, used = tile_rows * pack;
+    if (threadIdx.x < (unsigned int)kSpM)
+        sh->where[threadIdx.x] = threadIdx.x < used ? threadIdx.x / pack | (threadIdx.x % pack) << 16 : ~0u;
+    // rows of Q behind the used ones stay zero
+    for (unsigned int i = threadIdx.x; i < 2u * 2u * (kSpM - used) * 8u; i += kSpThreads)
+        *reinterpret_cast<uint4 *>(q_smem + i / ((kSpM - used) * 8u) * kSpHalfBytes + used * 128u + i % ((kSpM - used) * 8u) * 16u) =
+            make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async();
     if (threadIdx.x == 0) {
         mbar_init(&sh->next_full, 1);
         mbar_init(&sh->ask, 1);
@@ -253,16 +264,16 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 if (w == nullptr) break;
                 const int hull_first = w->hull_first, hull_end = w->hull_end, start = hull_first / kSpN;
                 const int stop = (hull_end + kSpN - 1) / kSpN;
-                const unsigned int b = w->b, kv_head = w->qhead / (p.query_heads / p.kv_heads);
+                const unsigned int b = w->b, kv_head = w->head / (p.query_heads / p.kv_heads);
                 if (lane == 0) {
                     if (stop > start) {
                         if (pieces) ok = mbar_wait(&sh->q_empty, (pieces - 1u) & 1u);
                         if (ok) {
-                            mbar_expect_tx(&sh->q_full, 2u * kSpTileBytes);
+                            mbar_expect_tx(&sh->q_full, 2u * 2u * used * 128u);
                             for (int x = 0; x < 2; ++x)
                                 for (int h = 0; h < 2; ++h)
                                     tma_load_4d(q_smem + x * kSpTileBytes + h * kSpHalfBytes, &maps.query, &sh->q_full, 64 * h,
-                                                (int)w->qhead, (int)(w->q0 + x * kSpM), (int)b);
+                                                (int)w->head, (int)(w->q0 + x * tile_rows), (int)b);
                         }
                     }
                     for (int j = stop - 1; ok && j >= start; --j) {
@@ -385,9 +396,9 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         } else {
             // ------------------------------ pieces of work ------------------------------------------
             // The block's own first, then those of blocks that have not started, as long as there are any.
-            const unsigned int pairs = (p.query_rows + 2 * kSpM - 1) / (2 * kSpM);
+            const unsigned int pairs = (p.query_rows + 2u * tile_rows - 1u) / (2u * tile_rows), lanes = p.query_heads / pack * p.sessions;
             const unsigned int per_group = pairs * lane_group;   // the grid holds it: below 2^31
-            const unsigned int per_split = (p.query_heads * p.sessions + lane_group - 1u) / lane_group * per_group;
+            const unsigned int per_split = (lanes + lane_group - 1u) / lane_group * per_group;
             unsigned int block = blockIdx.x, asked = 0u;
             bool ok = true, more = true;
             for (unsigned int turn = 0; ok && more; ++turn) {
@@ -399,7 +410,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     const unsigned int rest = SPLIT ? block % per_split : block;
                     within = rest % per_group;
                     work_lane = rest / per_group * lane_group + within % lane_group;
-                    return work_lane < p.query_heads * p.sessions;   // the last group may be short
+                    return work_lane < lanes;   // the last group may be short
                 };
                 bool look = turn > 0u || !given();
                 while (ok && look) {
@@ -416,8 +427,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 }
                 int tiles = 0;
                 if (more) {
-                    const unsigned int q0 = (pairs - 1u - within / lane_group) * 2u * kSpM;
-                    const unsigned int qhead = work_lane % p.query_heads, b = work_lane / p.query_heads;
+                    const unsigned int q0 = (pairs - 1u - within / lane_group) * 2u * tile_rows;
+                    const unsigned int head = work_lane % (p.query_heads / pack) * pack, b = work_lane / (p.query_heads / pack);
                     const unsigned int kv_tokens = admitted_kv_tokens(p.kv_tokens, b, p.kv_tokens_uniform, p.kv_tokens_max, p.status);
                     const long long query_start = scored_query_start(p, b, kv_tokens);
                     int hull_first, hull_end;
@@ -426,9 +437,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             int lo = 0x7fffffff, hi = 0;
-#pragma unroll
-                            for (int i = 0; i < kSpM / 32; ++i) {
-                                const unsigned int at = x * kSpM + 32u * i + lane;
+                            for (unsigned int at = x * tile_rows + lane; at < (x + 1) * tile_rows; at += 32u) {
                                 ScoredRange range = {0, 0, 0};
                                 if (q0 + at < p.query_rows) range = scored_range(p, b, q0 + at, kv_tokens, query_start);
                                 if (SPLIT) {
@@ -455,7 +464,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     }
                     if (hull_end == 0) hull_first = 0;
                     if (lane == 0)
-                        w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->qhead = qhead, w->b = b, w->split = split,
+                        w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->head = head, w->b = b, w->split = split,
                         w->query_start = query_start;
                     tiles = (hull_end + kSpN - 1) / kSpN - hull_first / kSpN;
                 }
@@ -489,13 +498,19 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         for (unsigned int turn = 0; ok; ++turn) {
         const SpWork *const w = take(turn);
         if (w == nullptr) break;
-        const unsigned int w_q0 = w->q0, my_row = w_q0 + threadIdx.x, qhead = w->qhead, b = w->b, split = w->split;
-        const bool exists = my_row < p.query_rows;
-        const ScoredRange range = {w->first[threadIdx.x], w->end[threadIdx.x], w->query_start + (long long)my_row};
+        ScoredRange range;
+        bool exists;
+        float slope2 = 0.0f;
+        {
+            const unsigned int place = sh->where[tile_row], at = place == ~0u ? 0u : place & 0xffffu;
+            const unsigned int row = w->q0 + x * tile_rows + at;
+            exists = place != ~0u && row < p.query_rows;
+            range = {exists ? w->first[x * tile_rows + at] : 0, exists ? w->end[x * tile_rows + at] : 0,
+                     w->query_start + (long long)row};
+            if (BIAS) slope2 = p.slopes[w->head + (exists ? place >> 16 : 0u)] * kScoredLog2e;
+        }
         const int hull_first = w->hull_first, hull_end = w->hull_end, my_from = w->from[x], my_until = w->until[x];
         const int stop = (hull_end + kSpN - 1) / kSpN, start = hull_first / kSpN;
-        give_back(turn);
-        const float slope2 = BIAS ? p.slopes[qhead] * kScoredLog2e : 0.0f;
         const float slope_held = BIAS ? (CAP ? slope2 : slope2 / mul) : 0.0f;
         float m = -INFINITY, l = 0.0f;
         for (int j = my_until - 1; j >= my_from; --j) {
@@ -723,14 +738,18 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             // time go through shared memory, their four 16-byte pieces in an order that spreads them over the banks.
             unsigned char *const out = out_smem + warp * kSpOutBytes;
             const bool narrow = !SPLIT && p.output_dtype == YVEX_DTYPE_BF16, sees = range.first < range.end;
+            const unsigned int q0 = w->q0 + x * tile_rows, head = w->head, b = w->b, split = w->split;
             const unsigned int out_lane = lane >> 2, width = narrow ? 2u : 4u;
-            const unsigned int out_row = w_q0 + x * kSpM + (warp & 3u) * 32u + out_lane;
-            const unsigned long long out_item = ((unsigned long long)b * p.query_rows + out_row) * p.query_heads + qhead;
-            unsigned char *const dst = 16u * (lane & 3u) +
-                (SPLIT ? reinterpret_cast<unsigned char *>(scored_partial(p, out_item, split))
-                         : reinterpret_cast<unsigned char *>(p.output) + out_item * kSpD * width);
-            const unsigned long long eight_rows =
-                8ull * p.query_heads * (SPLIT ? p.max_splits * (kSpD + 4ull) * sizeof(float) : (unsigned long long)kSpD * width);
+            const unsigned long long item0 = ((unsigned long long)b * p.query_rows + q0) * p.query_heads + head;
+            unsigned char *dst[4];   // of the rows that this thread stores, null where there is none
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned int place = sh->where[(warp & 3u) * 32u + 8u * i + out_lane];
+                const unsigned long long item = item0 + (unsigned long long)(place & 0xffffu) * p.query_heads + (place >> 16);
+                dst[i] = place == ~0u || q0 + (place & 0xffffu) >= p.query_rows ? nullptr
+                         : 16u * (lane & 3u) + (SPLIT ? reinterpret_cast<unsigned char *>(scored_partial(p, item, split))
+                                                      : reinterpret_cast<unsigned char *>(p.output) + item * kSpD * width);
+            }
             float check = l * 0.0f;   // NaN once a lane is not finite
             uint4 staged[4];
             auto send = [&](int chunk) {
@@ -741,7 +760,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 for (int i = 0; i < 4; ++i) {
                     const unsigned int r = 8u * i + out_lane;
                     const uint4 piece = *reinterpret_cast<const uint4 *>(out + r * 64u + 16u * ((lane & 3u) ^ ((r >> 1) & 3u)));
-                    if (out_row + 8u * i < p.query_rows) *reinterpret_cast<uint4 *>(dst + i * eight_rows + 64 * chunk) = piece;
+                    if (dst[i]) *reinterpret_cast<uint4 *>(dst[i] + 64 * chunk) = piece;
                 }
                 __syncwarp();
             };
@@ -776,15 +795,17 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             }
             bool finite = check == 0.0f;
             if (exists) {
-                float *part = SPLIT ? scored_partial(p, ((unsigned long long)b * p.query_rows + my_row) * p.query_heads + qhead, split)
-                                      : nullptr;
+                const unsigned int mine = sh->where[tile_row], my_head = head + (mine >> 16), my_row = q0 + (mine & 0xffffu);
+                const unsigned long long item = ((unsigned long long)b * p.query_rows + my_row) * p.query_heads + my_head;
+                float *part = SPLIT ? scored_partial(p, item, split) : nullptr;
                 if (SPLIT) part[kSpD] = fixed ? 0.0f : m, part[kSpD + 1] = l;
                 if (!finite) {
-                    if (p.row_first || p.row_end) finite = sp_row_again(p, b, qhead, range, my_row, part);
+                    if (p.row_first || p.row_end) finite = sp_row_again(p, b, my_head, range, my_row, part);
                     if (!finite) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
                 }
             }
         }
+        give_back(turn);
         }
     }
     tc_fence_before_sync();
@@ -794,7 +815,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
 
 bool scored_encode_rows(CUtensorMap *map, const void *base, int element_bytes, unsigned long long token_stride,
                         unsigned long long head_stride, unsigned long long outer_stride, unsigned long long tokens,
-                        unsigned long long heads, unsigned long long outer, bool head_inner, unsigned int box_tokens);
+                        unsigned long long heads, unsigned long long outer, bool head_inner, unsigned int box_tokens,
+                        unsigned int box_heads);
 
 // 1: launched, 0: not this kernel's shape, negative: an error.
 int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
@@ -805,23 +827,24 @@ int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
         (p.block_table && p.block_tokens % 64u) || head_stride > p.query_row_stride)
         return 0;
     const bool head_inner = p.key_head_stride < p.key_token_stride;
+    const unsigned int pack = scored_packed_heads(p), pair_rows = 2u * (kSpM / pack);
     if ((p.value_head_stride < p.value_token_stride) != head_inner) return 0;
     const unsigned long long tokens = p.block_table ? p.block_tokens : p.kv_tokens_max;
     const unsigned long long outer = p.block_table ? p.pool_blocks : p.sessions;
     SpMaps maps;
     if (!scored_encode_rows(&maps.query, p.query, 2, p.query_row_stride, head_stride, p.query_session_stride, p.query_rows,
-                            p.query_heads, p.sessions, true, kSpM) ||
+                            p.query_heads, p.sessions, true, kSpM / pack, pack) ||
         !scored_encode_rows(&maps.key, p.key, 2, p.key_token_stride, p.key_head_stride, p.key_outer_stride, tokens,
-                            p.kv_heads, outer, head_inner, 64u) ||
+                            p.kv_heads, outer, head_inner, 64u, 1u) ||
         !scored_encode_rows(&maps.value, p.value, 2, p.value_token_stride, p.value_head_stride, p.value_outer_stride,
-                            tokens, p.kv_heads, outer, head_inner, 64u))
+                            tokens, p.kv_heads, outer, head_inner, 64u, 1u))
         return 0;
     // lanes whose K + V fit half of the 126 MB L2 together form a group
-    const unsigned long long lanes = (unsigned long long)p.query_heads * p.sessions, group = p.query_heads / p.kv_heads;
+    const unsigned long long lanes = (unsigned long long)(p.query_heads / pack) * p.sessions, group = p.query_heads / p.kv_heads / pack;
     unsigned long long streams = (64ull << 20) / ((unsigned long long)p.kv_tokens_max * kSpD * 4ull);
     if (streams < 1ull) streams = 1ull;
     const unsigned long long lane_group = streams * group < lanes ? streams * group : lanes;
-    const unsigned long long pairs = (p.query_rows + 2ull * kSpM - 1ull) / (2ull * kSpM);
+    const unsigned long long pairs = (p.query_rows + pair_rows - 1ull) / pair_rows;
     const unsigned long long ctas = (lanes + lane_group - 1ull) / lane_group * lane_group * pairs * p.max_splits;
     if (lanes > 0xffffffffull || ctas > 0x7fffffffull) return 0;
     const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
