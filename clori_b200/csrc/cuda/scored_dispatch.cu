@@ -43,8 +43,16 @@ static unsigned long long scored_span(const yvx_scored_problem *p)
     return seen < all ? (seen + 63ull) / 64ull * 64ull : all;
 }
 
-// Calls of more than 64 vectors (query rows x heads of a KV head) on the shapes of the tensor cores. Decided by the
-// shape, types and alignment alone, before the plan.
+// Caches that the tensor-core kernel does not read in place: codes, and pages that are no multiple of 64 tokens.
+static bool scored_needs_stage(const yvx_scored_problem *p)
+{
+    return p->kv_code != YVX_KV_PLAIN || (p->block_table && p->block_tokens % 64u);
+}
+
+// Calls of more than 32 vectors (query rows x heads of a KV head) on the shapes of the tensor cores, of more than 64
+// where the cache has to be staged first. One session of 131072 tokens, 8 KV heads, groups of 4, the decode kernel
+// against this one: 8 rows 103 / 101 us, 12 rows 153 / 101, 16 rows 177 / 102; with e4m3 codes 16 rows 182 / 253,
+// 32 rows about 360 / 256. Decided by the shape, types and alignment alone, before the plan.
 static bool scored_prompt_shape(const yvx_scored_problem *p)
 {
     const unsigned long long bytes = p->kv_code == YVX_KV_PLAIN ? 2ull : 1ull;
@@ -53,7 +61,7 @@ static bool scored_prompt_shape(const yvx_scored_problem *p)
     const unsigned long long q_strides = p->query_row_stride | p->query_session_stride | p->query_head_stride;
     return !p->force_general && p->head_dim == 128u && p->query_dtype == YVEX_DTYPE_BF16 &&
            (p->kv_code != YVX_KV_PLAIN || p->kv_dtype == YVEX_DTYPE_BF16) &&
-           (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) > 64ull &&
+           (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) > (scored_needs_stage(p) ? 64ull : 32ull) &&
            !((reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value) |
               reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->output) | strides * bytes | q_strides * 2ull) & 15ull);
 }
@@ -66,12 +74,6 @@ static unsigned long long scored_partial_bytes(const yvx_scored_problem *p)
     return (items * p->max_splits * (p->head_dim + 4ull) * 4ull + 255ull) / 256ull * 256ull;
 }
 
-// Caches that the tensor-core kernel does not read in place: codes, and pages that are no multiple of 64 tokens.
-static bool scored_needs_stage(const yvx_scored_problem *p)
-{
-    return p->kv_code != YVX_KV_PLAIN || (p->block_table && p->block_tokens % 64u);
-}
-
 }  // namespace yvx
 
 extern "C" {
@@ -81,10 +83,10 @@ extern "C" {
 // partial rows); the chunk with the smallest sum is taken, at most 8192 tokens. One session of 4096 tokens:
 // 128 tokens 10.3 us, 64 tokens 15.4, 512 tokens 13.0; 64 sessions behind a window of 4096: one chunk 177 us,
 // two 193, four 190; one session of 131072 tokens: 3584 (one wave) 95 us, 1792 107, 4096 105.
-// Prompt-sized calls are split only to fill the machine: one CTA on an SM, a piece of work is 256 rows of a head, a
-// split costs its tiles of 128 tokens and about five more, the fold two tiles and its traffic. 32 heads over 131072
-// tokens, 20 rows: one split 1330 us, four 346, five 538, nine (taken) 313; 256 rows: 1655, 493, 813, 476;
-// 300 rows over 32768: one 422, two (taken) 260, three 305; 2048 rows over 16384: one (taken) 437, two 690.
+// Prompt-sized calls are split only to fill the machine: one CTA on an SM, a piece of work is two row tiles, a split
+// costs its tiles of 128 tokens and about five more, the fold two tiles and its traffic. 32 heads in groups of 4 over
+// 131072 tokens, 20 rows: one split 1307 us, four 348, sixteen 108, eighteen (taken) 102, twenty-four 143; 256 rows:
+// 1565, four 490, nine (taken) 479, sixteen 582; 2048 rows over 16384: one (taken) 440, two 679.
 void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
 {
     if (!p || !p->kv_heads || !p->query_rows || !p->kv_tokens_max) return;

@@ -42,7 +42,7 @@ DECODE = [
     (LENGTHS, 1, 8, 2, dict(page=64)),
     (LENGTHS, 1, 5, 1, dict(page=128, cap=30.0, q_scale=6.0)),
     (LENGTHS, 3, 8, 2, dict(out_dtype=BF16, slopes=True)),
-    ([500, 333], 8, 16, 2, dict(head_major=True, window=100)),
+    ([500, 333], 4, 16, 2, dict(head_major=True, window=100)),
     ([500, 333], 2, 16, 1, dict(causal=False, slopes=True, cap=5.0, pad=8)),
     (LENGTHS, 1, 8, 2, dict(cache=E4M3, page=64)),
     (LENGTHS, 4, 4, 1, dict(cache=E4M3, page=16, cap=50.0, q_scale=8.0)),
@@ -61,6 +61,7 @@ def test_decode_kernel(backend, lengths, rows, heads, kv_heads, fields, chunk):
     Case(12, lengths, rows, heads, kv_heads, 128, **fields).check(backend, path, chunk=chunk)
 
 
+LOUDNESS = np.repeat(np.float32([0.02, 8.0, 1.0, 40.0, 0.1]), 128)[None, :, None, None]   # of keys, tile by tile
 DOCS = [[100, 1, 130, 300, 0, 69]]
 PROMPT = [
     # lengths, rows, heads, kv_heads, fields
@@ -82,17 +83,31 @@ PROMPT = [
     ([390, 261], 200, 4, 2, dict(cache=I8, page=16, window=90, cap=9.0, q_scale=4.0)),
     ([200, 210], 130, 2, 1, dict(page=16)),
     ([0, 300], 257, 2, 1, {}),
+    # groups that fill a row tile, that leave rows of it unused, and one that no tile holds
+    ([500, 333], 8, 16, 2, dict(head_major=True, window=100)),
+    ([700, 0, 129], 11, 6, 2, dict(page=64, slopes=True)),
+    ([260, 300], 60, 10, 2, dict(cap=30.0, q_scale=3.0, out_dtype=BF16)),
+    ([300, 260], 33, 14, 2, dict(ranges="prefix", slopes=True, cap=4.0)),
+    ([200, 130], 10, 65, 1, dict(causal=False)),
+    ([200, 130], 2, 129, 1, dict(slopes=True)),
+    ([1000, 900], 9, 16, 2, dict(cache=E4M3, page=64, cap=30.0, q_scale=6.0)),
+    # caps: every form of tanh in turn, logits far below zero everywhere, caps beyond the fixed reference
+    ([640], 200, 2, 1, dict(cap=20.0, k_scale=LOUDNESS)),
+    ([400, 390], 130, 2, 1, dict(cap=54.0, q_scale=60.0)),
+    ([400, 390], 130, 2, 1, dict(cap=300.0, q_scale=60.0)),
+    ([400, 390], 130, 2, 1, dict(cap=300.0, q_scale=60.0, slopes=True)),
 ]
 
 
 @pytest.mark.parametrize("lengths,rows,heads,kv_heads,fields", PROMPT)
-def test_prompt_kernel(backend, lengths, rows, heads, kv_heads, fields):
+@pytest.mark.parametrize("chunk", [None, 128, 384])
+def test_prompt_kernel(backend, lengths, rows, heads, kv_heads, fields, chunk):
     fields = dict(fields)
     if fields.get("ranges") == "documents":
         fields["ranges"] = documents(DOCS, rows)
     elif fields.get("ranges") == "prefix":
-        fields["ranges"] = documents([[rows]], rows, [250])
-    Case(14, lengths, rows, heads, kv_heads, 128, **fields).check(backend, "prompt")
+        fields["ranges"] = documents([[rows]] * len(lengths), rows, [min(250, rows // 2)])
+    Case(14, lengths, rows, heads, kv_heads, 128, **fields).check(backend, "prompt", chunk=chunk)
 
 
 def test_prompt_rows_with_gaps_and_padding(backend):
@@ -100,8 +115,9 @@ def test_prompt_rows_with_gaps_and_padding(backend):
     first, end = np.zeros((1, 400), int), np.zeros((1, 400), int)
     for lo, hi in ((0, 90), (100, 101), (140, 330), (350, 390)):
         first[0, lo:hi], end[0, lo:hi] = lo, np.arange(lo, hi) + 1
-    Case(15, [400], 400, 2, 1, 128, ranges=(first, end)).check(backend, "prompt")
-    Case(15, [400], 400, 2, 1, 128, ranges=(first, end), cache=E4M3, page=64, slopes=True).check(backend, "prompt")
+    for chunk in (None, 128, 256):
+        Case(15, [400], 400, 2, 1, 128, ranges=(first, end)).check(backend, "prompt", chunk=chunk)
+        Case(15, [400], 400, 2, 1, 128, ranges=(first, end), cache=E4M3, page=64, slopes=True).check(backend, "prompt", chunk=chunk)
 
 
 def test_pages_in_front_of_a_window_may_be_gone(backend):
