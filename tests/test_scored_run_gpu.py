@@ -264,3 +264,59 @@ def test_an_asynchronous_backend_reports_at_the_next_synchronisation(backend):
     backend.sync()
     backend.bind_stream(None)
     assert backend.lib.yvx_cuda_stream_destroy(stream) == 0
+
+
+@pytest.mark.parametrize("code", [E4M3, I8])
+def test_pages_that_lie_beyond_32_bits(backend, code):
+    # five pages 2^30 bytes apart give, bit for bit, what they give side by side
+    rng = np.random.default_rng(44)
+    lib, n, table = backend.lib, 250, np.array([[4, 0, 3, 1]], np.int32)
+    new = [backend.tensor(x, clori_b200.f32_to_bf16_bits(bf16(rng.standard_normal((n, KV_HEADS * HD))))) for x in "ab"]
+    status = backend.tensor("status", np.zeros(1, np.int32))
+    tables = [backend.tensor("t", t) for t in (table, np.array([[2, 0, 3, 1]], np.int32))]
+    outputs = []
+    for stride in (2 * KV_HEADS * 64 * HD, 2 ** 30):
+        pool = backend.alloc("pool", abi.DTYPE_I8, (4 * stride + 2 * KV_HEADS * 64 * HD,))
+        scales = [backend.tensor(x, np.zeros((5, KV_HEADS), np.float32)) for x in "ks"]
+        a = abi.Kv8AppendArgs()
+        a.sessions, a.tokens, a.kv_heads, a.head_dim, a.code, a.dtype = 1, n, KV_HEADS, HD, code, BF16
+        a.key, a.value, a.token_stride, a.session_stride = new[0].data_ptr, new[1].data_ptr, KV_HEADS * HD, n * KV_HEADS * HD
+        a.block_table, a.block_tokens, a.block_table_stride, a.pool_blocks = tables[0].data_ptr, 64, 4, 5
+        a.key_codes, a.value_codes = pool.data_ptr, pool.data_ptr + KV_HEADS * 64 * HD
+        a.code_token_stride, a.code_head_stride, a.code_block_stride = HD, 64 * HD, stride
+        a.key_scales, a.value_scales, a.status = scales[0].data_ptr, scales[1].data_ptr, status.data_ptr
+        assert lib.yvx_cuda_kv8_append(C.byref(a), backend.stream) == 0, lib.yvx_cuda_last_error_text()
+
+        def attend(rows, general, pages):
+            q = backend.tensor("q", clori_b200.f32_to_bf16_bits(bf16(np.random.default_rng(rows).standard_normal((rows, HEADS * HD)))))
+            out = backend.tensor("o", np.full((rows, HEADS * HD), np.nan, np.float32))
+            p = abi.ScoredProblem()
+            p.sessions, p.query_rows, p.query_heads, p.kv_heads, p.head_dim, p.causal = 1, rows, HEADS, KV_HEADS, HD, 1
+            p.scale, p.query_dtype, p.kv_dtype, p.output_dtype, p.kv_code = 0.1, BF16, abi.DTYPE_I8, F32, code
+            p.query, p.query_row_stride, p.query_session_stride = q.data_ptr, HEADS * HD, rows * HEADS * HD
+            p.output, p.key, p.value, p.status = out.data_ptr, a.key_codes, a.value_codes, status.data_ptr
+            p.key_token_stride = p.value_token_stride = HD
+            p.key_head_stride = p.value_head_stride = 64 * HD
+            p.key_outer_stride = p.value_outer_stride = stride
+            p.key_scales, p.value_scales = a.key_scales, a.value_scales
+            p.block_table, p.block_tokens, p.block_table_stride, p.pool_blocks = pages.data_ptr, 64, 4, 5
+            p.kv_tokens_uniform, p.kv_tokens_max, p.query_start_from_end, p.force_general = n, n, 1, general
+            lib.yvx_cuda_scored_plan(C.byref(p), backend.sm_count)
+            work = backend.alloc("work", abi.DTYPE_I8, (max(256, lib.yvx_cuda_scored_workspace_bytes(C.byref(p))),))
+            p.workspace, p.workspace_bytes = work.data_ptr, work.nbytes
+            assert lib.yvx_cuda_scored_attention(C.byref(p), backend.stream, None) == 0, lib.yvx_cuda_last_error_text()
+            assert lib.yvx_cuda_stream_synchronize(backend.stream) == 0 and int(status.read()[0]) == 0
+            return out.read()
+
+        calls = [(1, 0), (1, 1), (40, 0), (40, 1)]
+        got = [attend(*x, tables[0]) for x in calls]
+        pools = (abi.KvPagePool * 3)(abi.KvPagePool(pool.data_ptr, stride, 64 * HD, HD, 0, 5, 2 * KV_HEADS),
+                                     *[abi.KvPagePool(s.data_ptr, KV_HEADS * 4, 0, 0, KV_HEADS * 4, 5, 1) for s in scales])
+        copies = (abi.KvCopy * 1)(abi.KvCopy(1, 4, 2, 64))
+        c = abi.KvPagesArgs()
+        c.pools, c.pool_count, c.copies, c.copy_count, c.block_tokens = pools, 3, copies, 1, 64
+        assert lib.yvx_cuda_kv_pages_copy(C.byref(c), backend.stream, None) == 0, lib.yvx_cuda_last_error_text()
+        for x, w in zip(calls, got):
+            assert np.array_equal(attend(*x, tables[1]), w)
+        outputs.append(got)
+    assert all(np.isfinite(x).all() and np.array_equal(x, y) for x, y in zip(*outputs))
