@@ -176,8 +176,9 @@ int yvx_cuda_gqa_attention_profiled(const yvx_gqa_problem *problem, void *stream
  * any other mask whose rows see one run of tokens are such arrays
  * (yvex_b200_attention_row_ranges writes the usual ones). A row that sees nothing is written
  * as zeros, and what lies in K and V where no row looks (beyond a session's length, in the
- * rest of a page, in padding) may be anything, NaN included. A NaN or infinity that a row
- * does see is reported in the status word (1).
+ * rest of a page, in padding) may be anything, NaN included. A NaN that a row does see is
+ * reported in the status word (1), and so is an infinity or a score beyond 1e29 unless the cap
+ * or a weight of zero takes it away.
  *
  * kv_code != YVX_KV_PLAIN: key and value are 8-bit codes in pages (block_table is required;
  * strides are in bytes) and a lane stands for code * scale, with one float scale for each
@@ -185,9 +186,10 @@ int yvx_cuda_gqa_attention_profiled(const yvx_gqa_problem *problem, void *stream
  * fraction bits, largest 448) or signed 8-bit integers.
  *
  * Everything is accumulated in F32. On the matrix units (head_dim 128 and bf16 queries) the
- * weights of the softmax are rounded once to 11 bits (codes), 16 bits (bf16 decode) or 8 bits
- * (prompt-sized calls), like their operands; other shapes run in F32 throughout. Results
- * repeat bit for bit. Offsets are 64 bits wide; lengths are below 2^31 - 1024. */
+ * weights of the softmax are rounded once: to 8 bits, like their operands, in calls of more than
+ * 32 vectors (query rows x heads of a KV head; 64 over codes or pages that are no multiple of 64
+ * tokens), else to 16 bits (bf16) or 11 bits (codes); other shapes run in F32 throughout.
+ * Results repeat bit for bit. Offsets are 64 bits wide; lengths are below 2^31 - 1024. */
 typedef enum { YVX_KV_PLAIN = 0, YVX_KV_E4M3 = 1, YVX_KV_I8 = 2 } yvx_kv_code;
 typedef struct yvx_scored_problem {
     unsigned int sessions, query_rows;        /* rows per session (uniform) */

@@ -153,6 +153,16 @@ def test_one_loud_token_does_not_hide_many_quiet_ones(backend):
         c.check(backend, path)
 
 
+@pytest.mark.parametrize("sessions,rows,heads,kv_heads,hd,fields", [
+    (256, 1, 8, 2, 128, dict(page=16)), (300, 1, 7, 7, 33, dict(kv_dtype=F32)), (40, 13, 4, 2, 128, dict(out_dtype=BF16)),
+])
+def test_many_items_of_few_splits(backend, sessions, rows, heads, kv_heads, hd, fields):
+    lengths = [(37 * i) % 200 for i in range(sessions)]
+    for chunk, general in ((64, False), (64, True)):
+        path = "general" if general or hd != 128 else "decode_bf16"
+        Case(31, lengths, rows, heads, kv_heads, hd, **fields).check(backend, path, force_general=general, chunk=chunk)
+
+
 def test_rows_in_front_of_the_session_and_empty_sessions_are_zero(backend):
     c = Case(5, [2, 0, 7], 4, 4, 2, 128)
     p = c.plan(backend, c.problem(backend))
