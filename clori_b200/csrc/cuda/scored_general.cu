@@ -5,7 +5,8 @@
 // used 16 times, and walks its split in tiles of 32 tokens: K and V are decoded into shared
 // memory as floats, a thread computes the scores of one token against four vectors, a warp runs
 // the softmax of four vectors, a thread accumulates one or two head dimensions of all 16. Bound
-// by the FMA pipe and shared-memory reads. It is the kernel of the F32 contract, of head
+// by the FMA pipe and shared-memory reads: 64 sessions of 512 to 32768 tokens of e4m3 codes 8.3 ms (22 times the decode
+// kernel), 4 x 1531 rows 10.4 ms (61 times the prompt kernel). It is the kernel of the F32 contract, of head
 // dimensions other than 128 and of layouts that the tiled copies cannot describe.
 #include "scored.cuh"
 

@@ -2,23 +2,33 @@
 // head_dim 128, contiguous rows or pages of 64 n tokens, any rule and any visible runs.
 //
 // A CTA owns two tiles (A, B) of 128 rows, a row being a (query row, head of the KV head's group) pair: a tile of
-// a group of 4 is 32 query rows, which see fewer tokens in vain than 128 do, and few rows fill it. While one tile is in its softmax the
-// other is in its matrix products. Warp 8 brings K and V in tiles of 128 tokens (tiled copies,
-// 128-byte swizzle, two stages each), warp 9 issues S = Q K^T (both operands in shared memory) and
-// O += P V (P in tensor memory, where it overwrites its scores), warps 0-3 and 4-7 run the softmax
-// of A and B, a thread per row; warps 10 and 11 only complete the warpgroup that gives its registers
-// to the softmax (224 and 56 a thread of the 168 at launch). A tile walks only the token tiles that some row of it sees,
-// the last one first: with a bias against distance, and often without, the largest weights come early.
+// a group of 4 is 32 query rows, which see fewer tokens in vain than 128 do, and few rows fill it (17 rows of 32
+// heads over 131072 tokens: 306 us with a head for each tile, 102 so). While one tile is in its softmax the other is
+// in its matrix products. Warp 8 brings K and V in tiles of 128 tokens (tiled copies, 128-byte swizzle, two stages
+// each), warp 9 issues S = Q K^T (both operands in shared memory) into one score buffer that is free again as soon
+// as it is read, warp 10 O += P V (P in tensor memory), warps 0-3 and 4-7 run the softmax of A and B, a thread per
+// row, and warp 11 fetches the CTA's next piece of work: the grid has a block for every piece, and a block that
+// is done takes the work of one that has not started (cluster launch control), so loads and first products of a
+// piece run beside the last tiles of the one before (4 x 1531 rows with a prefix: 260 us -> 242). Registers: 224 a
+// thread for the softmax and 56 for the others, of the 168 at launch. A tile walks only the token tiles that some
+// row of it sees, the last one first: with a bias against distance, and often without, the largest weights come
+// early. With few pieces of work the KV sequence is split and folded.
 //
-// A thread takes its row's 128 products out of tensor memory twice: once for the maximum, then 64 at a time
-// for the weights, which go back over products that have been read; P V of the first half starts while the
-// second is exponentiated. The score rule runs two lanes at a time (f32x2 instructions):
+// A thread takes its row's 128 products into registers, and P V of the first 64 starts while the others are
+// exponentiated. The score rule runs two lanes at a time (f32x2 instructions):
 //   cap    tanh(x) = x p(x^2) with p of degree 3 while every |x| of the warp's tile is at most 5/8, of degree 6 up to
-//          11/8, beyond 1 - 2 / (e^2x + 1) from the exponential unit, which is as loaded as the tensor cores. A cap bounds the
-//          logits: up to 55 the weights stay in range against the reference 0 and no maximum is looked for.
+//          11/8, beyond 1 - 2 / (e^2x + 1) from the exponential unit, which is as loaded as the tensor cores. A cap
+//          bounds the logits: up to 55 the weights stay in range against the reference 0 and no maximum is looked for.
 //   bias   slope * (s - position) is linear in the token inside a tile: one multiply-add per score and one
 //          constant per row and tile; tokens behind the row's position (prefixes) take |.| in full.
-// Weights are rounded to bf16, sums and the accumulator are F32.
+// Weights are rounded to bf16 (the tensor cores' operand; half a step, 2^-9), sums and the accumulator are F32.
+//
+// Measured, 37 heads x 1024 rows x 4096 tokens, nothing masked: 75 us (1.06 PFLOP/s), with a cap of 50 84 to 92, with
+// a bias 97. Two prompts of 8192 capped rows 1.25 ms, 1531-row prompts with a prefix and a cap 170 us (4 of 40 heads),
+// 16384 rows of packed documents with a bias 484 us (32 heads). A pair of tiles takes about 3300 cycles (no cap), of
+// which the products need 2048 and the exponential unit 2048; the rest is the softmax's other instructions and the
+// way between the two. A piece of work costs about 10000 cycles besides its tiles: its first and last tile have no
+// partner and run masks, rows leave, all of it code that the instruction cache has lost since the last piece.
 #include <type_traits>
 
 #include "scored.cuh"
