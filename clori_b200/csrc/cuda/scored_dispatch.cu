@@ -15,7 +15,8 @@ static int scored_check(const yvx_scored_problem *p)
         return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: query, output, key, value and status are required");
     if (!p->sessions || !p->query_rows || !p->query_heads || !p->kv_heads || !p->head_dim ||
         p->query_heads % p->kv_heads || !p->kv_tokens_max || (!p->kv_tokens && p->kv_tokens_uniform > p->kv_tokens_max) ||
-        !(p->scale > 0.0f) || !isfinite(p->scale) || !(p->cap >= 0.0f) || !isfinite(p->cap))
+        !(p->scale > 0.0f) || !isfinite(p->scale) || !(p->cap >= 0.0f) || !isfinite(p->cap) ||
+        (p->cap > 0.0f && (p->cap < 1e-30f || !isfinite(4.0f * p->scale / p->cap))))
         return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: inconsistent geometry, scale or cap");
     if (p->head_dim > 256u || (p->query_dtype != YVEX_DTYPE_F32 && p->query_dtype != YVEX_DTYPE_BF16) ||
         (p->output_dtype != YVEX_DTYPE_F32 && p->output_dtype != YVEX_DTYPE_BF16) || p->kv_code < YVX_KV_PLAIN ||
@@ -62,6 +63,7 @@ static bool scored_prompt_shape(const yvx_scored_problem *p)
     return !p->force_general && p->head_dim == 128u && p->query_dtype == YVEX_DTYPE_BF16 &&
            (p->kv_code != YVX_KV_PLAIN || p->kv_dtype == YVEX_DTYPE_BF16) &&
            (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) > (scored_needs_stage(p) ? 64ull : 32ull) &&
+           !(p->slopes && p->scale < 1e-12f) &&   // that kernel holds the bias in units of the raw product
            !((reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value) |
               reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->output) | strides * bytes | q_strides * 2ull) & 15ull);
 }

@@ -177,8 +177,8 @@ int yvx_cuda_gqa_attention_profiled(const yvx_gqa_problem *problem, void *stream
  * (yvex_b200_attention_row_ranges writes the usual ones). A row that sees nothing is written
  * as zeros, and what lies in K and V where no row looks (beyond a session's length, in the
  * rest of a page, in padding) may be anything, NaN included. A NaN that a row does see is
- * reported in the status word (1), and so is an infinity or a score beyond 1e29 unless the cap
- * or a weight of zero takes it away.
+ * reported in the status word (1), and so is an infinity or a product Q . K beyond 1e29 unless
+ * the cap or a weight of zero takes it away.
  *
  * kv_code != YVX_KV_PLAIN: key and value are 8-bit codes in pages (block_table is required;
  * strides are in bytes) and a lane stands for code * scale, with one float scale for each
@@ -189,13 +189,14 @@ int yvx_cuda_gqa_attention_profiled(const yvx_gqa_problem *problem, void *stream
  * weights of the softmax are rounded once: to 8 bits, like their operands, in calls of more than
  * 32 vectors (query rows x heads of a KV head; 64 over codes or pages that are no multiple of 64
  * tokens), else to 16 bits (bf16) or 11 bits (codes); other shapes run in F32 throughout.
- * Results repeat bit for bit. Offsets are 64 bits wide; lengths are below 2^31 - 1024. */
+ * Results repeat bit for bit. Offsets are 64 bits wide; lengths are below 2^31 - 1024, positions
+ * below 2^31. */
 typedef enum { YVX_KV_PLAIN = 0, YVX_KV_E4M3 = 1, YVX_KV_I8 = 2 } yvx_kv_code;
 typedef struct yvx_scored_problem {
     unsigned int sessions, query_rows;        /* rows per session (uniform) */
     unsigned int query_heads, kv_heads, head_dim; /* head_dim at most 256 */
     unsigned int causal;
-    float scale, cap;                         /* scale > 0; cap 0: none */
+    float scale, cap;                         /* scale > 0; cap 0: none, else at least 1e-30 */
     unsigned int window;                      /* 0: none */
     int query_dtype, kv_dtype, output_dtype;  /* F32 or BF16; kv_dtype is ignored for codes */
     int kv_code;                              /* yvx_kv_code */

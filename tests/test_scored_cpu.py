@@ -54,6 +54,7 @@ def scored_problem(**changes):
     (dict(query_heads=7), abi.YVEX_ERR_INVALID_ARG), (dict(query_rows=0), abi.YVEX_ERR_INVALID_ARG),
     (dict(scale=0.0), abi.YVEX_ERR_INVALID_ARG), (dict(scale=float("inf")), abi.YVEX_ERR_INVALID_ARG),
     (dict(cap=-1.0), abi.YVEX_ERR_INVALID_ARG), (dict(cap=float("nan")), abi.YVEX_ERR_INVALID_ARG),
+    (dict(cap=1e-31), abi.YVEX_ERR_INVALID_ARG), (dict(cap=1e-10, scale=1e30), abi.YVEX_ERR_INVALID_ARG),
     (dict(kv_tokens_max=0), abi.YVEX_ERR_INVALID_ARG), (dict(kv_tokens_uniform=101), abi.YVEX_ERR_INVALID_ARG),
     (dict(chunk_tokens=0), abi.YVEX_ERR_INVALID_ARG), (dict(chunk_tokens=100), abi.YVEX_ERR_INVALID_ARG),
     (dict(head_dim=257), abi.YVEX_ERR_UNSUPPORTED), (dict(query_dtype=abi.DTYPE_F16), abi.YVEX_ERR_UNSUPPORTED),

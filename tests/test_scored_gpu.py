@@ -5,7 +5,7 @@ import pytest
 
 import clori_b200
 from clori_b200 import abi
-from tests.scored_cases import Case, documents
+from tests.scored_cases import WEIGHTS, Case, attention, documents, tolerance
 
 pytestmark = pytest.mark.gpu
 E4M3, I8, PLAIN = abi.KV_E4M3, abi.KV_I8, abi.KV_PLAIN
@@ -161,6 +161,21 @@ def test_many_items_of_few_splits(backend, sessions, rows, heads, kv_heads, hd, 
     for chunk, general in ((64, False), (64, True)):
         path = "general" if general or hd != 128 else "decode_bf16"
         Case(31, lengths, rows, heads, kv_heads, hd, **fields).check(backend, path, force_general=general, chunk=chunk)
+
+
+@pytest.mark.parametrize("scale,cap", [(1e-14, 0.0), (1e-10, 0.0), (3e-5, 1e-4), (20.0, 60.0)])
+def test_extreme_scales_with_a_bias(backend, scale, cap):
+    c = Case(33, [300, 290], 70, 4, 2, 128, slopes=True, cap=cap, k_scale=min(1.0, 1e-2 / scale) if scale > 1 else 1.0)
+    p = c.problem(backend)
+    p.scale = scale
+    got, status = c.launch(backend, c.plan(backend, p))
+    assert status == 0
+    for b in range(2):
+        want, spread, size = attention(c.q[b].astype(np.float64), c.values["k"][b], c.values["v"][b], c.position[b], c.first[b],
+                                       c.end[b], float(np.float32(scale)), float(np.float32(cap)), c.slope.astype(np.float64))
+        visible = np.broadcast_to((c.end - c.first)[b][:, None].astype(np.float64), size.shape)
+        reach = np.abs(c.position[b])[:, None] * c.slope[None, :].astype(np.float64)
+        assert np.all(np.abs(got[b] - want) <= tolerance(want, spread, size, visible, 128, WEIGHTS["prompt"], 2.0 ** -24, cap, reach))
 
 
 def test_rows_in_front_of_the_session_and_empty_sessions_are_zero(backend):
