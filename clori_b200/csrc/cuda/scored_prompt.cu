@@ -23,8 +23,8 @@
 //          constant per row and tile; tokens behind the row's position (prefixes) take |.| in full.
 // Weights are rounded to bf16 (the tensor cores' operand; half a step, 2^-9), sums and the accumulator are F32.
 //
-// Measured, 37 heads x 1024 rows x 4096 tokens, nothing masked: 75 us (1.06 PFLOP/s), with a cap of 50 84 to 92, with
-// a bias 97. Two prompts of 8192 capped rows 1.25 ms, 1531-row prompts with a prefix and a cap 170 us (4 of 40 heads),
+// Measured, 37 heads x 1024 rows x 4096 tokens, nothing masked: 75 us (1.06 PFLOP/s), with a cap of 50 84, with
+// a bias 97. Two prompts of 8192 capped rows 1.25 ms, 1531-row prompts with a prefix and a cap 173 us (4 of 40 heads),
 // 16384 rows of packed documents with a bias 484 us (32 heads). A pair of tiles takes about 3300 cycles (no cap), of
 // which the products need 2048 and the exponential unit 2048; the rest is the softmax's other instructions and the
 // way between the two. A piece of work costs about 10000 cycles besides its tiles: its first and last tile have no
@@ -496,13 +496,15 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         const uint32_t p_col = lane_base + kSpPColumn + x * 64u, o_col = lane_base + kSpOColumn + x * kSpD;
         const unsigned int tile_row = threadIdx.x & 127u;
         // Raw products become exponents (log2 units): s * mul, or mul * tanh(s * to_unit) with
-        // tanh(x) = x (a0 + a1 x^2 + ..), the constants folded into the coefficients.
+        // tanh(x) = x (a0 + a1 x^2 + ..).
         const float mul = (CAP ? p.cap : p.scale) * kScoredLog2e;
         const float to_unit = CAP ? p.scale / p.cap : 0.0f;
         // Under a cap of at most 80 log2 units (55) every row's reference is 0: weights lie in 2^-80 .. 2^80, in range of
         // F32 and bf16, and no maximum is looked for.
-        const bool fixed = CAP && !BIAS && mul <= 80.0f;
-        const float inside_tiny = CAP ? 0.625f / to_unit : 0.0f, inside_small = CAP ? 1.375f / to_unit : 0.0f;
+        const bool fixed = CAP && !BIAS && mul <= 80.0f && mul >= 1e-20f;
+        const float inside_small = CAP ? 1.375f / to_unit : 0.0f, unit3 = to_unit * to_unit * to_unit;
+        const float last = mul * to_unit * unit3 * unit3;   // what the short polynomial's last coefficient is folded with
+        const float inside_tiny = CAP && last >= 1e-34f && last <= 1e30f ? 0.625f / to_unit : -1.0f;
         unsigned int tiles = 0u, count = 0u;   // so far: token tiles of the block, of this row tile
         bool ok = true;
         for (unsigned int turn = 0; ok; ++turn) {
@@ -618,17 +620,19 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 const float largest = fmaxf(top[0], top[1]);
                 small = __all_sync(0xffffffffu, largest <= inside_small);
                 // x p(x^2), the exponential, sum and rounding of both halves as one straight run of instructions (a branch
-                // between the halves costs the common tile 13 %)
-                auto weights = [&](const auto &a, auto masks) {
+                // between the halves costs the common tile 13 %). The short polynomial takes the products as they are,
+                // to_unit folded into its coefficients; the long one, whose coefficients would leave F32's range, x itself.
+                auto weights = [&](const auto &a) {
                     constexpr int kTerms = sizeof(a) / sizeof(a[0]);
-                    constexpr bool kMasks = decltype(masks)::value;
+                    constexpr bool kFolded = kTerms == 4;
                     unsigned long long poly2[kTerms];   // each coefficient twice
-                    float power = to_unit * mul;
+                    float power = mul * (kFolded ? to_unit : 1.0f);
 #pragma unroll
                     for (int i = 0; i < kTerms; ++i) {
                         poly2[i] = f2_pack(a[i] * power, a[i] * power);
-                        power *= to_unit * to_unit;
+                        if (kFolded) power *= to_unit * to_unit;
                     }
+                    const unsigned long long unit2 = f2_pack(to_unit, to_unit);
                     landed();
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -636,15 +640,18 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
 #pragma unroll
                         for (int i = 0; i < 64; i += 2) {
                             unsigned long long v = f2_load(s[2 * h + (i >> 5)], i & 31);
-                            if (kMasks || kTerms > 4) asm volatile("" : "+l"(v));   // or what several branches share is drawn in front of them
+                            if (!kFolded) {
+                                asm volatile("" : "+l"(v));   // or what both forms share is drawn in front of their branch
+                                v = f2_mul(v, unit2);
+                            }
                             const unsigned long long w2 = f2_mul(v, v);
                             unsigned long long r = poly2[kTerms - 1];
 #pragma unroll
                             for (int k = kTerms - 2; k >= 0; --k) r = f2_fma(r, w2, poly2[k]);
                             float e0, e1;
                             f2_unpack(f2_mul(v, r), e0, e1);
-                            e0 = exp2_approx(kMasks ? hide(e0, 64 * h + i) : e0);
-                            e1 = exp2_approx(kMasks ? hide(e1, 64 * h + i + 1) : e1);
+                            e0 = exp2_approx(e0);
+                            e1 = exp2_approx(e1);
                             sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(e0, e1));
                             packed[i >> 1] = pack_bf16(e0, e1);
                         }
@@ -652,8 +659,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     }
                 };
                 if (fixed && small && !cut[0] && !cut[1]) {
-                    if (__all_sync(0xffffffffu, largest <= inside_tiny)) weights(kSpTanhTiny, std::false_type{});
-                    else weights(kSpTanhSmall, std::false_type{});
+                    if (__all_sync(0xffffffffu, largest <= inside_tiny)) weights(kSpTanhTiny);
+                    else weights(kSpTanhSmall);
                     done = true;
                 }
             }
@@ -663,18 +670,13 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 if (CAP) {
                     const float to_exp = to_unit * (2.0f * kScoredLog2e);
                     if (small) {
-                        float power = to_unit * mul, a[7];
-#pragma unroll
-                        for (int i = 0; i < 7; ++i) {
-                            a[i] = kSpTanhSmall[i] * power;
-                            power *= to_unit * to_unit;
-                        }
+                        const unsigned long long unit2 = f2_pack(to_unit, to_unit);
 #pragma unroll
                         for (int i = 0; i < 128; i += 2) {
-                            const unsigned long long v = f2_load(s[i >> 5], i & 31), w2 = f2_mul(v, v);
-                            unsigned long long r = f2_pack(a[6], a[6]);
+                            const unsigned long long v = f2_mul(f2_load(s[i >> 5], i & 31), unit2), w2 = f2_mul(v, v);
+                            unsigned long long r = f2_pack(kSpTanhSmall[6] * mul, kSpTanhSmall[6] * mul);
 #pragma unroll
-                            for (int k = 5; k >= 0; --k) r = f2_fma(r, w2, f2_pack(a[k], a[k]));
+                            for (int k = 5; k >= 0; --k) r = f2_fma(r, w2, f2_pack(kSpTanhSmall[k] * mul, kSpTanhSmall[k] * mul));
                             f2_store(f2_mul(v, r), s[i >> 5], i & 31);
                         }
                     } else {

@@ -163,6 +163,17 @@ def test_many_items_of_few_splits(backend, sessions, rows, heads, kv_heads, hd, 
         Case(31, lengths, rows, heads, kv_heads, hd, **fields).check(backend, path, force_general=general, chunk=chunk)
 
 
+@pytest.mark.parametrize("cap,loud", [(300.0, 50.0), (300.0, 44.0), (1000.0, 150.0), (50.0, 7.0), (5.0, 0.6), (0.01, 0.0013)])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_the_whole_curve_of_a_cap(backend, cap, loud, slopes):
+    # products of one sign: logits around the cap and no cancellation that would hide an error of the tanh
+    c = Case(34, [300, 280], 70, 4, 2, 128, cap=cap, q_scale=loud, slopes=slopes)
+    c.q = np.abs(c.q)
+    for x in (c.arrays, c.values):
+        x["k"] = np.abs(x["k"])
+    c.check(backend, "prompt")
+
+
 @pytest.mark.parametrize("scale,cap", [(1e-14, 0.0), (1e-10, 0.0), (3e-5, 1e-4), (20.0, 60.0)])
 def test_extreme_scales_with_a_bias(backend, scale, cap):
     c = Case(33, [300, 290], 70, 4, 2, 128, slopes=True, cap=cap, k_scale=min(1.0, 1e-2 / scale) if scale > 1 else 1.0)
