@@ -165,13 +165,40 @@ def test_many_items_of_few_splits(backend, sessions, rows, heads, kv_heads, hd, 
 
 @pytest.mark.parametrize("cap,loud", [(300.0, 50.0), (300.0, 44.0), (1000.0, 150.0), (50.0, 7.0), (5.0, 0.6), (0.01, 0.0013)])
 @pytest.mark.parametrize("slopes", [False, True])
-def test_the_whole_curve_of_a_cap(backend, cap, loud, slopes):
+@pytest.mark.parametrize("rows,path", [(70, "prompt"), (2, "decode_bf16"), (5, "general")])
+def test_the_whole_curve_of_a_cap(backend, cap, loud, slopes, rows, path):
     # products of one sign: logits around the cap and no cancellation that would hide an error of the tanh
-    c = Case(34, [300, 280], 70, 4, 2, 128, cap=cap, q_scale=loud, slopes=slopes)
+    c = Case(34, [300, 280], rows, 4, 2, 128, cap=cap, q_scale=loud, slopes=slopes)
     c.q = np.abs(c.q)
     for x in (c.arrays, c.values):
         x["k"] = np.abs(x["k"])
-    c.check(backend, "prompt")
+    c.check(backend, path, force_general=path == "general")
+
+
+@pytest.mark.parametrize("fields", [{}, dict(cap=20.0, q_scale=4.0), dict(slopes=True, page=64), dict(ranges=True), dict(ranges=True, cap=9.0, slopes=True)])
+@pytest.mark.parametrize("chunk", [None, 128])
+def test_many_pieces_of_work(backend, fields, chunk):
+    # several pieces for every SM, empty ones and sessions of length 0 among them, against the F32 kernel; its result over
+    # |v| is the weighted mean of |v| that a weight's rounding (half a step of bf16) is a part of
+    fields, rng = dict(fields), np.random.default_rng(35)
+    rows, sessions = 100, 70
+    lengths = rng.integers(0, 420, sessions) * (rng.random(sessions) > 0.2)
+    if fields.pop("ranges", False):
+        end = rng.integers(0, 420, (sessions, rows))
+        fields["ranges"] = (np.maximum(0, end - rng.integers(1, 300, (sessions, rows))) * (rng.random((sessions, rows)) > 0.3), end)
+        fields["ranges"][1][rng.random(sessions) < 0.2] = 0
+
+    c = Case(36, lengths, rows, 8, 2, 128, garbage=False, kv_max=420, **fields)
+
+    def run(general):
+        got, status = c.launch(backend, c.plan(backend, c.problem(backend, general), chunk))
+        assert status == 0
+        return got
+
+    got, again, want = run(False), run(False), run(True)
+    c.arrays["v"] = np.abs(c.arrays["v"])
+    assert np.all(np.abs(got - want) <= 2.0 ** -8 * 1.05 * run(True) + 1e-6)
+    assert np.array_equal(got, again)
 
 
 @pytest.mark.parametrize("scale,cap", [(1e-14, 0.0), (1e-10, 0.0), (3e-5, 1e-4), (20.0, 60.0)])
