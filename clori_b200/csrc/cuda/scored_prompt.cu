@@ -25,10 +25,11 @@
 //
 // Measured, 37 heads x 1024 rows x 4096 tokens, nothing masked: 75 us (1.06 PFLOP/s), with a cap of 50 84, with
 // a bias 97. Two prompts of 8192 capped rows 1.25 ms, 1531-row prompts with a prefix and a cap 173 us (4 of 40 heads),
-// 16384 rows of packed documents with a bias 484 us (32 heads). A pair of tiles takes about 3300 cycles (no cap), of
-// which the products need 2048 and the exponential unit 2048; the rest is the softmax's other instructions and the
-// way between the two. A piece of work costs about 10000 cycles besides its tiles: its first and last tile have no
-// partner and run masks, rows leave, all of it code that the instruction cache has lost since the last piece.
+// 16384 rows of packed documents with a bias 484 us (32 heads). A pair of tiles takes about 3300 cycles without a cap;
+// the products need 2048, the exponential unit 2048. With the softmax's arithmetic taken out the same loop still takes
+// 2800: the one score buffer goes back and forth (products, read, free, products), and tensor memory has no room
+// for a second beside O and P. A piece of work costs about 10000 cycles besides its tiles: its first and last tile
+// have no partner and run masks, rows leave, all of it code that the instruction cache has lost since the last piece.
 #include <type_traits>
 
 #include "scored.cuh"
