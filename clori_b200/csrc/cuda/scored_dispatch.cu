@@ -9,6 +9,15 @@ static int scored_refuse(int code, const char *text)
     return code;
 }
 
+// Tokens a call's rows can see, as far as the host knows: a causal window bounds them.
+static unsigned long long scored_span(const yvx_scored_problem *p)
+{
+    const unsigned long long all = ((unsigned long long)p->kv_tokens_max + 63ull) / 64ull * 64ull;
+    if (!p->window || !p->causal || p->row_end) return all;
+    const unsigned long long seen = (unsigned long long)p->window + p->query_rows + 62ull;
+    return seen < all ? (seen + 63ull) / 64ull * 64ull : all;
+}
+
 static int scored_check(const yvx_scored_problem *p)
 {
     if (!p || !p->query || !p->output || !p->key || !p->value || !p->status)
@@ -32,16 +41,9 @@ static int scored_check(const yvx_scored_problem *p)
         return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: yvx_cuda_scored_plan has not been called");
     if (p->kv_tokens_max > 0x7fffffffu - 1024u || p->sessions > 65535u || p->max_splits > 8192u)
         return scored_refuse(YVEX_ERR_BOUNDS, "scored attention: lengths below 2^31 - 1024, at most 65535 sessions and 8192 splits");
+    if ((unsigned long long)p->chunk_tokens * p->max_splits < scored_span(p))
+        return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: the splits do not cover the tokens: planned for another call");
     return 0;
-}
-
-// Tokens a call's rows can see, as far as the host knows: a causal window bounds them.
-static unsigned long long scored_span(const yvx_scored_problem *p)
-{
-    const unsigned long long all = ((unsigned long long)p->kv_tokens_max + 63ull) / 64ull * 64ull;
-    if (!p->window || !p->causal || p->row_end) return all;
-    const unsigned long long seen = (unsigned long long)p->window + p->query_rows + 62ull;
-    return seen < all ? (seen + 63ull) / 64ull * 64ull : all;
 }
 
 // Caches that the tensor-core kernel does not read in place: codes, and pages that are no multiple of 64 tokens.

@@ -225,7 +225,8 @@ typedef struct yvx_scored_problem {
     int force_general;                        /* 1: the general kernel whatever the shape */
 } yvx_scored_problem;
 /* Splits of the KV sequence for a device with `sm_count` SMs; call it after every other field
- * is set. It depends on the problem's shape, types, strides and alignment only. */
+ * is set. It depends on the problem's shape, types, strides and alignment only; splits that do not
+ * cover kv_tokens_max (or what a causal window leaves of it) are refused. */
 void yvx_cuda_scored_plan(yvx_scored_problem *problem, int sm_count);
 unsigned long long yvx_cuda_scored_workspace_bytes(const yvx_scored_problem *problem);
 /* Enqueues the attention on `stream` (1 to 3 launches, reported in `launches` when given). No

@@ -57,6 +57,7 @@ def scored_problem(**changes):
     (dict(cap=1e-31), abi.YVEX_ERR_INVALID_ARG), (dict(cap=1e-10, scale=1e30), abi.YVEX_ERR_INVALID_ARG),
     (dict(kv_tokens_max=0), abi.YVEX_ERR_INVALID_ARG), (dict(kv_tokens_uniform=101), abi.YVEX_ERR_INVALID_ARG),
     (dict(chunk_tokens=0), abi.YVEX_ERR_INVALID_ARG), (dict(chunk_tokens=100), abi.YVEX_ERR_INVALID_ARG),
+    (dict(kv_tokens_max=200, kv_tokens_uniform=200), abi.YVEX_ERR_INVALID_ARG),  # planned for fewer tokens
     (dict(head_dim=257), abi.YVEX_ERR_UNSUPPORTED), (dict(query_dtype=abi.DTYPE_F16), abi.YVEX_ERR_UNSUPPORTED),
     (dict(kv_dtype=abi.DTYPE_I8), abi.YVEX_ERR_UNSUPPORTED), (dict(kv_code=3), abi.YVEX_ERR_UNSUPPORTED),
     (dict(output_dtype=abi.DTYPE_F64), abi.YVEX_ERR_UNSUPPORTED),
