@@ -377,6 +377,13 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                 keep_lo[u] = (bits & 1u ? 0x0000ffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
                 keep_hi[u] = (bits & 4u ? 0x0000ffffu : 0u) | (bits & 8u ? 0xffff0000u : 0u);
             }
+            if (CODE) {
+                // 16 tokens that no row sees may lie in a page that was never written: its scales count as zero
+                const uint32_t some = __reduce_or_sync(0xffffffffu, seen);
+#pragma unroll
+                for (int u = 0; u < kPair; ++u)
+                    if (!(some >> (4 * u) & 15u)) scales[u] = make_float2(0.0f, 0.0f);
+            }
         }
         // ---- online softmax with a lazy maximum ----------------------------------------------------
         float top[2];
