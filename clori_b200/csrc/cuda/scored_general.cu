@@ -225,6 +225,13 @@ __global__ void __launch_bounds__(kSgThreads) scored_general_kernel(const yvx_sc
     }
 }
 
+// What a split's weight is taken from: its maximum; -inf when it saw nothing. A sum that is NaN (a row saw a NaN) stands
+// above every maximum, which a NaN may not have moved, so that no fold leaves it out: its weight becomes inf - inf.
+__device__ __forceinline__ float scored_split_height(float m, float l)
+{
+    return l == 0.0f ? -INFINITY : l != l ? INFINITY : m;
+}
+
 // One CTA per item. The splits' weights go to shared memory once; then eight warps share the splits, a lane
 // owns four adjacent dims at a time and the rows of four splits are in flight together. Warps are added in
 // order: the result depends on the inputs alone.
@@ -243,8 +250,9 @@ __global__ void __launch_bounds__(kScThreads) scored_combine_kernel(const yvx_sc
     float top = -INFINITY;
     for (unsigned int j = threadIdx.x; j < p.max_splits; j += kScThreads) {
         const float m = parts[j * pitch + hd], l = parts[j * pitch + hd + 1];
-        weight[j] = l == 0.0f ? -INFINITY : m;
-        if (l != 0.0f) top = fmaxf(top, m);
+        const float height = scored_split_height(m, l);
+        weight[j] = height;
+        top = fmaxf(top, height);
     }
     top = warp_max(top);
     if (lane == 0) warp_top[warp] = top;
@@ -315,7 +323,7 @@ __global__ void __launch_bounds__(kScThreads) scored_combine_warp_kernel(const y
     const float *parts = scored_partial(p, item, 0u);
     const unsigned int pitch = hd + 4u;
     const float l = lane < p.max_splits ? parts[lane * pitch + hd + 1] : 0.0f;
-    const float m = l == 0.0f ? -INFINITY : parts[lane * pitch + hd];
+    const float m = l == 0.0f ? -INFINITY : scored_split_height(parts[lane * pitch + hd], l);
     const float top = warp_max(m), weight = m == -INFINITY ? 0.0f : exp2f(m - top), sum = warp_sum(l * weight);
     for (unsigned int d0 = 0; d0 < hd; d0 += 128u) {
         const unsigned int d = d0 + 4u * lane;

@@ -36,3 +36,53 @@ def test_scales_of_pages_that_no_row_sees(backend, cache, page, value, rows, pat
                 for x in ("k_scales", "v_scales"):
                     c.arrays[x][c.table[b, j]] = value
     c.check(backend, path, force_general=path == "general", chunk=chunk)
+
+
+def lonely_nan(c, b, token):
+    """The key of one token becomes NaN; where codes have none, by the scale of its page."""
+    where = c._slot(b, token)
+    if c.cache == I8:
+        c.arrays["k_scales"][where[0]] = np.nan
+    elif c.cache:
+        c.arrays["k"][where] = 0x7f
+    else:
+        c.arrays["k"][where] = np.nan
+
+
+NAN_CACHES = [dict(), dict(page=64), dict(cache=E4M3, page=64), dict(cache=I8, page=64)]
+
+
+@pytest.mark.parametrize("fields", NAN_CACHES)
+@pytest.mark.parametrize("sessions,heads", [(1, 4), (300, 8)])      # a block for each item of the fold, a warp for each
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_a_nan_that_fills_its_split_is_reported(backend, fields, sessions, heads, cap):
+    # the newest token alone in its split of 64
+    lengths = [321] + [65] * (sessions - 1)
+    c = Case(42, lengths, 1, heads, 2, 128, garbage=False, cap=cap, **fields)
+    lonely_nan(c, 0, 320)
+    got, status = c.launch(backend, c.plan(backend, c.problem(backend), 64))
+    assert status == 1 and np.isnan(got[0]).all() and np.isfinite(got[1:]).all()
+
+
+@pytest.mark.parametrize("fields", NAN_CACHES)
+@pytest.mark.parametrize("sessions,heads", [(1, 4), (300, 8)])
+def test_a_query_of_nan_is_reported(backend, fields, sessions, heads):
+    c = Case(43, [321] + [65] * (sessions - 1), 1, heads, 2, 128, garbage=False, **fields)
+    c.q[0, 0, 1, 77] = np.nan
+    got, status = c.launch(backend, c.plan(backend, c.problem(backend), 64))
+    assert status == 1 and np.isnan(got[0, 0, 1]).all() and np.isfinite(got[0, 0, 0]).all() and np.isfinite(got[1:]).all()
+
+
+@pytest.mark.parametrize("sessions,heads", [(1, 4), (300, 8)])
+@pytest.mark.parametrize("rows,general", [(1, False), (1, True), (40, False)])
+def test_a_nan_in_a_split_of_no_weight_is_reported(backend, sessions, heads, rows, general):
+    # the split's finite logits lie hundreds below those of the other splits
+    if rows > 1:
+        sessions = min(sessions, 20)
+    c = Case(44, [322] + [322] * (sessions - 1), rows, heads, 2, 128, garbage=False, causal=False)
+    c.q[:] = 1.0
+    c.arrays["k"][:] = 20.0
+    c.arrays["k"][0, 257:] = -20.0
+    c.arrays["k"][0, 256] = np.nan
+    got, status = c.launch(backend, c.plan(backend, c.problem(backend, general), 128 if rows > 1 else 64))
+    assert status == 1 and np.isnan(got[0]).all() and np.isfinite(got[1:]).all()
