@@ -158,6 +158,13 @@ __device__ __forceinline__ float exp2_approx(float x)
     return y;
 }
 
+__device__ __forceinline__ float log2_approx(float x)
+{
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ float rcp_approx(float x)
 {
     float y;
@@ -184,6 +191,14 @@ __device__ __forceinline__ float min3(float a, float b, float c)
 {
     float r;
     asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// The smaller one; NaN when either is.
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 

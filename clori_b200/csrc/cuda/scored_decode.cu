@@ -9,9 +9,9 @@
 // 5th-generation tensor cores have nothing to win: the memory system is the bound.
 //
 // Codes. A lane of 8 bits becomes an exact f16. A page's K scale multiplies the scores; its V scale
-// multiplies the weights, relative to the largest V scale the warp has met (the accumulator is
-// brought along when that grows), so the operand of P V stays inside f16: the arithmetic of a code
-// costs one conversion and nothing else. Queries are brought to f16 by a power of two per vector
+// multiplies the weights. Each row has a reference of its own for these products, as lazy as the maximum of
+// the scores: the operand of P V stays inside f16 however far the V scales of the pages that different rows
+// see lie apart, and the arithmetic of a code costs one conversion and nothing else. Queries are brought to f16 by a power of two per vector
 // (exact but for lanes below 2^-29 of the vector's largest). The order of head dimensions inside a
 // k-step is free, so a thread takes 32 adjacent dims of its token with two 16-byte reads.
 // Weights: the maximum is lazy, it moves when a score exceeds it by 2^4 (codes) or 2^8, and the
@@ -243,7 +243,9 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
     const bool capped = p.cap > 0.0f, biased = p.slopes != nullptr;
     const float inverse_cap = capped ? 1.0f / p.cap : 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    float v_ref = 1.17549435e-38f, v_inverse = 8.50705917e37f;  // 2^-126: no V scale is smaller and counts
+    // codes: a row's accumulators count in 2^(v_ref - kLift), and its weights are multiplied by v_unit = 2^(m - v_ref) and
+    // the page's V scale on their way to f16
+    float v_ref[2] = {-INFINITY, -INFINITY}, v_unit[2] = {0.0f, 0.0f};
     float o[16][4];
 #pragma unroll
     for (int n = 0; n < 16; ++n)
@@ -386,13 +388,19 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
             }
         }
         // ---- online softmax with a lazy maximum ----------------------------------------------------
-        float top[2];
+        float top[2], of[kPair][2], v_log[kPair];   // the largest score, of each tile; log2 of the tile's V scale
         bool grow = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            top[h] = fmaxf(sc[0][2 * h], sc[0][2 * h + 1]);
+        for (int u = 0; u < kPair; ++u) v_log[u] = CODE ? log2_approx(fabsf(scales[u].y)) : 0.0f;
 #pragma unroll
-            for (int n = 1; n < kCols; ++n) top[h] = max3(top[h], sc[n][2 * h], sc[n][2 * h + 1]);
+        for (int h = 0; h < 2; ++h) {
+            top[h] = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kPair; ++u) {
+                of[u][h] = max3(fmaxf(sc[2 * u][2 * h], sc[2 * u][2 * h + 1]), sc[2 * u + 1][2 * h], sc[2 * u + 1][2 * h + 1]);
+                top[h] = u ? fmaxf(top[h], of[u][h]) : of[u][h];
+                if (CODE) grow = grow || of[u][h] > v_ref[h] + kSlack - v_log[u];
+            }
             grow = grow || top[h] > m[h] + kSlack;   // m is -inf while the row has seen nothing
         }
         if (__any_sync(0xffffffffu, grow)) {
@@ -405,6 +413,18 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                 keep[h] = fresh == -INFINITY ? 1.0f : exp2_approx(m[h] - fresh);
                 m[h] = fresh;
                 l[h] *= keep[h];
+                if (CODE) {
+                    float heavy = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < kPair; ++u) heavy = fmaxf(heavy, of[u][h] + v_log[u]);
+                    heavy = fmaxf(heavy, __shfl_xor_sync(0xffffffffu, heavy, 1));
+                    heavy = fmaxf(heavy, __shfl_xor_sync(0xffffffffu, heavy, 2));
+                    const float next = fmaxf(v_ref[h], heavy);
+                    keep[h] = next == -INFINITY ? 1.0f : exp2_approx(v_ref[h] - next);
+                    v_ref[h] = next;
+                    // (a page of scale 0 may hold the largest score)
+                    v_unit[h] = next == -INFINITY ? 0.0f : exp2_approx(fminf(m[h] - next, 126.0f));
+                }
             }
 #pragma unroll
             for (int n = 0; n < 16; ++n) {
@@ -413,23 +433,6 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                 o[n][2] *= keep[1];
                 o[n][3] *= keep[1];
             }
-        }
-        float ratio[kPair];
-        if (CODE) {
-            float size = fabsf(scales[0].y);
-#pragma unroll
-            for (int u = 1; u < kPair; ++u) size = fmaxf(size, fabsf(scales[u].y));
-            if (size > v_ref) {  // a warp's 16 tokens of a tile share a page: uniform
-                const float factor = v_ref / size;
-#pragma unroll
-                for (int n = 0; n < 16; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[n][e] *= factor;
-                v_ref = size;
-                v_inverse = 1.0f / size;
-            }
-#pragma unroll
-            for (int u = 0; u < kPair; ++u) ratio[u] = scales[u].y * v_inverse;
         }
         float offset[2];
 #pragma unroll
@@ -442,7 +445,8 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                 const float p0 = exp2_approx(sc[n][2 * h] + offset[h]), p1 = exp2_approx(sc[n][2 * h + 1] + offset[h]);
                 l[h] += p0 + p1;
                 if (CODE) {
-                    p_head[n >> 1][2 * (n & 1) + h] = pack_f16(p0 * ratio[n >> 1], p1 * ratio[n >> 1]);
+                    const float times = min_nan(scales[n >> 1].y * v_unit[h], 1e36f);   // weights of 0 stay 0
+                    p_head[n >> 1][2 * (n & 1) + h] = pack_f16(p0 * times, p1 * times);
                 } else {
                     const uint32_t head = pack_bf16(p0, p1);
                     p_head[n >> 1][2 * (n & 1) + h] = head;
@@ -512,18 +516,17 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
     float *merge_o = reinterpret_cast<float *>(ring);                      // [4][16][132]
     float *merge_m = merge_o + kSdWarps * 16 * kSdMergeFloats;             // [4][16]
     float *merge_l = merge_m + kSdWarps * 16;                              // [4][16]
-    const float out_scale = CODE ? v_ref : 1.0f;
+    float *merge_r = CODE ? merge_l + kSdWarps * 16 : merge_m;             // [4][16]: what o counts in
 #pragma unroll
     for (int n = 0; n < 16; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float *row = merge_o + (warp * 16u + g + 8u * h) * kSdMergeFloats;
-            const float x0 = o[n][2 * h] * out_scale, x1 = o[n][2 * h + 1] * out_scale;
             if (CODE) {
-                row[16 * (n >> 1) + 4 * c + (n & 1)] = x0;
-                row[16 * (n >> 1) + 4 * c + 2 + (n & 1)] = x1;
+                row[16 * (n >> 1) + 4 * c + (n & 1)] = o[n][2 * h];
+                row[16 * (n >> 1) + 4 * c + 2 + (n & 1)] = o[n][2 * h + 1];
             } else {
-                *reinterpret_cast<float2 *>(row + 8 * n + 2 * c) = make_float2(x0, x1);
+                *reinterpret_cast<float2 *>(row + 8 * n + 2 * c) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
             }
         }
     if (c == 0) {
@@ -531,6 +534,7 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
         for (int h = 0; h < 2; ++h) {
             merge_m[warp * 16u + g + 8u * h] = m[h] - kLift;
             merge_l[warp * 16u + g + 8u * h] = l[h];
+            if (CODE) merge_r[warp * 16u + g + 8u * h] = v_ref[h] - kLift;
         }
     }
     named_barrier(1, kSdWarps * 32);
@@ -545,7 +549,8 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
             const float mw = merge_m[w * 16 + row];
             const float weight = mw == -INFINITY ? 0.0f : exp2_approx(mw - top);
             sum += merge_l[w * 16 + row] * weight;
-            acc += merge_o[(w * 16 + row) * kSdMergeFloats + d] * weight;
+            const float rw = CODE ? merge_r[w * 16 + row] : mw, of_o = !CODE ? weight : rw == -INFINITY ? 0.0f : exp2_approx(rw - top);
+            acc += merge_o[(w * 16 + row) * kSdMergeFloats + d] * of_o;
         }
         const unsigned long long item = item_of(row);
         if (p.max_splits > 1u) {

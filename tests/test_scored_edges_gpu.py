@@ -86,3 +86,39 @@ def test_a_nan_in_a_split_of_no_weight_is_reported(backend, sessions, heads, row
     c.arrays["k"][0, 256] = np.nan
     got, status = c.launch(backend, c.plan(backend, c.problem(backend, general), 128 if rows > 1 else 64))
     assert status == 1 and np.isnan(got[0]).all() and np.isfinite(got[1:]).all()
+
+
+@pytest.mark.parametrize("cache", [E4M3, I8])
+@pytest.mark.parametrize("apart", [30, 40, 80])
+@pytest.mark.parametrize("chunk", [None, 128, 384])
+def test_scales_of_values_far_apart(backend, cache, apart, chunk):
+    # a document for each tile of 64 tokens, their values 2^30 and more apart, up and down; the last rows see two of them
+    spans = [(64 * i + 3, 64 * i + 60) for i in range(6)] + [(130, 250), (0, 384)]
+    c = Case(45, [384], 8, 2, 2, 128, cache=cache, page=16, ranges=runs(1, spans))
+    power = np.array([0, apart, 0, -apart, apart, -apart])
+    for j in range(24):
+        c.arrays["v_scales"][c.table[0, j]] *= 2.0 ** power[j // 4]
+    c.values["v"][0] *= 2.0 ** np.repeat(power, 64)[:, None, None]
+    c.check(backend, "decode_codes", chunk=chunk)
+
+
+@pytest.mark.parametrize("cache", [E4M3, I8])
+@pytest.mark.parametrize("chunk", [None, 128, 384])
+def test_large_values_of_small_weight(backend, cache, chunk):
+    # one tile in three holds values 2^60 times the others' at a weight of 2^-65: both carry the result
+    c = Case(46, [384], 1, 2, 2, 128, cache=cache, page=16, garbage=False)
+    c.q[:] = 1.0
+    one = 0x38 if cache == E4M3 else 1
+    c.arrays["k"][:] = one
+    c.values["k"][:] = 1.0
+    c.arrays["k_scales"][:] = 4.0
+    c.values["k"] *= 4.0
+    for j in range(24):
+        if j // 4 % 3 == 1:
+            block = c.table[0, j]
+            c.arrays["k"][block] = 0xb8 if cache == E4M3 else 0xff
+            c.arrays["v_scales"][block] *= 2.0 ** 60
+            c.values["k"][0, 16 * j:16 * j + 16] *= -1.0
+            c.values["v"][0, 16 * j:16 * j + 16] *= 2.0 ** 60
+    c.q *= 0.5                                  # logits of +-22.6: weights 2^-65 apart
+    c.check(backend, "decode_codes", chunk=chunk)
