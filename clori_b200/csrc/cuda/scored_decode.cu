@@ -66,9 +66,23 @@ __device__ __forceinline__ void sd_codes(uint32_t word, uint32_t &lo, uint32_t &
     }
 }
 
+// Above this cap the exponential's error, a few 2^-23 of the cap, would count: a few 2^-17 there, as much as the
+// rounding of a bf16 call's weights.
+constexpr float kSdWideCap = 64.0f;
+
+// tanh(x) / x of x^2 for |x| <= 0.6, fitted for this kernel: relative error at most 1.7e-7.
+__device__ __forceinline__ float sd_tanh_ratio(float square)
+{
+    float r = 0.015475619f;
+    r = fmaf(r, square, -0.05210145f);
+    r = fmaf(r, square, 0.13310167f);
+    r = fmaf(r, square, -0.33332309f);
+    return fmaf(r, square, 0.99999994f);
+}
+
 // grid: x = split, y = kv_head * row_tiles + row_tile, z = session. `unit`: tokens of one tiled copy
-// (a page or 64). `head_inner`: the maps order their middle dimensions (head, token).
-template <int CODE>
+// (a page or 64). `head_inner`: the maps order their middle dimensions (head, token). WIDE: the cap is above kSdWideCap.
+template <int CODE, bool WIDE>
 __global__ void __launch_bounds__(kSdThreads, 2)
 scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps maps, const int unit, const int head_inner)
 {
@@ -340,8 +354,9 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
                     float z = sc[n][e] * (mul[e >> 1] * (CODE ? scales[n >> 1].x : 1.0f));
                     if (capped) {
                         // tanh from one exponential: 1 - 2 / (e^2x + 1), absolute error a few 2^-23
-                        const float t = exp2_approx(z * inverse_cap * (2.0f * kScoredLog2e));
-                        z = fmaf(-2.0f * p.cap, rcp_approx(t + 1.0f), p.cap);
+                        const float x = z * inverse_cap, t = exp2_approx(x * (2.0f * kScoredLog2e));
+                        const float curve = fmaf(-2.0f * p.cap, rcp_approx(t + 1.0f), p.cap);
+                        z = WIDE && fabsf(x) <= 0.6f ? z * sd_tanh_ratio(x * x) : curve;
                     }
                     if (biased) {
                         const int distance = position[e >> 1] - (token0 + 64 * (n >> 1) + 8 * (n & 1) + 2 * (int)c + (e & 1));
@@ -637,11 +652,14 @@ int scored_decode_launch(const yvx_scored_problem &p, cudaStream_t stream)
         !scored_encode_rows(&maps.value, p.value, element_bytes, p.value_token_stride, p.value_head_stride,
                             p.value_outer_stride, tokens, p.kv_heads, outer, head_inner, unit, 1u))
         return 0;
-    void (*const kernels[3])(const yvx_scored_problem, const SdMaps, const int, const int) = {
-        scored_decode_kernel<YVX_KV_PLAIN>, scored_decode_kernel<YVX_KV_E4M3>, scored_decode_kernel<YVX_KV_I8>};
-    YVX_CUDA_TRY(cudaFuncSetAttribute((const void *)kernels[p.kv_code], cudaFuncAttributeMaxDynamicSharedMemorySize, kSdSmemBytes));
+    // (in one kernel for both, the choice costs 4 rows over 131072 tokens of codes under a cap 78 -> 82 us)
+    void (*const kernels[6])(const yvx_scored_problem, const SdMaps, const int, const int) = {
+        scored_decode_kernel<YVX_KV_PLAIN, false>, scored_decode_kernel<YVX_KV_E4M3, false>, scored_decode_kernel<YVX_KV_I8, false>,
+        scored_decode_kernel<YVX_KV_PLAIN, true>,  scored_decode_kernel<YVX_KV_E4M3, true>,  scored_decode_kernel<YVX_KV_I8, true>};
+    const auto kernel = kernels[p.kv_code + (p.cap > kSdWideCap ? 3 : 0)];
+    YVX_CUDA_TRY(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSdSmemBytes));
     const dim3 grid(p.max_splits, p.kv_heads * (unsigned int)((vectors + 15ull) / 16ull), p.sessions);
-    kernels[p.kv_code]<<<grid, kSdThreads, kSdSmemBytes, stream>>>(p, maps, (int)unit, head_inner ? 1 : 0);
+    kernel<<<grid, kSdThreads, kSdSmemBytes, stream>>>(p, maps, (int)unit, head_inner ? 1 : 0);
     const int rc = yvx_cuda_check(cudaGetLastError(), "scored_decode_kernel");
     return rc != 0 ? rc : 1;
 }

@@ -122,3 +122,39 @@ def test_large_values_of_small_weight(backend, cache, chunk):
             c.values["v"][0, 16 * j:16 * j + 16] *= 2.0 ** 60
     c.q *= 0.5                                  # logits of +-22.6: weights 2^-65 apart
     c.check(backend, "decode_codes", chunk=chunk)
+
+
+# A logit under a cap may be off by this much of itself: tanh from its exponential or from a polynomial of its own, relative
+# to the result; the prompt kernel's polynomial for small arguments starts with 0.99999061 x.
+CAP_RELATIVE = {"general": 2.0 ** -21, "decode_bf16": 2.0 ** -20, "decode_codes": 2.0 ** -20, "prompt": 2.0 ** -16}
+
+
+def check_cap(c, backend, path):
+    got, status = c.launch(backend, c.plan(backend, c.problem(backend, path == "general")))
+    assert status == 0
+    for b in range(len(c.lengths)):
+        want, spread, size = attention(c.q[b].astype(np.float64), c.values["k"][b], c.values["v"][b], c.position[b], c.first[b],
+                                       c.end[b], float(np.float32(1 / np.sqrt(128))), float(np.float32(c.cap)))
+        visible = np.broadcast_to((c.end - c.first)[b][:, None].astype(np.float64), size.shape)
+        # size bounds |z|; tolerance() takes 2^-20 of its `cap`
+        allowed = tolerance(want, spread, size, visible, 128, WEIGHTS[path], 2.0 ** -24, size * CAP_RELATIVE[path] * 2.0 ** 20)
+        assert np.all(np.abs(got[b] - want) <= allowed), float((np.abs(got[b] - want) / allowed).max())
+
+
+CAPPED = [(2, "decode_bf16", {}), (2, "decode_codes", dict(cache=E4M3, page=16)), (1, "decode_codes", dict(cache=I8, page=64)),
+          (70, "prompt", {}), (3, "general", {})]
+
+
+@pytest.mark.parametrize("cap", [63.0, 65.0, 1e3, 2047.0, 2049.0, 1e5, 1e6, 1e7, 1e30])
+@pytest.mark.parametrize("rows,path,fields", CAPPED)
+def test_moderate_logits_under_a_large_cap(backend, cap, rows, path, fields):
+    check_cap(Case(47, [300, 280], rows, 4, 2, 128, cap=cap, q_scale=3.0, **fields), backend, path)
+
+
+@pytest.mark.parametrize("cap", [1e3, 3e3, 1e5])
+@pytest.mark.parametrize("rows,path,fields", CAPPED)
+def test_one_loud_row_beside_moderate_ones_under_a_large_cap(backend, cap, rows, path, fields):
+    # the loud row's logits leave the part of the curve where tanh x is nearly x, its neighbours' do not
+    c = Case(48, [300, 280], rows, 4, 2, 128, cap=cap, q_scale=2.0, **fields)
+    c.q[:, 0, 1] *= 2.0 ** np.ceil(np.log2(cap))
+    check_cap(c, backend, path if path != "prompt" or cap < 2048 else "general")
