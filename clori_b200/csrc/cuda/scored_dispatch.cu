@@ -65,7 +65,8 @@ static bool scored_prompt_shape(const yvx_scored_problem *p)
     return !p->force_general && p->head_dim == 128u && p->query_dtype == YVEX_DTYPE_BF16 &&
            (p->kv_code != YVX_KV_PLAIN || p->kv_dtype == YVEX_DTYPE_BF16) &&
            (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) > (scored_needs_stage(p) ? 64ull : 32ull) &&
-           !(p->slopes && p->scale < 1e-12f) &&   // that kernel holds the bias in units of the raw product
+           // that kernel holds the mask, and the bias, in units of the raw product unless a cap comes between
+           ((p->cap > 0.0f && !p->slopes) || (p->scale >= 1e-12f && p->scale <= 1e12f)) &&
            p->cap <= 2048.0f &&                   // its tanh from the exponential unit is off by some 2^-22 of the cap
            !((reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value) |
               reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->output) | strides * bytes | q_strides * 2ull) & 15ull);

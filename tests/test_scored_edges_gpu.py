@@ -158,3 +158,25 @@ def test_one_loud_row_beside_moderate_ones_under_a_large_cap(backend, cap, rows,
     c = Case(48, [300, 280], rows, 4, 2, 128, cap=cap, q_scale=2.0, **fields)
     c.q[:, 0, 1] *= 2.0 ** np.ceil(np.log2(cap))
     check_cap(c, backend, path if path != "prompt" or cap < 2048 else "general")
+
+
+@pytest.mark.parametrize("scale,q_scale,k_scale", [(1e-30, 1.0, 1.0), (1e-25, 1e3, 1e3), (1e-13, 1e6, 1e6), (1e30, 2.0 ** -50, 2.0 ** -49),
+                                                  (2e12, 2.0 ** -20, 2.0 ** -20)])
+@pytest.mark.parametrize("rows,fields", [(70, {}), (70, dict(slopes=True)), (70, dict(ranges=True)), (2, {}), (70, dict(cap=20.0)),
+                                         (40, dict(cache=E4M3, page=64))])
+def test_extreme_scales(backend, scale, q_scale, k_scale, rows, fields):
+    fields = dict(fields)
+    if fields.get("ranges"):
+        fields["ranges"] = runs(2, [(3 * i, 3 * i + 60) for i in range(rows)])
+    c = Case(49, [300, 290], rows, 4, 2, 128, q_scale=q_scale, k_scale=k_scale, **fields)
+    p = c.problem(backend)
+    p.scale = scale
+    got, status = c.launch(backend, c.plan(backend, p))
+    assert status == 0
+    slopes = None if c.slope is None else c.slope.astype(np.float64)
+    for b in range(2):
+        want, spread, size = attention(c.q[b].astype(np.float64), c.values["k"][b], c.values["v"][b], c.position[b], c.first[b],
+                                       c.end[b], float(np.float32(scale)), c.cap, slopes)
+        visible = np.broadcast_to((c.end - c.first)[b][:, None].astype(np.float64), size.shape)
+        reach = 0.0 if slopes is None else np.abs(c.position[b])[:, None] * slopes[None, :]
+        assert np.all(np.abs(got[b] - want) <= tolerance(want, spread, size, visible, 128, WEIGHTS["prompt"], 2.0 ** -24, c.cap, reach))
