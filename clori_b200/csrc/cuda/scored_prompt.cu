@@ -17,8 +17,9 @@
 // A thread takes its row's 128 products into registers, and P V of the first 64 starts while the others are
 // exponentiated. The score rule runs two lanes at a time (f32x2 instructions):
 //   cap    tanh(x) = x p(x^2) with p of degree 3 while every |x| of the warp's tile is at most 5/8, of degree 6 up to
-//          11/8, beyond 1 - 2 / (e^2x + 1) from the exponential unit, which is as loaded as the tensor cores. A cap
-//          bounds the logits: up to 55 the weights stay in range against the reference 0 and no maximum is looked for.
+//          11/8, beyond 1 - 2 / (e^2x + 1) from the exponential unit, which is as loaded as the tensor cores. What
+//          decides on the form bounds the logits as well: while the bound is at most 2^32 above the row's reference, no
+//          maximum is looked for.
 //   bias   slope * (s - position) is linear in the token inside a tile: one multiply-add per score and one
 //          constant per row and tile; tokens behind the row's position (prefixes) take |.| in full.
 // Weights are rounded to bf16 (the tensor cores' operand; at most 2^-8 of each), sums and the accumulator are F32.
@@ -43,6 +44,9 @@ constexpr int kSpTileBytes = 2 * kSpHalfBytes;     // 32 KB
 constexpr int kSpOutBytes = 32 * 64;               // a warp's rows on their way out, 64 bytes of each at a time
 constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 8 * kSpOutBytes + 1024 + 6 * 1024;
 constexpr float kSpRescale = 8.0f;                 // log2 units the maximum may lag behind
+// The same where a bound of the tile's logits stands for the maximum: values up to 1e23 stay in F32's range over 131072
+// tokens. Two prompts of 8192 rows under a cap of 50: 1800 us with 16, 1587 with 24, 1557 with 32, 1556 with 48.
+constexpr float kSpNear = 32.0f;
 constexpr uint32_t kSpTmemColumns = 512;           // S 128 | P_A 64 | P_B 64 | O_A 128 | O_B 128
 constexpr int kSpReaders = 11;                     // warps that read a piece of work
 constexpr uint32_t kSpPColumn = 128, kSpOColumn = 256;
@@ -500,9 +504,6 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         // tanh(x) = x (a0 + a1 x^2 + ..).
         const float mul = (CAP ? p.cap : p.scale) * kScoredLog2e;
         const float to_unit = CAP ? p.scale / p.cap : 0.0f;
-        // Under a cap of at most 80 log2 units (55) every row's reference is 0: weights lie in 2^-80 .. 2^80, in range of
-        // F32 and bf16, and no maximum is looked for.
-        const bool fixed = CAP && !BIAS && mul <= 80.0f && mul >= 1e-20f;
         const float inside_small = CAP ? 1.375f / to_unit : 0.0f, unit3 = to_unit * to_unit * to_unit;
         const float last = mul * to_unit * unit3 * unit3;   // what the short polynomial's last coefficient is folded with
         const float inside_tiny = CAP && last >= 1e-34f && last <= 1e30f ? 0.625f / to_unit : -1.0f;
@@ -605,7 +606,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             };
             unsigned long long sum2[2] = {0ull, 0ull};
             // ---- a cap: how large the products are decides on the form of tanh ---------------------------------------
-            bool done = false, small = false;
+            bool done = false, small = false;   // (a cap without a bias: also, whether a maximum is needed)
             if (CAP) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -634,6 +635,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         if (kFolded) power *= to_unit * to_unit;
                     }
                     const unsigned long long unit2 = f2_pack(to_unit, to_unit);
+                    const unsigned long long minus_m2 = f2_pack(-m, -m);
                     landed();
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -650,7 +652,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
 #pragma unroll
                             for (int k = kTerms - 2; k >= 0; --k) r = f2_fma(r, w2, poly2[k]);
                             float e0, e1;
-                            f2_unpack(f2_mul(v, r), e0, e1);
+                            f2_unpack(f2_fma(v, r, minus_m2), e0, e1);
                             e0 = exp2_approx(e0);
                             e1 = exp2_approx(e1);
                             sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(e0, e1));
@@ -659,7 +661,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         hand_over(packed, h);
                     }
                 };
-                if (fixed && small && !cut[0] && !cut[1]) {
+                // |cap tanh x| <= |cap x| bounds every logit of the tile: the reference that the row has will do
+                if (!BIAS && small && !cut[0] && !cut[1] && __all_sync(0xffffffffu, largest * (mul * to_unit) <= m + kSpNear)) {
                     if (__all_sync(0xffffffffu, largest <= inside_tiny)) weights(kSpTanhTiny);
                     else weights(kSpTanhSmall);
                     done = true;
@@ -705,19 +708,13 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         s[c >> 5][c & 31] = __float_as_uint(hide(__uint_as_float(s[c >> 5][c & 31]), c));
                 }
                 const float held = CAP ? 1.0f : mul;
-                float offset = 0.0f;
-                if (fixed) {
-                    landed();
-                } else {
-                    float top[2] = {-INFINITY, -INFINITY};
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 128; i += 2)
-                        top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
-                    const float found = fmaxf(top[0], top[1]);
-                    offset = agree(found < -1e29f ? -INFINITY : fmaf(found, held, slope2 * ahead_f));
-                    // a NaN (or infinity) inside the run: not lost in the mask (under a fixed reference its weight is infinite)
-                    if (found > 1e29f) offset = __int_as_float(0x7fffffff);
-                }
+                for (int i = 0; i < 128; i += 2)
+                    top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
+                const float found = fmaxf(top[0], top[1]);
+                float offset = agree(found < -1e29f ? -INFINITY : fmaf(found, held, slope2 * ahead_f));
+                if (found > 1e29f) offset = __int_as_float(0x7fffffff);   // a NaN (or infinity) inside the run: not lost in the mask
                 const unsigned long long offset2 = f2_pack(offset, offset), held2 = f2_pack(held, held);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -811,7 +808,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                 const unsigned int mine = sh->where[tile_row], my_head = head + (mine >> 16), my_row = q0 + (mine & 0xffffu);
                 const unsigned long long item = ((unsigned long long)b * p.query_rows + my_row) * p.query_heads + my_head;
                 float *part = SPLIT ? scored_partial(p, item, split) : nullptr;
-                if (SPLIT) part[kSpD] = fixed ? 0.0f : m, part[kSpD + 1] = l;
+                if (SPLIT) part[kSpD] = m, part[kSpD + 1] = l;
                 if (!finite) {
                     if (p.row_first || p.row_end) finite = sp_row_again(p, b, my_head, range, my_row, part);
                     if (!finite) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);

@@ -180,3 +180,41 @@ def test_extreme_scales(backend, scale, q_scale, k_scale, rows, fields):
         visible = np.broadcast_to((c.end - c.first)[b][:, None].astype(np.float64), size.shape)
         reach = 0.0 if slopes is None else np.abs(c.position[b])[:, None] * slopes[None, :]
         assert np.all(np.abs(got[b] - want) <= tolerance(want, spread, size, visible, 128, WEIGHTS["prompt"], 2.0 ** -24, c.cap, reach))
+
+
+@pytest.mark.parametrize("cap", [30.0, 54.0])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("power", [60, -90])
+@pytest.mark.parametrize("rows,path,fields", [(130, "prompt", {}), (130, "prompt", dict(ranges=True)), (2, "decode_bf16", {}),
+                                              (2, "decode_codes", dict(cache=E4M3, page=64)), (9, "general", {})])
+@pytest.mark.parametrize("chunk", [None, 128])
+def test_large_and_small_values_under_logits_at_the_cap(backend, cap, sign, power, rows, path, fields, chunk):
+    # every logit near the cap (or near its negative) and values of 10^18 or 10^-27: the answer is a mean of values
+    fields = dict(fields)
+    if fields.get("ranges"):
+        fields["ranges"] = runs(2, [(0, 2 * i + 1) for i in range(rows)])
+    c = Case(50, [400, 390], rows, 4, 2, 128, cap=cap, q_scale=40.0, **fields)
+    c.q = np.abs(c.q)
+    for x in (c.arrays, c.values):
+        if c.cache:
+            continue
+        x["k"] = sign * np.abs(x["k"])
+        x["v"] = x["v"] * np.float32(2.0 ** power)
+    if c.cache:
+        c.arrays["v_scales"] *= 2.0 ** power
+        c.values["v"] *= 2.0 ** power
+    c.check(backend, path, force_general=path == "general", chunk=chunk)
+
+
+def test_logits_that_grow_along_the_sequence_under_a_cap(backend):
+    # a prompt's tiles are walked from the last one: the reference of a row has to follow in both directions
+    for direction in (1, -1):
+        c = Case(51, [1500], 140, 2, 1, 128, cap=54.0, q_scale=1.0)
+        ramp = (np.linspace(-45.0, 45.0, 1500)[::direction, None, None] / np.sqrt(128)).astype(np.float32)
+        c.q[:] = 1.0
+        for x in (c.arrays, c.values):
+            x["k"] = np.where(np.isnan(x["k"]), np.nan, ramp[None] * np.ones_like(x["k"]))
+        rounded = clori_b200.bf16_bits_to_f32(clori_b200.f32_to_bf16_bits(c.arrays["k"].astype(np.float32)))
+        c.arrays["k"] = rounded
+        c.values["k"] = np.nan_to_num(rounded).astype(np.float64)
+        c.check(backend, "prompt")
