@@ -8,10 +8,10 @@ namespace yvx {
 
 constexpr float kScoredLog2e = 1.4426950408889634f;
 
-// Tokens [first, end) and the row's own position.
+// Tokens [first, end), and where the distance bias counts from: the row's own position, or the end of the run that is
+// nearest to it. A row's logits may all move alike, and distances of millions would take their last bits along.
 struct ScoredRange {
-    int first, end;
-    long long position;
+    int first, end, position;
 };
 
 __device__ __forceinline__ long long scored_query_start(const yvx_scored_problem &p, unsigned int b,
@@ -26,15 +26,16 @@ __device__ __forceinline__ ScoredRange scored_range(const yvx_scored_problem &p,
                                                     unsigned int kv_tokens, long long query_start)
 {
     ScoredRange r;
-    r.position = query_start + (long long)row;
+    const long long position = query_start + (long long)row;
     const unsigned long long at = (unsigned long long)b * p.query_rows + row;
     long long first = p.row_first ? (long long)p.row_first[at] : 0;
-    if (p.window) first = max(first, r.position + 1 - (long long)p.window);
-    long long end = p.row_end ? (long long)p.row_end[at] : (p.causal ? r.position + 1 : (long long)kv_tokens);
+    if (p.window) first = max(first, position + 1 - (long long)p.window);
+    long long end = p.row_end ? (long long)p.row_end[at] : (p.causal ? position + 1 : (long long)kv_tokens);
     end = min(max(end, 0ll), (long long)kv_tokens);
     first = min(max(first, 0ll), end);
     r.first = (int)first;
     r.end = (int)end;
+    r.position = (int)max(min(position, end - 1), first);
     return r;
 }
 

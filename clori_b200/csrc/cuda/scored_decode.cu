@@ -244,7 +244,7 @@ scored_decode_kernel(const yvx_scored_problem p, const __grid_constant__ SdMaps 
         if (row < live) {
             const unsigned int v = vector_base + row;
             const ScoredRange r = scored_range(p, b, v / group, kv_tokens, query_start);
-            first[h] = r.first, end[h] = r.end, position[h] = (int)min(r.position, 0x7fffffffll);
+            first[h] = r.first, end[h] = r.end, position[h] = r.position;
             if (p.slopes) slope[h] = p.slopes[kv_head * group + v % group];
             inner_first = max(inner_first, r.first);
             inner_end = min(inner_end, r.end);

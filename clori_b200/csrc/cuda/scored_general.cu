@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kSgThreads) scored_general_kernel(const yvx_sc
         for (int i = 0; i < 4; ++i) {
             float s = z[i] * p.scale;
             if (p.cap > 0.0f) s = p.cap * tanhf(s / p.cap);
-            if (p.slopes) s -= slope[i] * (float)llabs(range[i].position - (long long)t);
+            if (p.slopes) s -= slope[i] * (float)abs(range[i].position - t);
             s = t >= range[i].first && t < range[i].end ? s * kScoredLog2e : -INFINITY;
             // a NaN that a row sees has to reach its result: max() alone would drop it
             const float top = warp_max(s != s ? INFINITY : s);

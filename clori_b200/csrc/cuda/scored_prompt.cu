@@ -42,7 +42,8 @@ constexpr int kSpM = 128, kSpN = 128, kSpD = 128, kSpStages = 2, kSpThreads = 38
 constexpr int kSpHalfBytes = kSpM * 64 * 2;        // [128][64] bf16, swizzled
 constexpr int kSpTileBytes = 2 * kSpHalfBytes;     // 32 KB
 constexpr int kSpOutBytes = 32 * 64;               // a warp's rows on their way out, 64 bytes of each at a time
-constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 8 * kSpOutBytes + 1024 + 6 * 1024;
+constexpr int kSpSharedBytes = 8 * 1024;
+constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 8 * kSpOutBytes + 1024 + kSpSharedBytes;
 constexpr float kSpRescale = 8.0f;                 // log2 units the maximum may lag behind
 // The same where a bound of the tile's logits stands for the maximum: values up to 1e23 stay in F32's range over 131072
 // tokens. Two prompts of 8192 rows under a cap of 50: 1800 us with 16, 1587 with 24, 1557 with 32, 1556 with 48.
@@ -58,11 +59,11 @@ struct SpMaps {
 // One piece of work: two row tiles and what they see. Warp 11 fills it.
 struct SpWork {
     int first[2 * kSpM], end[2 * kSpM];   // visible run of each query row; rows that do not exist see nothing
+    int position[2 * kSpM];               // where its bias counts from
     int hull_first, hull_end;             // of all of them
     int from[2], until[2];                // token tiles [from[x], until[x]) of the two row tiles
     unsigned int q0, head, b, split;      // first query row, first query head
     int valid;                            // 0: nothing is left
-    long long query_start;
 };
 
 struct SpShared {
@@ -75,7 +76,7 @@ struct SpShared {
     unsigned int where[kSpM];             // a tile's row: its query row | its head << 16, or ~0 when it is not used
     SpWork work[2];
 };
-static_assert(sizeof(SpShared) <= 6 * 1024, "the barrier block outgrew its slot");
+static_assert(sizeof(SpShared) <= kSpSharedBytes, "the barrier block outgrew its slot");
 
 // Asks the hardware for a block of the grid that has not started: its index, or "none is left", arrives in *slot.
 __device__ __forceinline__ void sp_ask_block(uint4 *slot, uint64_t *bar)
@@ -175,7 +176,7 @@ __device__ __noinline__ bool sp_row_again(const yvx_scored_problem &p, unsigned 
         for (int d = 0; d < kSpD; ++d) z = fmaf(__bfloat162float(q[d]), __bfloat162float(k[d]), z);
         z *= p.scale;
         if (p.cap > 0.0f) z = p.cap * tanhf(z / p.cap);
-        if (p.slopes) z -= p.slopes[qhead] * (float)llabs(range.position - (long long)t);
+        if (p.slopes) z -= p.slopes[qhead] * (float)abs(range.position - t);
         z *= kScoredLog2e;
         const float fresh = z != z ? INFINITY : fmaxf(m, z);
         const float keep = m == -INFINITY ? 0.0f : exp2f(m - fresh), weight = exp2f(z - fresh);
@@ -460,6 +461,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                                     if (range.first >= range.end) range.first = range.end = 0;
                                 }
                                 w->first[at] = range.first, w->end[at] = range.end;
+                                if (BIAS) w->position[at] = range.position;
                                 if (range.first < range.end) lo = min(lo, range.first), hi = max(hi, range.end);
                             }
                             lo = __reduce_min_sync(0xffffffffu, lo);
@@ -479,8 +481,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     }
                     if (hull_end == 0) hull_first = 0;
                     if (lane == 0)
-                        w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->head = head, w->b = b, w->split = split,
-                        w->query_start = query_start;
+                        w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->head = head, w->b = b, w->split = split;
                     tiles = (hull_end + kSpN - 1) / kSpN - hull_first / kSpN;
                 }
                 if (lane == 0) w->valid = more;
@@ -520,7 +521,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             const unsigned int row = w->q0 + x * tile_rows + at;
             exists = place != ~0u && row < p.query_rows;
             range = {exists ? w->first[x * tile_rows + at] : 0, exists ? w->end[x * tile_rows + at] : 0,
-                     w->query_start + (long long)row};
+                     BIAS ? w->position[x * tile_rows + at] : 0};
             if (BIAS) slope2 = p.slopes[w->head + (exists ? place >> 16 : 0u)] * kScoredLog2e;
         }
         const int hull_first = w->hull_first, hull_end = w->hull_end, my_from = w->from[x], my_until = w->until[x];
@@ -567,8 +568,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             const float up = kHuge * (0.5f - (float)max(lo, -kSpN)), down = kHuge * ((float)min(max(hi, -1), 2 * kSpN) - 0.5f);
             auto hide = [&](float value, int c) { return min3(value, fmaf((float)c, kHuge, up), fmaf((float)c, -kHuge, down)); };
             // the bias of column c: slope * (ahead + c), or -slope * |ahead + c| where a row sees tokens behind itself
-            const int ahead = BIAS ? (int)max(min((long long)k0 - range.position, 0x3fffffffll), -0x3fffffffll) : 0;
-            const bool linear = !BIAS || __all_sync(0xffffffffu, !exists || (long long)min(range.end, k0 + kSpN) <= range.position + 1);
+            const int ahead = BIAS ? k0 - range.position : 0;
+            const bool linear = !BIAS || __all_sync(0xffffffffu, !exists || min(range.end, k0 + kSpN) <= range.position + 1);
             const float ahead_f = BIAS && linear ? (float)ahead : 0.0f;
             // The reference m follows the maximum when it lags by more than 2^8. P of the previous tile is overwritten
             // afterwards, and O may be touched: its P V has to have landed.

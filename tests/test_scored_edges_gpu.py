@@ -218,3 +218,34 @@ def test_logits_that_grow_along_the_sequence_under_a_cap(backend):
         c.arrays["k"] = rounded
         c.values["k"] = np.nan_to_num(rounded).astype(np.float64)
         c.check(backend, "prompt")
+
+
+FAR = [(1, "decode_bf16", {}), (3, "decode_codes", dict(cache=E4M3, page=64)), (70, "prompt", {}), (70, "prompt", dict(cap=20.0)),
+       (50, "prompt", dict(cache=I8, page=16)), (5, "general", {}), (5, "general", dict(cap=9.0, kv_dtype=F32, q_dtype=F32))]
+
+
+def check_far(backend, c, path, chunk):
+    got, status = c.launch(backend, c.plan(backend, c.problem(backend, path == "general"), chunk))
+    assert status == 0
+    for b in range(len(c.lengths)):
+        want, spread, size = attention(c.q[b].astype(np.float64), c.values["k"][b], c.values["v"][b], c.position[b], c.first[b],
+                                       c.end[b], float(np.float32(1 / np.sqrt(128))), c.cap, c.slope.astype(np.float64))
+        visible = (c.end - c.first)[b][:, None].astype(np.float64)
+        # a softmax does not change when a row's logits all move: only distances among the tokens that it sees count
+        allowed = tolerance(want, spread, size, np.broadcast_to(visible, size.shape), 128, WEIGHTS[path], 2.0 ** -24, c.cap,
+                            visible * c.slope[None, :].astype(np.float64))
+        assert np.all(np.abs(got[b] - want) <= allowed), float((np.abs(got[b] - want) / allowed).max())
+
+
+@pytest.mark.parametrize("start", [[2 ** 31 - 200, 2 ** 30 + 77], [2 ** 24 + 5, 70000]])
+@pytest.mark.parametrize("rows,path,fields", FAR)
+@pytest.mark.parametrize("chunk", [None, 128])
+def test_a_bias_far_behind_the_cache(backend, start, rows, path, fields, chunk):
+    check_far(backend, Case(52, [300, 257], rows, 4, 2, 128, slopes=True, query_start=start, **fields), path, chunk)
+
+
+@pytest.mark.parametrize("rows,path,fields", FAR)
+@pytest.mark.parametrize("chunk", [None, 128])
+def test_a_bias_in_front_of_what_a_row_sees(backend, rows, path, fields, chunk):
+    c = Case(53, [700, 650], rows, 4, 2, 128, slopes=True, query_start=[0, 5], ranges=runs(2, [(300 + i, 640) for i in range(rows)]), **fields)
+    check_far(backend, c, path, chunk)
