@@ -61,6 +61,7 @@ struct SpWork {
     int first[2 * kSpM], end[2 * kSpM];   // visible run of each query row; rows that do not exist see nothing
     int position[2 * kSpM];               // where its bias counts from
     int hull_first, hull_end;             // of all of them
+    int solid_end;                        // every token of [hull_first, solid_end) is seen by some row
     int from[2], until[2];                // token tiles [from[x], until[x]) of the two row tiles
     unsigned int q0, head, b, split;      // first query row, first query head
     int valid;                            // 0: nothing is left
@@ -147,54 +148,6 @@ __device__ __forceinline__ void f2_store(unsigned long long v, uint32_t (&s)[32]
 __device__ constexpr float kSpTanhTiny[4] = {0.999987904734053f, -0.33290581616016607f, 0.1292045463446343f, -0.03864439123986797f};
 __device__ constexpr float kSpTanhSmall[7] = {0.9999906071821962f,  -0.3331309371709024f,   0.13205654305843492f, -0.050316830005499996f,
                                               0.016203115118873665f, -0.0035891439879808845f, 0.00038086217121292696f};
-
-// A row of a finite call that came out non-finite: weights of zero met a NaN or infinity in rows of V that
-// this row does not see (between packed documents, say). It is computed again token by token over what it
-// does see, into `part` or as the final row. Rare and slow (a thread per row).
-__device__ __noinline__ bool sp_row_again(const yvx_scored_problem &p, unsigned int b, unsigned int qhead,
-                                          const ScoredRange &range, unsigned int row, float *part)
-{
-    const unsigned int kv_head = qhead / (p.query_heads / p.kv_heads);
-    const __nv_bfloat16 *q = reinterpret_cast<const __nv_bfloat16 *>(p.query) + (unsigned long long)b * p.query_session_stride +
-                             (unsigned long long)row * p.query_row_stride +
-                             (unsigned long long)qhead * (p.query_head_stride ? p.query_head_stride : kSpD);
-    const unsigned long long item = (((unsigned long long)b * p.query_rows + row) * p.query_heads + qhead) * kSpD;
-    float o[kSpD], m = -INFINITY, l = 0.0f;
-    for (int d = 0; d < kSpD; ++d) o[d] = 0.0f;
-    for (int t = range.first; t < range.end; ++t) {
-        unsigned long long outer = b, inner = (unsigned int)t;
-        if (p.block_table) {
-            const int page = scored_page(p, b, (unsigned int)t / p.block_tokens);
-            outer = (unsigned long long)(page < 0 ? 0 : page);
-            inner = (unsigned int)t % p.block_tokens;
-        }
-        const __nv_bfloat16 *k = reinterpret_cast<const __nv_bfloat16 *>(p.key) + outer * p.key_outer_stride +
-                                 inner * p.key_token_stride + kv_head * p.key_head_stride;
-        const __nv_bfloat16 *v = reinterpret_cast<const __nv_bfloat16 *>(p.value) + outer * p.value_outer_stride +
-                                 inner * p.value_token_stride + kv_head * p.value_head_stride;
-        float z = 0.0f;
-        for (int d = 0; d < kSpD; ++d) z = fmaf(__bfloat162float(q[d]), __bfloat162float(k[d]), z);
-        z *= p.scale;
-        if (p.cap > 0.0f) z = p.cap * tanhf(z / p.cap);
-        if (p.slopes) z -= p.slopes[qhead] * (float)abs(range.position - t);
-        z *= kScoredLog2e;
-        const float fresh = z != z ? INFINITY : fmaxf(m, z);
-        const float keep = m == -INFINITY ? 0.0f : exp2f(m - fresh), weight = exp2f(z - fresh);
-        if (z == -INFINITY && fresh == -INFINITY) continue;
-        l = l * keep + weight;
-        for (int d = 0; d < kSpD; ++d) o[d] = fmaf(weight, __bfloat162float(v[d]), o[d] * keep);
-        m = fresh;
-    }
-    bool finite = true;
-    for (int d = 0; d < kSpD; ++d) {
-        const float x = part ? o[d] : l == 0.0f ? 0.0f : o[d] / l;
-        finite = finite && isfinite(x);
-        if (part) part[d] = x;
-        else store_output(p.output, p.output_dtype, item + d, x);
-    }
-    if (part) part[kSpD] = m, part[kSpD + 1] = l;
-    return finite;
-}
 
 // grid: one dimension, the split of the KV sequence slowest. (session, head) lanes in groups whose K and V fit the L2 together; inside a group the
 // pair of row tiles varies slowest, last rows first, and the lane fastest.
@@ -480,8 +433,21 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                                      split + 1u < p.max_splits ? (int)min(t0 + p.chunk_tokens, (long long)hull_end) : hull_end);
                     }
                     if (hull_end == 0) hull_first = 0;
+                    // Runs of the rows may leave gaps. Every pass goes on to the last token that a run reaches from where
+                    // the pass before ended; it ends at the first gap.
+                    int solid_end = hull_end;
+                    if (p.row_first || p.row_end) {
+                        __syncwarp();
+                        int reach = hull_first;
+                        do {
+                            solid_end = reach;
+                            for (unsigned int at = lane; at < 2u * tile_rows; at += 32u)
+                                if (w->first[at] <= solid_end) reach = max(reach, w->end[at]);
+                            reach = __reduce_max_sync(0xffffffffu, reach);
+                        } while (reach > solid_end);
+                    }
                     if (lane == 0)
-                        w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->head = head, w->b = b, w->split = split;
+                        w->solid_end = solid_end, w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->head = head, w->b = b, w->split = split;
                     tiles = (hull_end + kSpN - 1) / kSpN - hull_first / kSpN;
                 }
                 if (lane == 0) w->valid = more;
@@ -524,8 +490,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                      BIAS ? w->position[x * tile_rows + at] : 0};
             if (BIAS) slope2 = p.slopes[w->head + (exists ? place >> 16 : 0u)] * kScoredLog2e;
         }
-        const int hull_first = w->hull_first, hull_end = w->hull_end, my_from = w->from[x], my_until = w->until[x];
-        const int stop = (hull_end + kSpN - 1) / kSpN, start = hull_first / kSpN;
+        const int hull_first = w->hull_first, solid_end = w->solid_end, my_from = w->from[x], my_until = w->until[x];
+        const int stop = (w->hull_end + kSpN - 1) / kSpN, start = hull_first / kSpN;
         const float slope_held = BIAS ? (CAP ? slope2 : slope2 / mul) : 0.0f;
         float m = -INFINITY, l = 0.0f;
         for (int j = my_until - 1; j >= my_from; --j) {
@@ -540,12 +506,23 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             tmem_wait_ld();
             tc_fence_before_sync();
             mbar_arrive(&sh->s_free);   // the other tile's products may come
-            if (k0 < hull_first || k0 + kSpN > hull_end) {
+            if (k0 < hull_first || k0 + kSpN > solid_end) {
                 // tokens that no row of the CTA sees: their rows of V may hold anything and become zero
                 const unsigned int n = tiles + (unsigned int)(stop - 1 - j), stage = n % kSpStages;
                 if (!waited(&sh->v_full[stage], (n / kSpStages) & 1u)) ok = false;
-                const int token = k0 + (int)tile_row;
-                if (token < hull_first || token >= hull_end) {
+                const int token = k0 + (int)tile_row, warp_token = token - (int)lane;
+                bool unseen = token < hull_first || token >= solid_end;
+                if (warp_token < w->hull_end && warp_token + 32 > solid_end) {
+                    // behind a gap: a lane looks which of the warp's 32 tokens some of the rows see
+                    uint32_t some = 0u;
+                    for (unsigned int at = lane; at < 2u * tile_rows; at += 32u) {
+                        const int lo = max(w->first[at] - warp_token, 0), hi = min(w->end[at] - warp_token, 32);
+                        if (lo < hi) some |= (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo);
+                    }
+                    some = __reduce_or_sync(0xffffffffu, some);
+                    unseen = !(some >> lane & 1u);
+                }
+                if (unseen) {
                     unsigned char *v_row = v_smem + stage * kSpTileBytes + tile_row * 128u;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -804,16 +781,13 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                     }
                 }
             }
-            bool finite = check == 0.0f;
             if (exists) {
-                const unsigned int mine = sh->where[tile_row], my_head = head + (mine >> 16), my_row = q0 + (mine & 0xffffu);
-                const unsigned long long item = ((unsigned long long)b * p.query_rows + my_row) * p.query_heads + my_head;
-                float *part = SPLIT ? scored_partial(p, item, split) : nullptr;
-                if (SPLIT) part[kSpD] = m, part[kSpD + 1] = l;
-                if (!finite) {
-                    if (p.row_first || p.row_end) finite = sp_row_again(p, b, my_head, range, my_row, part);
-                    if (!finite) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
+                const unsigned int mine = sh->where[tile_row];
+                if (SPLIT) {
+                    float *part = scored_partial(p, item0 + (unsigned long long)(mine & 0xffffu) * p.query_heads + (mine >> 16), split);
+                    part[kSpD] = m, part[kSpD + 1] = l;
                 }
+                if (check != 0.0f) atomicCAS(p.status, 0, YVX_STATUS_NONFINITE);
             }
         }
         give_back(turn);

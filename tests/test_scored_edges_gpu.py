@@ -249,3 +249,32 @@ def test_a_bias_far_behind_the_cache(backend, start, rows, path, fields, chunk):
 def test_a_bias_in_front_of_what_a_row_sees(backend, rows, path, fields, chunk):
     c = Case(53, [700, 650], rows, 4, 2, 128, slopes=True, query_start=[0, 5], ranges=runs(2, [(300 + i, 640) for i in range(rows)]), **fields)
     check_far(backend, c, path, chunk)
+
+
+@pytest.mark.parametrize("fields", [{}, dict(slopes=True), dict(cap=20.0), dict(cache=E4M3, page=64)])
+@pytest.mark.parametrize("chunk", [None, 1280])
+def test_padding_of_nan_inside_a_long_run(backend, fields, chunk):
+    # few tokens that no row sees between the runs of many rows over a long cache: values and keys there are NaN
+    rows, tokens = 40, 6000
+    spans = [(17 * i, 2900 - i) if i % 2 else (2911 + i, tokens - i) for i in range(rows)]
+    c = Case(54, [tokens], rows, 4, 2, 128, ranges=runs(1, spans), **fields)
+    assert not c.seen[0].all() and c.seen[0, 2950]
+    c.check(backend, "prompt", chunk=chunk)
+
+
+def test_padding_of_infinities_between_documents(backend):
+    rng = np.random.default_rng(55)
+    for trial in range(6):
+        first, end = np.zeros((2, 300), int), np.zeros((2, 300), int)
+        for b in range(2):
+            at = 0
+            while at < 300:
+                n = int(rng.integers(1, 90))
+                first[b, at:at + n], end[b, at:at + n] = at, np.minimum(np.arange(at, at + n) + 1, 300)[:300 - at]
+                at += n + int(rng.integers(0, 40))
+        c = Case(56 + trial, [300, 280], 300, 4, 2, 128, ranges=(first, end))
+        for x in ("k", "v"):
+            bad = np.isnan(c.arrays[x])
+            c.arrays[x][bad] = np.where(rng.random(int(bad.sum())) < 0.5, np.inf, -np.inf)
+        for chunk in (None, 128):
+            c.check(backend, "prompt", chunk=chunk)
