@@ -31,8 +31,6 @@
 // 2800: the one score buffer goes back and forth (products, read, free, products), and tensor memory has no room
 // for a second beside O and P. A piece of work costs about 10000 cycles besides its tiles: its first and last tile
 // have no partner and run masks, rows leave, all of it code that the instruction cache has lost since the last piece.
-#include <type_traits>
-
 #include "scored.cuh"
 #include "tcgen05.cuh"
 
@@ -494,7 +492,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
         const int stop = (w->hull_end + kSpN - 1) / kSpN, start = hull_first / kSpN;
         const float slope_held = BIAS ? (CAP ? slope2 : slope2 / mul) : 0.0f;
         float m = -INFINITY, l = 0.0f;
-        for (int j = my_until - 1; j >= my_from; --j) {
+        for (int j = my_until - 1; ok && j >= my_from; --j) {   // (a wait that gave up is the last one)
             const uint32_t parity = count & 1u;
             ++count;
             const int k0 = j * kSpN;
