@@ -47,6 +47,24 @@ __host__ __device__ __forceinline__ unsigned int scored_packed_heads(const yvx_s
     return group <= 128u ? group : 1u;
 }
 
+// A session's staged rows: all that its rows can see, which a causal window bounds (the same tokens on both sides: from
+// the first row's window on, rounded down to a tile of 128).
+__host__ __device__ __forceinline__ bool scored_stage_windowed(const yvx_scored_problem &p)
+{
+    return p.window && p.causal && !p.row_end &&
+           (unsigned long long)p.window + p.query_rows + 126ull < (unsigned long long)p.kv_tokens_max;
+}
+__host__ __device__ __forceinline__ unsigned long long scored_stage_tokens(const yvx_scored_problem &p)
+{
+    const unsigned long long seen = scored_stage_windowed(p) ? (unsigned long long)p.window + p.query_rows + 126ull : p.kv_tokens_max;
+    return (seen + 63ull) / 64ull * 64ull;
+}
+__device__ __forceinline__ int scored_stage_first(const yvx_scored_problem &p, unsigned int kv_tokens, long long query_start)
+{
+    if (!scored_stage_windowed(p)) return 0;
+    return (int)min(max(query_start + 1 - (long long)p.window, 0ll), (long long)kv_tokens) & ~127;
+}
+
 // The run of tokens that some row of [row0, row1) sees (first == end: none does); all 32 lanes.
 __device__ __forceinline__ void scored_hull(const yvx_scored_problem &p, unsigned int b, unsigned int row0,
                                             unsigned int row1, unsigned int kv_tokens, long long query_start,
@@ -108,8 +126,10 @@ __device__ __forceinline__ void scored_store_empty(const yvx_scored_problem &p, 
 }
 
 int scored_general_launch(const yvx_scored_problem &p, cudaStream_t stream);
-int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream);
+// `staged`: K and V are staged rows; scored_stage_tokens of a session, from scored_stage_first on.
+int scored_prompt_launch(const yvx_scored_problem &p, bool staged, cudaStream_t stream);
 unsigned long long scored_stage_bytes(const yvx_scored_problem &p);
+unsigned int scored_stage_sessions(const yvx_scored_problem &p);
 int scored_stage_launch(const yvx_scored_problem &p, void *rows, yvx_scored_problem *staged, cudaStream_t stream);
 int scored_decode_launch(const yvx_scored_problem &p, cudaStream_t stream);
 int scored_combine_launch(const yvx_scored_problem &p, cudaStream_t stream);

@@ -46,6 +46,25 @@ static int scored_check(const yvx_scored_problem *p)
     return 0;
 }
 
+// The sessions of `whole` from `begin` on, `count` of them, as a call of their own.
+static yvx_scored_problem scored_group(const yvx_scored_problem &whole, unsigned int begin, unsigned int count)
+{
+    yvx_scored_problem p = whole;
+    const unsigned long long rows = (unsigned long long)begin * whole.query_rows, items = rows * whole.query_heads;
+    p.sessions = count;
+    p.query = static_cast<const unsigned char *>(whole.query) +
+              (unsigned long long)begin * whole.query_session_stride * (whole.query_dtype == YVEX_DTYPE_BF16 ? 2ull : 4ull);
+    p.output = static_cast<unsigned char *>(whole.output) + items * whole.head_dim * (whole.output_dtype == YVEX_DTYPE_BF16 ? 2ull : 4ull);
+    p.block_table = whole.block_table + (unsigned long long)begin * whole.block_table_stride;
+    if (whole.kv_tokens) p.kv_tokens += begin;
+    if (whole.query_start) p.query_start += begin;
+    if (whole.row_first) p.row_first += rows;
+    if (whole.row_end) p.row_end += rows;
+    if (whole.workspace)
+        p.workspace = static_cast<unsigned char *>(whole.workspace) + items * whole.max_splits * (whole.head_dim + 4ull) * sizeof(float);
+    return p;
+}
+
 // Caches that the tensor-core kernel does not read in place: codes, and pages that are no multiple of 64 tokens.
 static bool scored_needs_stage(const yvx_scored_problem *p)
 {
@@ -103,8 +122,9 @@ void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
     unsigned long long best = span, best_cost = ~0ull;
     if (yvx::scored_prompt_shape(p)) {
         const unsigned long long heads = yvx::scored_packed_heads(*p), rows = 2ull * (128ull / heads);   // of a piece of work
-        const unsigned long long pieces = p->sessions * (p->query_heads / heads) * ((p->query_rows + rows - 1ull) / rows);
-        const unsigned long long moved = (unsigned long long)p->sessions * p->query_rows * p->query_heads * 1056ull;
+        const unsigned long long together = yvx::scored_needs_stage(p) ? yvx::scored_stage_sessions(*p) : p->sessions;
+        const unsigned long long pieces = together * (p->query_heads / heads) * ((p->query_rows + rows - 1ull) / rows);
+        const unsigned long long moved = together * p->query_rows * p->query_heads * 1056ull;
         for (unsigned long long splits = 1ull; splits <= (span + 127ull) / 128ull && splits <= 8192ull; ++splits) {
             const unsigned long long tiles = ((span + 127ull) / 128ull + splits - 1ull) / splits;
             const unsigned long long cost = (pieces * splits + wave / 2ull - 1ull) / (wave / 2ull) * (tiles + 5ull) +
@@ -133,7 +153,7 @@ void yvx_cuda_scored_plan(yvx_scored_problem *p, int sm_count)
 
 unsigned long long yvx_cuda_scored_workspace_bytes(const yvx_scored_problem *p)
 {
-    if (!p || !p->kv_heads || !p->query_rows) return 0ull;
+    if (!p || !p->kv_heads || !p->query_rows || !p->kv_tokens_max) return 0ull;
     return yvx::scored_partial_bytes(p) +
            (yvx::scored_prompt_shape(p) && yvx::scored_needs_stage(p) ? yvx::scored_stage_bytes(*p) : 0ull);
 }
@@ -143,6 +163,8 @@ int yvx_cuda_scored_attention(const yvx_scored_problem *p, void *stream, unsigne
     if (launches) *launches = 0u;
     int rc = yvx::scored_check(p);
     if (rc != 0) return rc;
+    if (yvx::scored_prompt_shape(p) && yvx::scored_needs_stage(p) && p->kv_heads > 65535u)
+        return yvx::scored_refuse(YVEX_ERR_BOUNDS, "scored attention: more than 65535 KV heads over codes or small pages");
     const unsigned long long needed = yvx_cuda_scored_workspace_bytes(p);
     if (needed && (!p->workspace || p->workspace_bytes < needed || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)))
         return yvx::scored_refuse(YVEX_ERR_BOUNDS, "scored attention: the workspace is missing, misaligned or too small");
@@ -150,13 +172,23 @@ int yvx_cuda_scored_attention(const yvx_scored_problem *p, void *stream, unsigne
     unsigned int count = 0u;
     rc = 0;  // specialised kernels answer 1 when they took the call, 0 when its shape is not theirs
     if (yvx::scored_prompt_shape(p)) {
-        yvx_scored_problem staged = *p;
         if (yvx::scored_needs_stage(p)) {
-            rc = yvx::scored_stage_launch(*p, static_cast<unsigned char *>(p->workspace) + yvx::scored_partial_bytes(p), &staged, s);
-            if (rc != 0) return rc;
-            ++count;
+            unsigned char *rows = static_cast<unsigned char *>(p->workspace) + yvx::scored_partial_bytes(p);
+            const unsigned int together = yvx::scored_stage_sessions(*p);
+            for (unsigned int begin = 0; begin < p->sessions; begin += together) {
+                const yvx_scored_problem group = yvx::scored_group(*p, begin, p->sessions - begin < together ? p->sessions - begin : together);
+                yvx_scored_problem staged;
+                rc = yvx::scored_stage_launch(group, rows, &staged, s);
+                if (rc == 0) rc = yvx::scored_prompt_launch(staged, true, s);
+                if (rc == 0) rc = yvx::scored_general_launch(group, s);
+                if (rc < 0) return rc;
+                count += 2u;
+            }
+            --count;   // the last one is counted below
+            rc = 1;
+        } else {
+            rc = yvx::scored_prompt_launch(*p, false, s);
         }
-        rc = yvx::scored_prompt_launch(staged, s);
     } else if (!p->force_general && (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) <= 64ull) {
         rc = yvx::scored_decode_launch(*p, s);
     }

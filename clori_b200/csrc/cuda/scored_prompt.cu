@@ -59,6 +59,7 @@ struct SpWork {
     int first[2 * kSpM], end[2 * kSpM];   // visible run of each query row; rows that do not exist see nothing
     int position[2 * kSpM];               // where its bias counts from
     int hull_first, hull_end;             // of all of them
+    int staged_first;                     // the token that staged rows begin with
     int solid_end;                        // every token of [hull_first, solid_end) is seen by some row
     int from[2], until[2];                // token tiles [from[x], until[x]) of the two row tiles
     unsigned int q0, head, b, split;      // first query row, first query head
@@ -152,7 +153,7 @@ __device__ constexpr float kSpTanhSmall[7] = {0.9999906071821962f,  -0.333130937
 template <bool CAP, bool BIAS, bool SPLIT>
 __global__ void __launch_bounds__(kSpThreads, 1)
 scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps maps, const int head_inner,
-                     const unsigned int lane_group)
+                     const unsigned int lane_group, const int staged)
 {
     extern __shared__ unsigned char sp_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(sp_raw) + 1023u) & ~uintptr_t(1023));
@@ -229,7 +230,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
             for (unsigned int turn = 0; ok; ++turn) {
                 const SpWork *const w = take(turn);
                 if (w == nullptr) break;
-                const int hull_first = w->hull_first, hull_end = w->hull_end, start = hull_first / kSpN;
+                const int hull_first = w->hull_first, hull_end = w->hull_end, start = hull_first / kSpN, staged_first = w->staged_first;
                 const int stop = (hull_end + kSpN - 1) / kSpN;
                 const unsigned int b = w->b, kv_head = w->head / (p.query_heads / p.kv_heads);
                 if (lane == 0) {
@@ -251,7 +252,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         for (int r = 0; r < 2; ++r) {
                             const int token = j * kSpN + 64 * r;
                             if (token >= hull_end) break;
-                            outer[r] = (int)b, inner[r] = token;
+                            outer[r] = (int)b, inner[r] = token - staged_first;
                             if (p.block_table) {
                                 const int page = token + 64 > hull_first ? scored_page(p, b, (unsigned int)token / p.block_tokens) : 0;
                                 outer[r] = page < 0 ? 0 : page;
@@ -445,7 +446,7 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         } while (reach > solid_end);
                     }
                     if (lane == 0)
-                        w->solid_end = solid_end, w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->head = head, w->b = b, w->split = split;
+                        w->staged_first = staged ? scored_stage_first(p, kv_tokens, query_start) : 0, w->solid_end = solid_end, w->hull_first = hull_first, w->hull_end = hull_end, w->q0 = q0, w->head = head, w->b = b, w->split = split;
                     tiles = (hull_end + kSpN - 1) / kSpN - hull_first / kSpN;
                 }
                 if (lane == 0) w->valid = more;
@@ -802,7 +803,7 @@ bool scored_encode_rows(CUtensorMap *map, const void *base, int element_bytes, u
                         unsigned int box_heads);
 
 // 1: launched, 0: not this kernel's shape, negative: an error.
-int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
+int scored_prompt_launch(const yvx_scored_problem &p, bool staged, cudaStream_t stream)
 {
     const unsigned long long head_stride = p.query_head_stride ? p.query_head_stride : kSpD;
     if (p.head_dim != (unsigned)kSpD || p.query_dtype != YVEX_DTYPE_BF16 || p.kv_code != YVX_KV_PLAIN ||
@@ -812,7 +813,7 @@ int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
     const bool head_inner = p.key_head_stride < p.key_token_stride;
     const unsigned int pack = scored_packed_heads(p), pair_rows = 2u * (kSpM / pack);
     if ((p.value_head_stride < p.value_token_stride) != head_inner) return 0;
-    const unsigned long long tokens = p.block_table ? p.block_tokens : p.kv_tokens_max;
+    const unsigned long long tokens = p.block_table ? p.block_tokens : staged ? scored_stage_tokens(p) : p.kv_tokens_max;
     const unsigned long long outer = p.block_table ? p.pool_blocks : p.sessions;
     SpMaps maps;
     if (!scored_encode_rows(&maps.query, p.query, 2, p.query_row_stride, head_stride, p.query_session_stride, p.query_rows,
@@ -831,7 +832,7 @@ int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
     const unsigned long long ctas = (lanes + lane_group - 1ull) / lane_group * lane_group * pairs * p.max_splits;
     if (lanes > 0xffffffffull || ctas > 0x7fffffffull) return 0;
     const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
-    void (*const kernels[8])(const yvx_scored_problem, const SpMaps, const int, const unsigned int) = {
+    void (*const kernels[8])(const yvx_scored_problem, const SpMaps, const int, const unsigned int, const int) = {
         scored_prompt_kernel<false, false, false>, scored_prompt_kernel<true, false, false>,
         scored_prompt_kernel<false, true, false>,  scored_prompt_kernel<true, true, false>,
         scored_prompt_kernel<false, false, true>,  scored_prompt_kernel<true, false, true>,
@@ -839,7 +840,7 @@ int scored_prompt_launch(const yvx_scored_problem &p, cudaStream_t stream)
     const auto kernel = kernels[(cap ? 1 : 0) + (bias ? 2 : 0) + (p.max_splits > 1u ? 4 : 0)];
     YVX_CUDA_TRY(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpSmemBytes));
     kernel<<<dim3((unsigned int)ctas, 1, 1), kSpThreads, kSpSmemBytes, stream>>>(p, maps, head_inner ? 1 : 0,
-                                                                              (unsigned int)lane_group);
+                                                                              (unsigned int)lane_group, staged ? 1 : 0);
     const int rc = yvx_cuda_check(cudaGetLastError(), "scored_prompt_kernel");
     return rc != 0 ? rc : 1;
 }

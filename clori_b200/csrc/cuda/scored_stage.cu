@@ -8,10 +8,10 @@ namespace yvx {
 
 constexpr int kStThreads = 256;
 
-static unsigned long long stage_tokens(const yvx_scored_problem &p)
-{
-    return ((unsigned long long)p.kv_tokens_max + 63ull) / 64ull * 64ull;
-}
+// Staged rows of at most this many bytes at a time (or one session's): calls of more go through groups of sessions, one after
+// the other in the same workspace. 64 sessions of 512 to 32768 tokens, 17 rows of 32 heads in groups of 4: all together
+// (8.6 GB) 1994 us, in two groups 2090, in four (2 GiB) 2471, whose ends no longer fill the machine.
+constexpr unsigned long long kStBytes = 4ull << 30;
 
 // grid: x = 32 tokens, y = kv_head, z = session. A thread moves 16 lanes of a token's K, then of its V.
 template <int CODE>
@@ -22,7 +22,7 @@ scored_stage_kernel(const yvx_scored_problem p, unsigned short *key, unsigned sh
     const unsigned int kv_tokens = admitted_kv_tokens(p.kv_tokens, b, p.kv_tokens_uniform, p.kv_tokens_max, p.status);
     // Only what the rows see is looked up: pages in front of it may be gone. Without row runs both ends move
     // with the row, so the first and the last row bound them.
-    __shared__ int run[2];
+    __shared__ int run[3];
     if (threadIdx.x < 32u) {
         const long long query_start = scored_query_start(p, b, kv_tokens);
         int first, end;
@@ -32,14 +32,14 @@ scored_stage_kernel(const yvx_scored_problem p, unsigned short *key, unsigned sh
             first = scored_range(p, b, 0u, kv_tokens, query_start).first;
             end = scored_range(p, b, p.query_rows - 1u, kv_tokens, query_start).end;
         }
-        if (threadIdx.x == 0) run[0] = first, run[1] = end;
+        if (threadIdx.x == 0) run[0] = first, run[1] = end, run[2] = scored_stage_first(p, kv_tokens, query_start);
     }
     __syncthreads();
-    const unsigned int token = blockIdx.x * 32u + (threadIdx.x >> 3), d = (threadIdx.x & 7u) * 16u;
+    const unsigned int at = blockIdx.x * 32u + (threadIdx.x >> 3), token = (unsigned int)run[2] + at, d = (threadIdx.x & 7u) * 16u;
     if (token < (unsigned int)run[0] || token >= (unsigned int)run[1]) return;
     const int named = scored_page(p, b, token / p.block_tokens);
     const unsigned long long page = (unsigned long long)(named < 0 ? 0 : named), slot = token % p.block_tokens;
-    const unsigned long long to = (((unsigned long long)b * p.kv_heads + kv_head) * tokens + token) * 128ull + d;
+    const unsigned long long to = (((unsigned long long)b * p.kv_heads + kv_head) * tokens + at) * 128ull + d;
 #pragma unroll
     for (int operand = 0; operand < 2; ++operand) {
         const unsigned long long from = page * (operand ? p.value_outer_stride : p.key_outer_stride) +
@@ -81,19 +81,22 @@ scored_stage_kernel(const yvx_scored_problem p, unsigned short *key, unsigned sh
     }
 }
 
+// Sessions of a group, and the bytes of its staged rows.
+unsigned int scored_stage_sessions(const yvx_scored_problem &p)
+{
+    const unsigned long long fit = kStBytes / (2ull * p.kv_heads * scored_stage_tokens(p) * 128ull * 2ull);
+    return fit < 1ull ? 1u : fit < p.sessions ? (unsigned int)fit : p.sessions;
+}
+
 unsigned long long scored_stage_bytes(const yvx_scored_problem &p)
 {
-    return 2ull * p.sessions * p.kv_heads * stage_tokens(p) * 128ull * 2ull;
+    return 2ull * scored_stage_sessions(p) * p.kv_heads * scored_stage_tokens(p) * 128ull * 2ull;
 }
 
 // Enqueues the staging into `rows` and describes the staged rows.
 int scored_stage_launch(const yvx_scored_problem &p, void *rows, yvx_scored_problem *staged, cudaStream_t stream)
 {
-    if (p.kv_heads > 65535u) {
-        yvx_cuda_set_error_text("scored attention: more than 65535 KV heads");
-        return YVEX_ERR_BOUNDS;
-    }
-    const unsigned long long tokens = stage_tokens(p);
+    const unsigned long long tokens = scored_stage_tokens(p);
     unsigned short *key = reinterpret_cast<unsigned short *>(rows);
     unsigned short *value = key + (unsigned long long)p.sessions * p.kv_heads * tokens * 128ull;
     const dim3 grid((unsigned int)(tokens / 32ull), p.kv_heads, p.sessions);

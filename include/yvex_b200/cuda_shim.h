@@ -228,8 +228,13 @@ typedef struct yvx_scored_problem {
  * is set. It depends on the problem's shape, types, strides and alignment only; splits that do not
  * cover kv_tokens_max (or what a causal window leaves of it) are refused. */
 void yvx_cuda_scored_plan(yvx_scored_problem *problem, int sm_count);
+/* Partial rows of the splits, and for the matrix units' prompt kernel over codes or over pages that are no
+ * multiple of 64 tokens the cache as bf16 rows: 512 bytes for each KV head and token of kv_tokens_max (of
+ * what a causal window without row_end leaves of it), for as many sessions as 4 GiB hold, but for one at
+ * least. */
 unsigned long long yvx_cuda_scored_workspace_bytes(const yvx_scored_problem *problem);
-/* Enqueues the attention on `stream` (1 to 3 launches, reported in `launches` when given). No
+/* Enqueues the attention on `stream` (1 or 2 launches, 2 more for each further group of sessions whose rows
+ * lie in the workspace together; reported in `launches` when given). No
  * allocation and no synchronisation: it may be captured into a graph. Refusals, before anything
  * is enqueued: YVEX_ERR_INVALID_ARG (missing pointers, inconsistent geometry),
  * YVEX_ERR_UNSUPPORTED (types, head_dim above 256), YVEX_ERR_BOUNDS (launch limits, workspace). */

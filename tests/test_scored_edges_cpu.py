@@ -1,0 +1,27 @@
+"""Scored attention, the 8-bit cache and page copies at the edges of what they accept, without a GPU."""
+import ctypes as C
+
+import pytest
+
+from clori_b200 import abi
+from tests.test_scored_cpu import scored_problem
+
+
+def coded_prompt(library, **changes):
+    p = scored_problem(kv_code=abi.KV_E4M3, block_table=4096, key_scales=4096, value_scales=4096, block_tokens=64, pool_blocks=1000,
+                       query_heads=32, kv_heads=8, key_token_stride=128, value_token_stride=128, key_head_stride=64 * 128,
+                       value_head_stride=64 * 128, key_outer_stride=8 * 64 * 128, value_outer_stride=8 * 64 * 128,
+                       query_row_stride=32 * 128, query_session_stride=17 * 32 * 128, **changes)
+    p.block_table_stride = -(-p.kv_tokens_max // 64)
+    library.yvx_cuda_scored_plan(C.byref(p), 148)
+    partial = p.sessions * p.query_rows * 32 * p.max_splits * 132 * 4 if p.max_splits > 1 else 0
+    return library.yvx_cuda_scored_workspace_bytes(C.byref(p)) - partial
+
+
+@pytest.mark.parametrize("sessions,tokens,window,most", [
+    (64, 32768, 0, 4 << 30), (64, 131072, 0, 4 << 30), (64, 32768, 4096, 64 * 8 * 4288 * 512 + 256), (1, 2000, 0, 8 * 2048 * 512 + 256),
+    (3, 1 << 20, 0, 8 * (1 << 20) * 512 + 256), (1, 1 << 20, 1000, 8 * 1152 * 512 + 256), (20000, 1 << 20, 1000, 4 << 30),
+])
+def test_staged_rows_follow_what_the_call_sees(library, sessions, tokens, window, most):
+    staged = coded_prompt(library, sessions=sessions, query_rows=17, kv_tokens_max=tokens, kv_tokens_uniform=tokens, window=window)
+    assert 0 < staged <= most

@@ -278,3 +278,45 @@ def test_padding_of_infinities_between_documents(backend):
             c.arrays[x][bad] = np.where(rng.random(int(bad.sum())) < 0.5, np.inf, -np.inf)
         for chunk in (None, 128):
             c.check(backend, "prompt", chunk=chunk)
+
+
+@pytest.mark.parametrize("chunk", [None, 128])
+@pytest.mark.parametrize("cache,page", [(E4M3, 16), (I8, 64), (PLAIN, 16)])
+@pytest.mark.parametrize("start", [None, [4000, 2980], [0, 2999]])
+def test_staged_rows_of_a_window_begin_where_it_does(backend, cache, page, start, chunk):
+    # sessions much longer than the window; rows at their end, in their middle, at their beginning and behind the cache
+    Case(61, [5000, 3000], 40, 4, 2, 128, cache=cache, page=page, window=300, query_start=start).check(backend, "prompt", chunk=chunk)
+
+
+def test_staged_rows_of_a_window_and_first_tokens(backend):
+    c = Case(62, [3000, 2700], 40, 4, 2, 128, cache=E4M3, page=64, window=500, slopes=True)
+    given = np.tile(np.arange(40) * 20 + 2400, (2, 1))
+    c.first = np.minimum(np.maximum(c.first, given), c.end)
+    p = c.problem(backend)
+    p.row_first = backend.tensor("first", given.astype(np.int32)).data_ptr
+    got, status = c.launch(backend, c.plan(backend, p))
+    want, spread, size = c.answer()
+    assert status == 0 and np.all(np.abs(got - want) <= c.allowed(want, spread, size, "prompt"))
+
+
+@pytest.mark.parametrize("fields", [dict(cache=E4M3, page=64), dict(page=16), dict(cache=I8, page=16, ranges=True, slopes=True, out_dtype=BF16),
+                                    dict(cache=E4M3, page=64, query_start=[100, 50, 0, 200, 10], cap=20.0)])
+def test_sessions_whose_staged_rows_do_not_fit_together(backend, fields):
+    # capacity for 524288 tokens a session: two sessions at a time in a workspace of 4 GiB, three groups
+    fields = dict(fields)
+    if fields.get("ranges"):
+        first = np.random.default_rng(63).integers(0, 100, (5, 70))
+        fields["ranges"] = (first, first + 150)
+    c = Case(64, [300, 129, 0, 257, 64], 70, 8, 8, 128, **fields)
+    c.table = np.pad(c.table, ((0, 0), (0, 524288 // c.page - c.table.shape[1])), constant_values=-1)
+    p = c.problem(backend)
+    p.kv_tokens_max = 524288
+    p = c.plan(backend, p)
+    n = C.c_uint()
+    for _ in range(2):
+        assert backend.lib.yvx_cuda_scored_attention(C.byref(p), backend.stream, C.byref(n)) == 0
+        assert backend.lib.yvx_cuda_stream_synchronize(backend.stream) == 0
+        assert n.value == 3 * 2 + (p.max_splits > 1) and int(c.status.read()[0]) == 0
+        got = c.result()
+        want, spread, size = c.answer()
+        assert np.all(np.abs(got - want) <= c.allowed(want, spread, size, "prompt"))
