@@ -41,6 +41,11 @@ static int scored_check(const yvx_scored_problem *p)
         return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: yvx_cuda_scored_plan has not been called");
     if (p->kv_tokens_max > 0x7fffffffu - 1024u || p->sessions > 65535u || p->max_splits > 8192u)
         return scored_refuse(YVEX_ERR_BOUNDS, "scored attention: lengths below 2^31 - 1024, at most 65535 sessions and 8192 splits");
+    // what the kernels' grids hold, whichever of them runs: refused before the first is enqueued
+    const unsigned long long vectors = (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads);
+    if ((vectors + 15ull) / 16ull * p->kv_heads > 0x7fffffffull ||
+        (p->max_splits > 1u && (unsigned long long)p->sessions * p->query_rows > 0x7fffffffull / p->query_heads))
+        return scored_refuse(YVEX_ERR_BOUNDS, "scored attention: more rows and heads than a grid holds");
     if ((unsigned long long)p->chunk_tokens * p->max_splits < scored_span(p))
         return scored_refuse(YVEX_ERR_INVALID_ARG, "scored attention: the splits do not cover the tokens: planned for another call");
     return 0;

@@ -368,7 +368,6 @@ __global__ void __launch_bounds__(kScThreads) scored_combine_warp_kernel(const y
 int scored_combine_launch(const yvx_scored_problem &p, cudaStream_t stream)
 {
     const unsigned long long items = (unsigned long long)p.sessions * p.query_rows * p.query_heads;
-    if (items > 0x7fffffffull) return YVEX_ERR_BOUNDS;
     // A block for an item has more loads in flight, a warp for an item wastes no threads: 32 items of 32 splits 10.1 us
     // (whole call) against 13.9, 640 of 18 102.1 / 103.7; 2560 of 4 388 / 381, 9600 of 7 209 / 190, 16384 of 2 180 / 143.
     const bool warps = p.max_splits <= 32u && items >= 2048ull;
@@ -391,10 +390,6 @@ int scored_general_launch(const yvx_scored_problem &p, cudaStream_t stream)
 {
     const unsigned long long vectors = (unsigned long long)p.query_rows * (p.query_heads / p.kv_heads);
     const unsigned long long tiles = (vectors + kSgVectors - 1ull) / kSgVectors * p.kv_heads;
-    if (tiles > 0x7fffffffull) {
-        yvx_cuda_set_error_text("scored attention: more (row tile, kv head) pairs than a grid holds");
-        return YVEX_ERR_BOUNDS;
-    }
     const unsigned int hd = p.head_dim;
     const int smem = (int)(sizeof(float) * (kSgVectors * hd + kSgTokens * (hd + 1u) + kSgTokens * hd +
                                             kSgVectors * kSgTokens + 3 * kSgVectors));

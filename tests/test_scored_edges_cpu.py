@@ -25,3 +25,14 @@ def coded_prompt(library, **changes):
 def test_staged_rows_follow_what_the_call_sees(library, sessions, tokens, window, most):
     staged = coded_prompt(library, sessions=sessions, query_rows=17, kv_tokens_max=tokens, kv_tokens_uniform=tokens, window=window)
     assert 0 < staged <= most
+
+
+@pytest.mark.parametrize("changes", [
+    dict(query_rows=2 ** 29, max_splits=2), dict(sessions=60000, query_rows=5000, max_splits=2), dict(query_rows=2 ** 32 - 1, force_general=1),
+    dict(query_rows=2 ** 32 - 1, kv_code=abi.KV_E4M3, block_table=4096, key_scales=4096, value_scales=4096, block_tokens=64,
+         block_table_stride=2, pool_blocks=9),
+])
+def test_calls_beyond_the_grids_are_refused_before_any_launch(library, changes):
+    p, n = scored_problem(workspace_bytes=2 ** 64 - 1, **changes), C.c_uint(7)
+    assert library.yvx_cuda_scored_attention(C.byref(p), None, C.byref(n)) == abi.YVEX_ERR_BOUNDS and n.value == 0
+    assert b"grid" in library.yvx_cuda_last_error_text()
