@@ -62,11 +62,13 @@ static int pages_check(const yvx_kv_pages_args *a)
     unsigned int blocks = 0xffffffffu;
     for (unsigned int i = 0; i < a->pool_count; ++i) {
         const yvx_kv_page_pool &p = a->pools[i];
-        const unsigned long long segment = p.fixed_bytes ? p.fixed_bytes : p.row_bytes * a->block_tokens;
-        if (!p.base || !p.blocks || p.blocks > 0x7fffffffu || !p.segments || !segment ||
-            segment > 0xffffffffffull || (p.segments > 1u && p.segment_stride < segment) ||
-            p.segment_stride > 0xffffffffffull ||
-            p.block_stride < (p.segments - 1ull) * p.segment_stride + segment)
+        // sizes bounded one by one, so that no product below leaves 64 bits
+        const unsigned long long most = 0xffffffffffull;
+        const bool bounded = p.base && p.blocks && p.blocks <= 0x7fffffffu && p.segments && p.row_bytes <= most && p.fixed_bytes <= most &&
+                             p.segment_stride <= most && p.block_stride <= (1ull << 62) / p.blocks;
+        const unsigned long long segment = !bounded ? 0ull : p.fixed_bytes ? p.fixed_bytes : p.row_bytes * a->block_tokens;
+        if (!segment || segment > most || (p.segments > 1u && p.segment_stride < segment) || p.block_stride < segment ||
+            (p.segments > 1u && p.segment_stride > (p.block_stride - segment) / (p.segments - 1ull)))
             return pages_refuse(YVEX_ERR_INVALID_ARG, "kv pages: a pool's strides do not hold its pages");
         if (p.blocks < blocks) blocks = p.blocks;
     }

@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 from clori_b200 import abi
-from tests.test_scored_cpu import scored_problem
+from tests.test_scored_cpu import pages_args, scored_problem
 
 
 def coded_prompt(library, **changes):
@@ -36,3 +36,13 @@ def test_calls_beyond_the_grids_are_refused_before_any_launch(library, changes):
     p, n = scored_problem(workspace_bytes=2 ** 64 - 1, **changes), C.c_uint(7)
     assert library.yvx_cuda_scored_attention(C.byref(p), None, C.byref(n)) == abi.YVEX_ERR_BOUNDS and n.value == 0
     assert b"grid" in library.yvx_cuda_last_error_text()
+
+
+@pytest.mark.parametrize("fields", [
+    dict(row_bytes=2 ** 58 + 1), dict(row_bytes=2 ** 60 + 4, segments=2, segment_stride=256),          # rows x row_bytes is 64 again
+    dict(segments=2 ** 24 + 1, segment_stride=2 ** 40 - 2 ** 16, block_stride=2 ** 62), dict(segments=2 ** 25 + 1, segment_stride=2 ** 39),
+    dict(fixed_bytes=2 ** 41, block_stride=2 ** 42), dict(block_stride=2 ** 61), dict(blocks=2 ** 31 - 1, block_stride=2 ** 40),
+])
+def test_page_sizes_that_leave_64_bits_are_refused(library, fields):
+    a, n = pages_args([], **fields), C.c_uint(5)
+    assert library.yvx_cuda_kv_pages_copy(C.byref(a), None, C.byref(n)) == abi.YVEX_ERR_INVALID_ARG and n.value == 0
