@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(kA8Threads, kA8Resident) kv8_append_kernel(con
         if (threadIdx.x == 0) atomicCAS(a.status, 0, YVX_STATUS_CONTRACT);
         return;
     }
+    if (!fresh) return;   // its pages are neither looked up nor touched: the slot may be idle, its last page shared
     const unsigned long long index = present / a.block_tokens + blockIdx.x;
     const unsigned long long page_start = index * a.block_tokens;
     if (page_start >= present + fresh) return;
