@@ -737,7 +737,8 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                          : 16u * (lane & 3u) + (SPLIT ? reinterpret_cast<unsigned char *>(scored_partial(p, item, split))
                                                       : reinterpret_cast<unsigned char *>(p.output) + item * kSpD * width);
             }
-            float check = l * 0.0f;   // NaN once a lane is not finite
+            // NaN once a lane is not finite, or when all that the row sees fell below the mask's range
+            float check = sees && l == 0.0f ? __int_as_float(0x7fffffff) : l * 0.0f;
             uint4 staged[4];
             auto send = [&](int chunk) {
 #pragma unroll

@@ -320,3 +320,33 @@ def test_sessions_whose_staged_rows_do_not_fit_together(backend, fields):
         got = c.result()
         want, spread, size = c.answer()
         assert np.all(np.abs(got - want) <= c.allowed(want, spread, size, "prompt"))
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("fields", [{}, dict(slopes=True), dict(causal=False)])
+@pytest.mark.parametrize("chunk", [None, 128])
+def test_products_beyond_the_range_of_the_mask_are_reported(backend, sign, fields, chunk):
+    # Q . K of +-2^107 for every token: the prompt kernel says that it cannot weigh them, the others give the mean of V
+    c = Case(65, [300], 70, 4, 2, 128, garbage=False, **fields)
+    c.q[:] = 2.0 ** 50
+    for x in (c.arrays, c.values):
+        x["k"][:] = sign * 2.0 ** 50
+    assert c.launch(backend, c.plan(backend, c.problem(backend), chunk))[1] == 1
+    c = Case(66, [300], 2, 4, 2, 128, garbage=False, causal=False)
+    c.q[:] = 2.0 ** 50
+    for x in (c.arrays, c.values):
+        x["k"][:] = sign * 2.0 ** 50
+    for general in (False, True):
+        got, status = c.launch(backend, c.plan(backend, c.problem(backend, general)))
+        mean = np.repeat(c.values["v"][0].mean(0), 2, axis=0)
+        spread = np.repeat(np.abs(c.values["v"][0]).mean(0), 2, axis=0)
+        assert status == 0 and np.all(np.abs(got[0] - mean) <= spread * (2.0 ** -16 + 300 * 2.0 ** -22))
+
+
+def test_a_loud_negative_token_has_no_weight(backend):
+    c = Case(67, [300], 70, 4, 2, 128, garbage=False)
+    c.q[:] = 2.0 ** 50
+    for x in (c.arrays, c.values):
+        x["k"][:] = 0.0
+        x["k"][0, 3] = -(2.0 ** 50)
+    c.check(backend, "prompt")
