@@ -6,10 +6,11 @@
 // is exact and a lane is rounded once when it is stored (again only if its page's scale grows;
 // e4m3 codes then lose nothing above the subnormal range). Memory bound: an element is read once
 // (2 or 4 bytes) and one byte is written; a thread owns 16 adjacent lanes of a row, so both sides
-// move in 16-byte pieces; the new rows of a page of up to 64 tokens of 128 lanes stay in registers between
-// the two passes. Measured: 4 x 4093 rows of 8 KV heads of 128 bf16 lanes 21.0 us (4.8 TB/s of reads and
+// move in 16-byte pieces; the new rows of a page of up to 64 tokens of 128 bf16 lanes (32 tokens of F32
+// lanes; the others are read again) stay in registers between the two passes. Measured, replayed in a
+// graph (a call adds 3 us): 4 x 4093 rows of 8 KV heads of 128 bf16 lanes 21.2 us (4.8 TB/s of reads and
 // writes; 28.8 us when the second pass read the rows again, 27.9 without the bound on registers, which
-// let half as many blocks be resident); 64 sessions of one row each 3.0 us, a launch.
+// let half as many blocks be resident); 64 sessions of one row each 3.2 us, a launch.
 #include "common.cuh"
 
 namespace yvx {
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kA8Threads, kA8Resident) kv8_append_kernel(con
     const unsigned long long origin = (unsigned long long)b * a.session_stride + (from - present) * a.token_stride +
                                       (unsigned long long)kv_head * a.head_dim;
     // Up to kA8Held pieces of 16 lanes of a thread stay in registers between the two passes (a whole page of 64
-    // tokens of 128 lanes), all loads in flight at once and beside the table's; what is more is read again.
+    // tokens of 128 bf16 lanes, half of one of F32 lanes), all loads in flight at once and beside the table's; what is more is read again.
     const unsigned int pieces = rows * chunks;
     auto piece_at = [&](unsigned int piece) {
         return origin + (unsigned long long)(piece / chunks) * a.token_stride + 16u * (piece % chunks);

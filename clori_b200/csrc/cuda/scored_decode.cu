@@ -18,10 +18,11 @@
 // weights of codes carry a factor 2^11 (at most 2^15): one rounding to 11 bits, full precision down
 // to 2^-25 of the largest. bf16 caches carry a weight as head + tail, 16 bits.
 //
-// Measured: 64 sessions of 512 to 32768 tokens, 8 KV heads, groups of 5, e4m3: 381 us for 2.16 GB (5.7 TB/s; the same
-// copies without the arithmetic 327 us). 131072 tokens of int8 codes, 16 vectors, capped: 73 us for 268 MB (3.7 TB/s;
-// its copies alone 55). 64 sessions behind a window of 4096, bf16 rows, capped: 152 us for 1.0 GB. One session of
-// 4096 tokens, e4m3: 10 us, of which the two launches and their first loads are most. A pass waits for its matrix
+// Measured, a call between events (replayed in a graph): 64 sessions of 512 to 32768 tokens, 8 KV heads, groups of 5, e4m3
+// 433 us (390) for 2.16 GB, the same copies without the arithmetic 327 in a graph. 131072 tokens of int8 codes, 16 vectors,
+// capped: 78 us (76) for 268 MB, its copies alone 55. 64 sessions behind a window of 4096, bf16 rows, capped: 163 us (152)
+// for 1.0 GB. One session of 4096 tokens, e4m3: 12.3 us (10.2), of which the two launches and their first loads are most.
+// A row's own reference for weights times V scales costs 1.5 to 3 % (426 -> 433, 75.7 -> 78). A pass waits for its matrix
 // instructions and conversions (an SM issues in 40 % of its cycles), which two tiles of codes a pass hide in part;
 // with 8 warps an SM has no others to turn to.
 #include "scored.cuh"

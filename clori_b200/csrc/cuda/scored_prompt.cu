@@ -24,9 +24,9 @@
 //          constant per row and tile; tokens behind the row's position (prefixes) take |.| in full.
 // Weights are rounded to bf16 (the tensor cores' operand; at most 2^-8 of each), sums and the accumulator are F32.
 //
-// Measured, 37 heads x 1024 rows x 4096 tokens, nothing masked: 75 us (1.06 PFLOP/s), with a cap of 50 84, with
-// a bias 97. Two prompts of 8192 capped rows 1.25 ms, 1531-row prompts with a prefix and a cap 173 us (4 of 40 heads),
-// 16384 rows of packed documents with a bias 484 us (32 heads). A pair of tiles takes about 3300 cycles without a cap;
+// Measured, calls between events with the L2 flushed before: 37 heads x 1024 rows x 4096 tokens, nothing masked, 82 us
+// (75 in a loop: 1.06 PFLOP/s), with a cap of 50 92, with a bias 100; two prompts of 8192 capped rows 1.56 ms, 1531-row prompts with a prefix and a cap 190 us
+// (4 of 40 heads), 16384 rows of packed documents with a bias 485 us (32 heads). A pair of tiles takes about 3300 cycles without a cap;
 // the products need 2048, the exponential unit 2048. With the softmax's arithmetic taken out the same loop still takes
 // 2800: the one score buffer goes back and forth (products, read, free, products), and tensor memory has no room
 // for a second beside O and P. A piece of work costs about 10000 cycles besides its tiles: its first and last tile

@@ -1,7 +1,7 @@
 // Pages of codes (or small pages of bf16) laid out as bf16 rows [session][kv_head][token][128] for the
 // prompt-sized attention kernel. Values of a power-of-two scale are exact in bf16; others are rounded once.
-// Memory bound: 1 byte read and 2 written per lane, 150 us for 131072 tokens of 8 KV heads (5.4 TB/s), a small part
-// of a prompt's attention.
+// Memory bound: 1 byte read and 2 written per lane, 150 us for 131072 tokens of 8 KV heads (5.4 TB/s): a small part of a
+// long prompt's attention, more than half of a call of 17 rows.
 #include "scored.cuh"
 
 namespace yvx {

@@ -497,7 +497,8 @@ int yvex_b200_kv_pool_session_truncate(yvex_b200_kv_pool *pool, unsigned int ses
 /* Moves the blocks in use to the front: afterwards they are [0, blocks in use), every session's table says
  * so, and the pools may be cut or handed back behind them. `copies` receives the whole-block copies that
  * the caller makes in every layer's pools (yvex_b200_kv_pages_copy_execute) before it uses a table again;
- * no copy's source or destination is another's destination. *count is their number; when `capacity` is too
+ * copies that a reserve reported are made before the call. No copy's source or destination is another's
+ * destination. *count is their number; when `capacity` is too
  * small it still is, nothing changes, and the call is YVEX_ERR_BOUNDS. */
 int yvex_b200_kv_pool_compact(yvex_b200_kv_pool *pool, yvex_b200_kv_copy *copies, unsigned int capacity,
                               unsigned int *count);

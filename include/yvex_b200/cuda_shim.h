@@ -175,10 +175,13 @@ int yvx_cuda_gqa_attention_profiled(const yvx_gqa_problem *problem, void *stream
  * both clipped to [0, kv_tokens[b]]. Packed documents, padding, bidirectional prefixes and
  * any other mask whose rows see one run of tokens are such arrays
  * (yvex_b200_attention_row_ranges writes the usual ones). A row that sees nothing is written
- * as zeros, and what lies in K and V where no row looks (beyond a session's length, in the
- * rest of a page, in padding) may be anything, NaN included. A NaN that a row does see is
- * reported in the status word (1), and so is an infinity or a product Q . K beyond 1e29 unless
- * the cap or a weight of zero takes it away.
+ * as zeros, and what lies in K, V and the scales of pages where no row looks (beyond a session's
+ * length, in the rest of a page, in padding between runs) may be anything, NaN included. The
+ * block table names a page for every token between the first and the last that some row of the
+ * session sees; entries in front of and behind them may be anything. A NaN that a row sees in
+ * Q or K is reported in the status word (1); so is one in V, an infinity, or a product Q . K
+ * beyond 1e29, unless the cap or a weight of zero takes it away. Other rows of a call that
+ * reports one may be non-finite too.
  *
  * kv_code != YVX_KV_PLAIN: key and value are 8-bit codes in pages (block_table is required;
  * strides are in bytes) and a lane stands for code * scale, with one float scale for each
@@ -188,9 +191,14 @@ int yvx_cuda_gqa_attention_profiled(const yvx_gqa_problem *problem, void *stream
  * Everything is accumulated in F32. On the matrix units (head_dim 128 and bf16 queries) the
  * weights of the softmax are rounded once: to 8 bits, like their operands, in calls of more than
  * 32 vectors (query rows x heads of a KV head; 64 over codes or pages that are no multiple of 64
- * tokens), else to 16 bits (bf16) or 11 bits (codes); other shapes run in F32 throughout.
- * Results repeat bit for bit. Offsets are 64 bits wide; lengths are below 2^31 - 1024, positions
- * below 2^31. */
+ * tokens), else to 16 bits (bf16) or 11 bits (codes; a weight times its page's V scale that is
+ * below 2^-25 of the row's largest keeps steps of 2^-35 of that); other shapes run in F32
+ * throughout. In the calls rounded to 8 bits a code times a scale that is no power of two is
+ * rounded to bf16 as well, and weights reach 2^32 before they are divided: |V| up to 1e23 has room
+ * over 131072 tokens. Calls with a cap above 2048 or a scale outside 1e-12 .. 1e12 (but under a cap
+ * without slopes) take the kernels of few vectors up to 64, F32 throughout beyond. Over codes the
+ * V scales of a session and head lie within 2^100 of one another. Results repeat bit for bit.
+ * Offsets are 64 bits wide; lengths are below 2^31 - 1024, positions below 2^31. */
 typedef enum { YVX_KV_PLAIN = 0, YVX_KV_E4M3 = 1, YVX_KV_I8 = 2 } yvx_kv_code;
 typedef struct yvx_scored_problem {
     unsigned int sessions, query_rows;        /* rows per session (uniform) */
@@ -233,9 +241,9 @@ void yvx_cuda_scored_plan(yvx_scored_problem *problem, int sm_count);
  * what a causal window without row_end leaves of it), for as many sessions as 4 GiB hold, but for one at
  * least. */
 unsigned long long yvx_cuda_scored_workspace_bytes(const yvx_scored_problem *problem);
-/* Enqueues the attention on `stream` (1 or 2 launches, 2 more for each further group of sessions whose rows
- * lie in the workspace together; reported in `launches` when given). No
- * allocation and no synchronisation: it may be captured into a graph. Refusals, before anything
+/* Enqueues the attention on `stream`, in 1 to 3 launches, 2 more for each further group of sessions
+ * whose rows lie in the workspace together (reported in `launches` when given). No allocation and no
+ * synchronisation: it may be captured into a graph. Refusals, before anything
  * is enqueued: YVEX_ERR_INVALID_ARG (missing pointers, inconsistent geometry),
  * YVEX_ERR_UNSUPPORTED (types, head_dim above 256), YVEX_ERR_BOUNDS (launch limits, workspace). */
 int yvx_cuda_scored_attention(const yvx_scored_problem *problem, void *stream, unsigned int *launches);
@@ -245,10 +253,12 @@ int yvx_cuda_scored_attention(const yvx_scored_problem *problem, void *stream, u
  * block_table names, K and V alike. Per page and head the scale is the smallest power of two
  * s >= 2^-126 with max|x| <= s * limit over the page's new rows (limit 448 for e4m3, 127 for
  * integers); a page that held rows keeps its scale when that is larger, else its old codes are
- * brought to the new scale. Codes are rounded to nearest even; divisions by s are exact. What a
- * page holds behind the last row is left as it was. A lane that is not finite is stored as 0
- * and recorded in the status word (1); a table entry outside the pool, or a session whose rows do
- * not fit its table row, is recorded (2) and skipped. A page belongs to one session of a call: a
+ * brought to the new scale (rows that are given up again, rejected drafts say, leave it grown).
+ * Codes are rounded to nearest even; divisions by s are exact. Sessions without new rows are left
+ * alone, their table rows are not read. What a page holds behind the last row is left as it was.
+ * A lane that is not finite is stored as 0 and recorded in the status word (1); a table entry
+ * outside the pool, or a session whose rows do not fit its table row, is recorded (2) and skipped.
+ * A page belongs to one session of a call: a
  * shared one is copied first (yvex_b200_kv_pool_reserve). No counterpart in the reference. */
 typedef struct yvx_kv8_append_args {
     unsigned int sessions, tokens;            /* tokens: the largest number of new rows of a session */
