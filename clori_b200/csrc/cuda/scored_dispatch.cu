@@ -91,7 +91,7 @@ static bool scored_prompt_shape(const yvx_scored_problem *p)
            (unsigned long long)p->query_rows * (p->query_heads / p->kv_heads) > (scored_needs_stage(p) ? 64ull : 32ull) &&
            // that kernel holds the mask, and the bias, in units of the raw product unless a cap comes between
            ((p->cap > 0.0f && !p->slopes) || (p->scale >= 1e-12f && p->scale <= 1e12f)) &&
-           p->cap <= 2048.0f &&                   // its tanh from the exponential unit is off by some 2^-22 of the cap
+           p->cap <= 1e36f &&                     // and the cap in log2 units
            !((reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value) |
               reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->output) | strides * bytes | q_strides * 2ull) & 15ull);
 }

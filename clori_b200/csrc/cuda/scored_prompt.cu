@@ -42,6 +42,7 @@ constexpr int kSpTileBytes = 2 * kSpHalfBytes;     // 32 KB
 constexpr int kSpOutBytes = 32 * 64;               // a warp's rows on their way out, 64 bytes of each at a time
 constexpr int kSpSharedBytes = 8 * 1024;
 constexpr int kSpSmemBytes = (2 + 2 * kSpStages) * kSpTileBytes + 8 * kSpOutBytes + 1024 + kSpSharedBytes;
+constexpr float kSpWideCap = 2048.0f;              // the exponential unit's tanh is off by some 2^-22 of the cap: 5e-4 here
 constexpr float kSpRescale = 8.0f;                 // log2 units the maximum may lag behind
 // The same where a bound of the tile's logits stands for the maximum: values up to 1e23 stay in F32's range over 131072
 // tokens. Two prompts of 8192 rows under a cap of 50: 1800 us with 16, 1587 with 24, 1557 with 32, 1556 with 48.
@@ -150,7 +151,8 @@ __device__ constexpr float kSpTanhSmall[7] = {0.9999906071821962f,  -0.333130937
 
 // grid: one dimension, the split of the KV sequence slowest. (session, head) lanes in groups whose K and V fit the L2 together; inside a group the
 // pair of row tiles varies slowest, last rows first, and the lane fastest.
-template <bool CAP, bool BIAS, bool SPLIT>
+// WIDE: a cap above kSpWideCap, under which a logit that is small beside the cap keeps its accuracy whatever its tile holds.
+template <bool CAP, bool BIAS, bool SPLIT, bool WIDE>
 __global__ void __launch_bounds__(kSpThreads, 1)
 scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps maps, const int head_inner,
                      const unsigned int lane_group, const int staged)
@@ -662,9 +664,14 @@ scored_prompt_kernel(const yvx_scored_problem p, const __grid_constant__ SpMaps 
                         }
                     } else {
 #pragma unroll
-                        for (int c = 0; c < 128; ++c)
-                            s[c >> 5][c & 31] = __float_as_uint(fmaf(
-                                -2.0f * mul, rcp_approx(exp2_approx(__uint_as_float(s[c >> 5][c & 31]) * to_exp) + 1.0f), mul));
+                        for (int c = 0; c < 128; ++c) {
+                            const float value = __uint_as_float(s[c >> 5][c & 31]), x = value * to_unit;
+                            const float curve = fmaf(-2.0f * mul, rcp_approx(exp2_approx(value * to_exp) + 1.0f), mul);
+                            float r = kSpTanhSmall[6];
+#pragma unroll
+                            for (int k = 5; k >= 0; --k) r = fmaf(r, x * x, kSpTanhSmall[k]);
+                            s[c >> 5][c & 31] = __float_as_uint(WIDE && fabsf(x) <= 1.375f ? x * mul * r : curve);
+                        }
                     }
                 }
                 if (BIAS) {
@@ -833,12 +840,13 @@ int scored_prompt_launch(const yvx_scored_problem &p, bool staged, cudaStream_t 
     const unsigned long long ctas = (lanes + lane_group - 1ull) / lane_group * lane_group * pairs * p.max_splits;
     if (lanes > 0xffffffffull || ctas > 0x7fffffffull) return 0;
     const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
-    void (*const kernels[8])(const yvx_scored_problem, const SpMaps, const int, const unsigned int, const int) = {
-        scored_prompt_kernel<false, false, false>, scored_prompt_kernel<true, false, false>,
-        scored_prompt_kernel<false, true, false>,  scored_prompt_kernel<true, true, false>,
-        scored_prompt_kernel<false, false, true>,  scored_prompt_kernel<true, false, true>,
-        scored_prompt_kernel<false, true, true>,   scored_prompt_kernel<true, true, true>};
-    const auto kernel = kernels[(cap ? 1 : 0) + (bias ? 2 : 0) + (p.max_splits > 1u ? 4 : 0)];
+    typedef void (*Kernel)(const yvx_scored_problem, const SpMaps, const int, const unsigned int, const int);
+    const Kernel kernels[4][3] = {   // without a cap, with one, with a wide one
+        {scored_prompt_kernel<false, false, false, false>, scored_prompt_kernel<true, false, false, false>, scored_prompt_kernel<true, false, false, true>},
+        {scored_prompt_kernel<false, true, false, false>, scored_prompt_kernel<true, true, false, false>, scored_prompt_kernel<true, true, false, true>},
+        {scored_prompt_kernel<false, false, true, false>, scored_prompt_kernel<true, false, true, false>, scored_prompt_kernel<true, false, true, true>},
+        {scored_prompt_kernel<false, true, true, false>, scored_prompt_kernel<true, true, true, false>, scored_prompt_kernel<true, true, true, true>}};
+    const Kernel kernel = kernels[(bias ? 1 : 0) + (p.max_splits > 1u ? 2 : 0)][cap ? p.cap > kSpWideCap ? 2 : 1 : 0];
     YVX_CUDA_TRY(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpSmemBytes));
     kernel<<<dim3((unsigned int)ctas, 1, 1), kSpThreads, kSpSmemBytes, stream>>>(p, maps, head_inner ? 1 : 0,
                                                                               (unsigned int)lane_group, staged ? 1 : 0);

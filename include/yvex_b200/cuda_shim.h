@@ -195,8 +195,8 @@ int yvx_cuda_gqa_attention_profiled(const yvx_gqa_problem *problem, void *stream
  * below 2^-25 of the row's largest keeps steps of 2^-35 of that); other shapes run in F32
  * throughout. In the calls rounded to 8 bits a code times a scale that is no power of two is
  * rounded to bf16 as well, and weights reach 2^32 before they are divided: |V| up to 1e23 has room
- * over 131072 tokens. Calls with a cap above 2048 or a scale outside 1e-12 .. 1e12 (but under a cap
- * without slopes) take the kernels of few vectors up to 64, F32 throughout beyond. Over codes the
+ * over 131072 tokens. Calls with a scale outside 1e-12 .. 1e12 (but under a cap without slopes) or a
+ * cap above 1e36 take the kernels of few vectors up to 64, F32 throughout beyond. Over codes the
  * V scales of a session and head lie within 2^100 of one another. Results repeat bit for bit.
  * Offsets are 64 bits wide; lengths are below 2^31 - 1024, positions below 2^31. */
 typedef enum { YVX_KV_PLAIN = 0, YVX_KV_E4M3 = 1, YVX_KV_I8 = 2 } yvx_kv_code;
